@@ -1,0 +1,171 @@
+// C-ABI of attention over a paged KV cache. Declarations: include/clef_fused.h. Same contract as the other entry
+// points: asynchronous on the caller's stream, no allocation (the caller gives the workspace), no synchronisation,
+// grids that depend on the shape arguments only.
+
+#include "../../include/clef_fused.h"
+
+#include <atomic>
+#include <type_traits>
+
+#include "abi_support.cuh"
+#include "kernels_attention.cuh"
+
+using namespace clef;
+using namespace clef::abi;
+
+namespace {
+
+constexpr int kAttnMaxCtas = 320;     // two per SM of 160: the workspace does not depend on the device
+constexpr int kAttnMaxGroup = 64;
+
+struct AttnPlan {
+    int rows;            // R: rows of a row tile
+    size_t items;        // bound on the (sequence, kv head, row tile) triples
+    size_t bytes;        // of the workspace
+};
+
+AttnPlan attn_plan(int n_seqs, int total_q, int q_heads, int kv_heads, int head_dim) {
+    AttnPlan p;
+    const long long rows = (long long)total_q * (q_heads / kv_heads);
+    p.rows = rows > 8LL * n_seqs ? 16 : 8;
+    p.items = ((size_t)(rows / p.rows) + n_seqs) * kv_heads;
+    p.bytes = (size_t)kAttnMaxCtas * 2 * (sizeof(int4) + (size_t)p.rows * (head_dim + 2) * sizeof(float));
+    return p;
+}
+
+// Raises a kernel's dynamic shared memory limit, once per device.
+template <typename K>
+int allow_smem(K kernel, size_t bytes, std::atomic<unsigned long long>& done, const char* what) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && !(done.load(std::memory_order_relaxed) >> dev & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    return e == cudaSuccess ? CLEF_OK : fail(CLEF_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+template <typename T, bool FP8, int D, int NT>
+int launch_rows(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const AttnPlan& plan, const char* what) {
+    constexpr int R = 8 * NT;
+    constexpr size_t smem = (size_t)(kAttnThreads / 32) * R * (D + 4 + 2) * sizeof(float);
+    static std::atomic<unsigned long long> allowed{0};
+    static std::atomic<int> occ{0};
+    auto kernel = attn_rows_kernel<T, FP8, D, NT>;
+    if (int r = allow_smem(kernel, smem, allowed, what)) return r;
+    const size_t key_tiles = ((size_t)a.table_width * a.page_size + kAttnKeys - 1) / kAttnKeys;
+    size_t most = (size_t)dev.sms * ctas_per_sm(kernel, smem, occ);
+    if (most > kAttnMaxCtas) most = kAttnMaxCtas;
+    const unsigned ctas = clamp_grid(plan.items * key_tiles, most);
+    launch_hot(kernel, ctas, smem, s, a);
+    if (int r = check_launch(what)) return r;
+    if (key_tiles <= 1 || ctas <= 1) return CLEF_OK;   // no row tile has been cut
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(clamp_grid(plan.items, ctas), R, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    (void)cudaLaunchKernelEx(&cfg, attn_combine_kernel<T, D, R>, a, (int)ctas);
+    return check_launch(what);
+}
+
+template <typename T, bool FP8>
+int launch_attention(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const AttnPlan& plan, int head_dim,
+                     const char* what) {
+#define CLEF_ATTN_ROWS(D) \
+    return plan.rows == 8 ? launch_rows<T, FP8, D, 1>(s, dev, a, plan, what) : launch_rows<T, FP8, D, 2>(s, dev, a, plan, what);
+    if (head_dim == 64) {
+        CLEF_ATTN_ROWS(64)
+    } else if (head_dim == 128) {
+        CLEF_ATTN_ROWS(128)
+    } else {
+        CLEF_ATTN_ROWS(256)
+    }
+#undef CLEF_ATTN_ROWS
+}
+
+int check_attention_shape(const char* what, int n_seqs, int total_q, int q_heads, int kv_heads, int head_dim) {
+    if (n_seqs < 0 || total_q < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0) {
+        return fail(CLEF_ERR_INVALID, "%s: n_seqs %d total_q %d q_heads %d kv_heads %d (q_heads a multiple of kv_heads)", what,
+                    n_seqs, total_q, q_heads, kv_heads);
+    }
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) {
+        return fail(CLEF_ERR_INVALID, "%s: head_dim %d (64, 128 and 256 are served)", what, head_dim);
+    }
+    const int group = q_heads / kv_heads;
+    if (group > kAttnMaxGroup) return fail(CLEF_ERR_TOO_LARGE, "%s: %d query heads per kv head, above %d", what, group, kAttnMaxGroup);
+    if ((long long)total_q * group >= 0x40000000LL || (long long)n_seqs * kv_heads >= 0x40000000LL) {
+        return fail(CLEF_ERR_TOO_LARGE, "%s: total_q %d x %d heads, %d sequences", what, total_q, q_heads, n_seqs);
+    }
+    return CLEF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int clef_paged_attention_workspace(int n_seqs, int total_q, int q_heads, int kv_heads, int head_dim, size_t* bytes) {
+    const char* what = "clef_paged_attention_workspace";
+    if (!bytes) return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
+    if (int r = check_attention_shape(what, n_seqs, total_q, q_heads, kv_heads, head_dim)) return r;
+    *bytes = n_seqs == 0 || total_q == 0 ? 0 : attn_plan(n_seqs, total_q, q_heads, kv_heads, head_dim).bytes;
+    return CLEF_OK;
+}
+
+int clef_paged_attention(clef_stream_t stream, void* out, const void* q, const void* cache_k, const void* cache_v,
+                         const float* k_scales, const float* v_scales, const int32_t* page_table, const int32_t* q_start,
+                         const int32_t* kv_len, int n_seqs, int total_q, int q_heads, int kv_heads, int head_dim,
+                         int page_size, int table_width, int cache_pages, float scale, void* workspace,
+                         size_t workspace_bytes, int cache_dtype, int dtype) {
+    const char* what = "clef_paged_attention";
+    if (int r = check_dtype(dtype, what)) return r;
+    if (cache_dtype != CLEF_BF16 && cache_dtype != CLEF_E4M3) {
+        return fail(CLEF_ERR_INVALID, "%s: cache_dtype %d is neither CLEF_BF16 nor CLEF_E4M3", what, cache_dtype);
+    }
+    if (int r = check_attention_shape(what, n_seqs, total_q, q_heads, kv_heads, head_dim)) return r;
+    const int group = q_heads / kv_heads;
+    if (page_size <= 0 || table_width <= 0 || cache_pages < 0) {
+        return fail(CLEF_ERR_INVALID, "%s: page_size %d table_width %d cache_pages %d", what, page_size, table_width, cache_pages);
+    }
+    if ((long long)table_width * page_size * group >= 0x40000000LL || (long long)cache_pages * page_size >= 0x7fffffffLL) {
+        return fail(CLEF_ERR_TOO_LARGE, "%s: %d pages of %d tokens per sequence, %d pages in the cache", what, table_width,
+                    page_size, cache_pages);
+    }
+    if (n_seqs == 0 || total_q == 0) return CLEF_OK;
+    if (!out || !q || !cache_k || !cache_v || !page_table || !q_start || !kv_len || !workspace ||
+        (cache_dtype == CLEF_E4M3 && (!k_scales || !v_scales))) {
+        return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
+    }
+    if (out == q) return fail(CLEF_ERR_INVALID, "%s: out must not alias q", what);
+    if (!aligned(out, 16) || !aligned(q, 16) || !aligned(cache_k, 16) || !aligned(cache_v, 16) || !aligned(workspace, 16)) {
+        return fail(CLEF_ERR_INVALID, "%s: out, q, caches and workspace must be 16-byte aligned", what);
+    }
+    const AttnPlan plan = attn_plan(n_seqs, total_q, q_heads, kv_heads, head_dim);
+    if (workspace_bytes < plan.bytes) {
+        return fail(CLEF_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, plan.bytes);
+    }
+    DeviceInfo dev;
+    if (int r = device_info(dev)) return r;
+    AttnArgs a{};
+    a.q = q, a.out = out, a.k = cache_k, a.v = cache_v, a.k_scales = k_scales, a.v_scales = v_scales;
+    a.table = page_table, a.q_start = q_start, a.kv_len = kv_len;
+    a.n_seqs = n_seqs, a.total_q = total_q, a.q_heads = q_heads, a.kv_heads = kv_heads, a.group = group;
+    a.page_size = page_size, a.table_width = table_width, a.cache_pages = cache_pages;
+    a.group_div = make_fast_div((uint32_t)group), a.page_div = make_fast_div((uint32_t)page_size);
+    a.scale_log2 = scale * 1.44269504088896341f;
+    a.desc = static_cast<int4*>(workspace);
+    a.part = reinterpret_cast<float*>(a.desc + 2 * kAttnMaxCtas);
+    cudaStream_t s = as_stream(stream);
+    if (dtype == CLEF_BF16) {
+        return cache_dtype == CLEF_BF16 ? launch_attention<Bf16, false>(s, dev, a, plan, head_dim, what)
+                                        : launch_attention<Bf16, true>(s, dev, a, plan, head_dim, what);
+    }
+    return cache_dtype == CLEF_BF16 ? launch_attention<F32, false>(s, dev, a, plan, head_dim, what)
+                                    : launch_attention<F32, true>(s, dev, a, plan, head_dim, what);
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@ import torch
 
 CLEF_BF16 = 0
 CLEF_F32 = 1
+CLEF_E4M3 = 2
 
 CLEF_OK = 0
 CLEF_DECLINED = 1
@@ -60,6 +61,8 @@ SYMBOLS = {
     "clef_add_rms_norm_quantise_nvfp4": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _F, _I, _I, _I]),
     "clef_embed_rms_norm_quantise_nvfp4": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _F, _I, _I, _I]),
     "clef_embed_rms_norm_quantise_nvfp4_ex": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _F, _I, _I, _I, _I]),
+    "clef_paged_attention_workspace": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(_SZ)]),
+    "clef_paged_attention": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _SZ, _I, _I]),
     "clef_quantise_fp8": (_I, [_P, _P, _P, _P, _I, _I, _I]),
     "clef_swiglu_quantise_fp8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I]),
     "clef_rms_norm_fp8_bf16": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _F, _I]),
@@ -175,6 +178,14 @@ def set_scale_layout(layout: int) -> None:
     """Row order inside a scale tile for every NVFP4 entry point: SF_ACTIVATION (the reference's activation side,
     default) or SF_INTERLEAVED (the 32 x 4 x 4 order of src/swizzle.rs:66-68, read directly by block-scaled GEMMs)."""
     _check(load().clef_set_scale_layout(int(layout)), "clef_set_scale_layout")
+
+
+def paged_attention_workspace(n_seqs: int, total_q: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of workspace a paged_attention_dev call of these shapes needs."""
+    n = _SZ(0)
+    _check(load().clef_paged_attention_workspace(n_seqs, total_q, q_heads, kv_heads, head_dim, ctypes.byref(n)),
+           "clef_paged_attention_workspace")
+    return n.value
 
 
 class Device:
@@ -452,6 +463,50 @@ class Device:
                                                                blk_mn, chunk, _dtype_code(table)),
                    "clef_embed_rms_norm_quantise_nvfp4")
         return h_out, packed, scales
+
+    # ==== attention over a paged KV cache ========================================================
+
+    def paged_attention_dev(self, q, cache_k, cache_v, page_table, q_start, kv_len, q_heads: int, kv_heads: int,
+                            head_dim: int, page_size: int, scale: float, k_scales=None, v_scales=None, out=None,
+                            workspace=None):
+        """Attention of new tokens q [total_q, q_heads, head_dim] over a paged bf16 or E4M3 (uint8 codes, with k_scales
+        and v_scales) cache; page_table [n_seqs, width], q_start [n_seqs + 1] and kv_len [n_seqs] are int32. `out` rows
+        outside every sequence are left as they are; without `out` a new tensor is returned. `workspace` defaults to a
+        fresh one of paged_attention_workspace bytes."""
+        for t, name in ((q, "q"), (cache_k, "cache_k"), (cache_v, "cache_v"), (page_table, "page_table"),
+                        (q_start, "q_start"), (kv_len, "kv_len")):
+            _dev_tensor(t, name)
+        for t, name in ((page_table, "page_table"), (q_start, "q_start"), (kv_len, "kv_len")):
+            if t.dtype != torch.int32:
+                raise ClefError(f"{name} must be int32, got {t.dtype}")
+        n_seqs, total_q = kv_len.numel(), q.numel() // (q_heads * head_dim)
+        if page_table.dim() != 2 or page_table.shape[0] != n_seqs or q_start.numel() != n_seqs + 1:
+            raise ClefError(f"page_table {tuple(page_table.shape)} and q_start {tuple(q_start.shape)} must be [n_seqs, width] "
+                            f"and [n_seqs + 1] for n_seqs = {n_seqs}")
+        fp8 = cache_k.dtype in (torch.uint8, torch.float8_e4m3fn)
+        if cache_v.dtype != cache_k.dtype or not (fp8 or cache_k.dtype == torch.bfloat16):
+            raise ClefError(f"the caches must both be bfloat16 or E4M3 codes, got {cache_k.dtype} and {cache_v.dtype}")
+        cache_rows = cache_k.numel() // (kv_heads * head_dim)
+        if cache_v.numel() != cache_k.numel():
+            raise ClefError("cache_k and cache_v must have the same size")
+        if fp8:
+            for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+                if t is None or t.dtype != torch.float32 or t.numel() != cache_rows * kv_heads:
+                    raise ClefError(f"{name} must be float32 with one value per cache row and kv head")
+                _dev_tensor(t, name)
+        if out is None:
+            out = torch.empty_like(q)
+        elif _dev_tensor(out, "out").dtype != q.dtype or out.numel() != q.numel():
+            raise ClefError("out must have the type and the size of q")
+        if workspace is None:
+            workspace = self._empty((paged_attention_workspace(n_seqs, total_q, q_heads, kv_heads, head_dim),), torch.uint8)
+        with torch.cuda.device(self.device):
+            _check(self.lib.clef_paged_attention(
+                _stream(), _ptr(out), _ptr(q), _ptr(cache_k), _ptr(cache_v), _ptr(k_scales), _ptr(v_scales),
+                _ptr(page_table), _ptr(q_start), _ptr(kv_len), n_seqs, total_q, q_heads, kv_heads, head_dim, page_size,
+                page_table.shape[1], cache_rows // page_size, scale, _ptr(workspace), workspace.numel(),
+                CLEF_E4M3 if fp8 else CLEF_BF16, _dtype_code(q)), "clef_paged_attention")
+        return out
 
     # ==== FP8 (E4M3) activation quantisers ======================================================
 

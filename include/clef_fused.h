@@ -48,7 +48,7 @@ extern "C" {
 
 typedef void* clef_stream_t; /* CUstream / cudaStream_t; NULL is the legacy default stream */
 
-enum clef_dtype { CLEF_BF16 = 0, CLEF_F32 = 1 };
+enum clef_dtype { CLEF_BF16 = 0, CLEF_F32 = 1, CLEF_E4M3 = 2 /* KV caches only */ };
 
 enum clef_status {
     CLEF_OK = 0,
@@ -238,6 +238,37 @@ int clef_add_rms_norm_quantise_nvfp4(clef_stream_t stream, void* sum_out, const 
 int clef_embed_rms_norm_quantise_nvfp4(clef_stream_t stream, const void* table, const int32_t* ids, void* h_out,
                                        const float* weight, uint8_t* packed, uint8_t* scales, int tokens, int hidden,
                                        float eps, float global_scale, int blk_mn, int chunk, int dtype);
+
+/* ------------------------------------------------------------------------------------------------
+ * Attention over a paged KV cache, and the FP8 (E4M3) cache.
+ * ------------------------------------------------------------------------------------------------ */
+
+/* Attention of the new tokens of n_seqs sequences over their cached keys and values, the new tokens' own among them
+ * (written beforehand with clef_rope_kv_write or one of its kin). Serves chunks of a prompt, single generated tokens, and
+ * batches that mix both. No counterpart as an entry point of this path in the reference (its Device::attention_dev,
+ * src/cuda/mod.rs:3201-3227, reads an unpaged bf16 cache).
+ *   q, out      [total_q, q_heads, head_dim]; sequence s owns rows q_start[s] .. q_start[s + 1] - 1 (q_start has
+ *               n_seqs + 1 non-decreasing entries). Rows outside every sequence are not written. out must not alias q.
+ *   kv_len      [n_seqs] cached tokens per sequence; the new tokens are the last of them, so new token i of n sees the
+ *               keys 0 .. kv_len - n + i. A row that sees no key (kv_len < n) is written as zeros.
+ *   cache_k/v   [cache_pages * page_size, kv_heads, head_dim], bf16 (cache_dtype CLEF_BF16) or E4M3 codes (CLEF_E4M3)
+ *               with k_scales / v_scales, one f32 per row and head, [cache_pages * page_size, kv_heads].
+ *   page_table  [n_seqs, table_width]: key t of sequence s is cache row page_table[s][t / page_size] * page_size +
+ *               t % page_size. Any page_size (an unpaged cache is one page per sequence). Entries past the last page in
+ *               use are not read; a page number outside 0 .. cache_pages - 1 is never followed, its keys read as zeros.
+ *   scale       multiplies the scores (1 / sqrt(head_dim) as a rule).
+ * Lengths are read on the device and clamped to the shapes (kv_len to table_width * page_size, q_start to total_q). q and
+ * the softmax weights enter the products as bf16, everything is summed in f32. Keys past kv_len are never read. A key
+ * that the causal mask hides from a row has weight exactly 0, but in a bf16 cache its value still enters the row's
+ * product: values of the new tokens must be finite. head_dim 64, 128 or 256; at most 64 query heads per kv head.
+ * workspace: clef_paged_attention_workspace bytes, 16-byte aligned, contents arbitrary; two calls that may run at the
+ * same time need two of them. Results do not depend on timing. */
+int clef_paged_attention_workspace(int n_seqs, int total_q, int q_heads, int kv_heads, int head_dim, size_t* bytes);
+int clef_paged_attention(clef_stream_t stream, void* out, const void* q, const void* cache_k, const void* cache_v,
+                         const float* k_scales, const float* v_scales, const int32_t* page_table, const int32_t* q_start,
+                         const int32_t* kv_len, int n_seqs, int total_q, int q_heads, int kv_heads, int head_dim,
+                         int page_size, int table_width, int cache_pages, float scale, void* workspace,
+                         size_t workspace_bytes, int cache_dtype, int dtype);
 
 /* ------------------------------------------------------------------------------------------------
  * FP8 (E4M3) activation quantisers, for the FP8 projections of a mixed NVFP4 + FP8 checkpoint.
