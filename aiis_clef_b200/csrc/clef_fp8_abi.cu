@@ -65,7 +65,7 @@ int fp8_rows_impl(const char* what, int mode, clef_stream_t stream, const void* 
         static std::atomic<int> occ{0};                                                                             \
         const int per_sm = ctas_per_sm(fp8_rows_hot_kernel<NB, MODE, T>, smem, occ);                                \
         launch_hot(fp8_rows_hot_kernel<NB, MODE, T>, clamp_grid(groups, (size_t)dev.sms * per_sm), smem, s,         \
-                   (const Storage<T>*)a, weight, out, scales, bf_out, rows, eps);                                   \
+                   (const Storage<T>*)a, weight, out, scales, bf_out, rows, eps, nullptr, nullptr);                 \
     }
         if (dtype == CLEF_BF16) {
             if (cols == 2048) CLEF_FP8_HOT(4, kFp8RmsNorm, Bf16) else CLEF_FP8_HOT(8, kFp8RmsNorm, Bf16)
@@ -123,6 +123,33 @@ int fp8_rows_impl(const char* what, int mode, clef_stream_t stream, const void* 
     return check_launch(what);
 }
 
+template <typename T, int QMAX>
+void launch_add_norm_q(cudaStream_t s, const DeviceInfo& dev, const void* a, const void* b, void* sum_out, const float* weight,
+                       uint8_t* out, uint16_t* scales, uint16_t* bf_out, int rows, int cols, float eps) {
+    const int team = ref_threads_per_row(cols);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(clamp_grid((size_t)rows, (size_t)dev.sms * (2048 / team)), 1, 1);
+    cfg.blockDim = dim3((unsigned)team, 1, 1);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    (void)cudaLaunchKernelEx(&cfg, add_rms_norm_fp8_kernel<T, QMAX>, (const Storage<T>*)a, (const Storage<T>*)b, (Storage<T>*)sum_out,
+                             weight, out, scales, bf_out, rows, cols, eps);
+}
+
+template <typename T>
+void launch_add_norm(cudaStream_t s, const DeviceInfo& dev, const void* a, const void* b, void* sum_out, const float* weight,
+                     uint8_t* out, uint16_t* scales, uint16_t* bf_out, int rows, int cols, float eps) {
+    const int team = ref_threads_per_row(cols), quads = (cols / 4 + team - 1) / team;   // 2 up to 2,048 columns
+    if (quads <= 2) launch_add_norm_q<T, 2>(s, dev, a, b, sum_out, weight, out, scales, bf_out, rows, cols, eps);
+    else if (quads <= 4) launch_add_norm_q<T, 4>(s, dev, a, b, sum_out, weight, out, scales, bf_out, rows, cols, eps);
+    else if (quads <= 8) launch_add_norm_q<T, 8>(s, dev, a, b, sum_out, weight, out, scales, bf_out, rows, cols, eps);
+    else launch_add_norm_q<T, 16>(s, dev, a, b, sum_out, weight, out, scales, bf_out, rows, cols, eps);
+}
+
 template <typename T, int HMAX>
 void launch_fp8_gated(cudaStream_t s, const DeviceInfo& dev, const void* x, const void* gate, const float* weight,
                       uint8_t* out, uint16_t* scales, int tokens, int cols, float eps, int vh, int rows_live) {
@@ -153,6 +180,49 @@ int clef_rms_norm_fp8_bf16(clef_stream_t stream, const void* x, const float* wei
                            uint16_t* q_scales, uint16_t* bf_out, int rows, int cols, float eps, int dtype) {
     return fp8_rows_impl("clef_rms_norm_fp8_bf16", kFp8RmsNorm, stream, x, nullptr, weight, q_out, q_scales, bf_out, rows,
                          cols, eps, dtype);
+}
+
+int clef_add_rms_norm_fp8_bf16(clef_stream_t stream, void* sum_out, const void* a, const void* b, const float* weight,
+                               uint8_t* q_out, uint16_t* q_scales, uint16_t* bf_out, int rows, int cols, float eps,
+                               int dtype) {
+    const char* what = "clef_add_rms_norm_fp8_bf16";
+    if (int r = check_dtype(dtype, what)) return r;
+    if (!sum_out || !a || !b || !weight || !q_out || !q_scales) return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
+    if (rows < 0 || cols <= 0 || cols % 8 != 0) {
+        return fail(CLEF_ERR_INVALID, "%s: rows %d, cols %d (cols must be a positive multiple of 8)", what, rows, cols);
+    }
+    if (cols > kFp8MaxCols) return fail(CLEF_ERR_TOO_LARGE, "%s: cols %d above %d", what, cols, kFp8MaxCols);
+    if (!aligned(sum_out, 16) || !aligned(a, 16) || !aligned(b, 16) || !aligned(weight, 16) || !aligned(q_out, 8) ||
+        !aligned(q_scales, 2) || (bf_out && !aligned(bf_out, 16))) {
+        return fail(CLEF_ERR_INVALID, "%s: activations, weight and the bf16 output must be 16-byte aligned, codes 8-byte", what);
+    }
+    if (rows == 0) return CLEF_OK;
+    DeviceInfo dev;
+    if (int r = device_info(dev)) return r;
+    cudaStream_t s = as_stream(stream);
+    if (use_hot() && (cols == 2048 || cols == 4096) && aligned(a, 32) && aligned(b, 32) && aligned(sum_out, 32) &&
+        aligned(q_out, 16) && (!bf_out || aligned(bf_out, 32))) {
+        const size_t groups = ((size_t)rows + 7) / 8;
+        const size_t smem = (size_t)cols * sizeof(float);
+#define CLEF_FP8_ADD_HOT(NB, T)                                                                                      \
+    {                                                                                                                \
+        static std::atomic<int> occ{0};                                                                              \
+        auto kernel = fp8_rows_hot_kernel<NB, kFp8RmsNorm, T, true>;                                                 \
+        const int per_sm = ctas_per_sm(kernel, smem, occ);                                                           \
+        launch_hot(kernel, clamp_grid(groups, (size_t)dev.sms * per_sm), smem, s, (const Storage<T>*)a, weight, q_out, \
+                   q_scales, bf_out, rows, eps, (const Storage<T>*)b, (Storage<T>*)sum_out);                         \
+    }
+        if (dtype == CLEF_BF16) {
+            if (cols == 2048) CLEF_FP8_ADD_HOT(4, Bf16) else CLEF_FP8_ADD_HOT(8, Bf16)
+        } else {
+            if (cols == 2048) CLEF_FP8_ADD_HOT(4, F32) else CLEF_FP8_ADD_HOT(8, F32)
+        }
+#undef CLEF_FP8_ADD_HOT
+        return check_launch(what);
+    }
+    if (dtype == CLEF_BF16) launch_add_norm<Bf16>(s, dev, a, b, sum_out, weight, q_out, q_scales, bf_out, rows, cols, eps);
+    else launch_add_norm<F32>(s, dev, a, b, sum_out, weight, q_out, q_scales, bf_out, rows, cols, eps);
+    return check_launch(what);
 }
 
 int clef_rms_norm_gated_quantise_fp8(clef_stream_t stream, const void* x, const void* gate, const float* weight,

@@ -1,0 +1,146 @@
+// C-ABI of the FP8 (E4M3) KV cache: written behind RoPE, read back through a row map. Declarations:
+// include/clef_fused.h. Same contract as the other entry points: asynchronous on the caller's stream, no allocation, no
+// synchronisation, grids that depend on the shape arguments only.
+
+#include "../../include/clef_fused.h"
+
+#include <atomic>
+
+#include "abi_support.cuh"
+#include "kernels_kv_cache.cuh"
+
+using namespace clef;
+using namespace clef::abi;
+
+namespace {
+
+template <typename T, int G, bool NORM>
+void launch_kv_write(cudaStream_t s, const DeviceInfo& dev, const KvWriteArgs& a) {
+    static std::atomic<int> occ{0};
+    auto kernel = kv_write_fp8_kernel<T, G, NORM>;
+    const int per_sm = ctas_per_sm(kernel, 0, occ);
+    const size_t per_cta = (size_t)(kCtaThreads / 32) * (32 / G);
+    const size_t rows = (size_t)a.tokens * a.heads_div.d;
+    launch_hot(kernel, balanced_grid((rows + per_cta - 1) / per_cta, (size_t)dev.sms * per_sm), 0, s, a);
+}
+
+template <typename T, bool NORM>
+void launch_kv_write_for(cudaStream_t s, const DeviceInfo& dev, const KvWriteArgs& a) {
+    if (a.head_dim <= 64) launch_kv_write<T, 8, NORM>(s, dev, a);
+    else if (a.head_dim <= 128) launch_kv_write<T, 16, NORM>(s, dev, a);
+    else launch_kv_write<T, 32, NORM>(s, dev, a);
+}
+
+int kv_write_impl(const char* what, clef_stream_t stream, KvWriteArgs a, bool with_q, bool norm, int dtype) {
+    if (int r = check_dtype(dtype, what)) return r;
+    if (!a.cache_k || !a.cache_v || !a.k_scales || !a.v_scales || !a.k || !a.v || !a.cos_t || !a.sin_t ||
+        (with_q && (!a.q || !a.q_out)) || (norm && !a.weight)) {
+        return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
+    }
+    if (a.tokens < 0 || a.kv_heads <= 0 || (with_q && a.q_heads <= 0) || a.head_dim <= 0 || a.rotary_dim < 0 || a.cache_rows < 0) {
+        return fail(CLEF_ERR_INVALID, "%s: tokens %d q_heads %d kv_heads %d head_dim %d rotary_dim %d cache_rows %d", what, a.tokens,
+                    a.q_heads, a.kv_heads, a.head_dim, a.rotary_dim, a.cache_rows);
+    }
+    if (a.head_dim % 8 != 0 || a.rotary_dim % 16 != 0 || a.rotary_dim > a.head_dim) {
+        return fail(CLEF_ERR_INVALID, "%s: head_dim %d must be a multiple of 8, rotary_dim %d one of 16 and not above head_dim", what,
+                    a.head_dim, a.rotary_dim);
+    }
+    if (a.head_dim > kKvMaxHeadDim) return fail(CLEF_ERR_TOO_LARGE, "%s: head_dim %d above %d", what, a.head_dim, kKvMaxHeadDim);
+    if (with_q && a.q_out == a.q) return fail(CLEF_ERR_INVALID, "%s: q_out must not alias q", what);
+    if ((with_q && (!aligned(a.q, 16) || !aligned(a.q_out, 16))) || !aligned(a.k, 16) || !aligned(a.v, 16) ||
+        !aligned(a.cos_t, 16) || !aligned(a.sin_t, 16) || !aligned(a.cache_k, 8) || !aligned(a.cache_v, 8) ||
+        !aligned(a.k_scales, 4) || !aligned(a.v_scales, 4) || !aligned(a.weight, 4)) {
+        return fail(CLEF_ERR_INVALID, "%s: activations and tables must be 16-byte aligned, codes 8-byte", what);
+    }
+    const long long per_token = (long long)a.q_heads + 2LL * a.kv_heads;
+    // the grid-stride counter advances past the last head row by up to one grid of them
+    if (per_token * a.tokens >= 0x40000000LL) return fail(CLEF_ERR_TOO_LARGE, "%s: %d tokens x %lld head rows", what, a.tokens, per_token);
+    if (a.tokens == 0) return CLEF_OK;
+    DeviceInfo dev;
+    if (int r = device_info(dev)) return r;
+    a.heads_div = make_fast_div((uint32_t)per_token);
+    cudaStream_t s = as_stream(stream);
+    if (dtype == CLEF_BF16) {
+        if (norm) launch_kv_write_for<Bf16, true>(s, dev, a);
+        else launch_kv_write_for<Bf16, false>(s, dev, a);
+    } else {
+        if (norm) launch_kv_write_for<F32, true>(s, dev, a);
+        else launch_kv_write_for<F32, false>(s, dev, a);
+    }
+    return check_launch(what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int clef_rope_kv_write_fp8(clef_stream_t stream, uint8_t* cache_k, uint8_t* cache_v, float* k_scales, float* v_scales,
+                           const void* k, const void* v, const float* cos_table, const float* sin_table, int tokens,
+                           int kv_heads, int head_dim, int rotary_dim, const int32_t* seq_start, const int32_t* pos_base,
+                           const int32_t* pos_map, const int32_t* cache_map, const int32_t* cache_len, int cache_rows,
+                           int dtype) {
+    return kv_write_impl("clef_rope_kv_write_fp8", stream,
+                         KvWriteArgs{nullptr, nullptr, 0, k, v, cache_k, cache_v, k_scales, v_scales, nullptr, cos_table, sin_table,
+                                     seq_start, pos_base, pos_map, cache_map, cache_len, tokens, kv_heads, head_dim, rotary_dim,
+                                     cache_rows, 0.0f, FastDiv{}}, false, false, dtype);
+}
+
+int clef_rope_qkv_write_fp8(clef_stream_t stream, void* q_out, const void* q, int q_heads, uint8_t* cache_k,
+                            uint8_t* cache_v, float* k_scales, float* v_scales, const void* k, const void* v, int kv_heads,
+                            const float* cos_table, const float* sin_table, int tokens, int head_dim, int rotary_dim,
+                            const int32_t* seq_start, const int32_t* pos_base, const int32_t* pos_map,
+                            const int32_t* cache_map, const int32_t* cache_len, int cache_rows, int dtype) {
+    return kv_write_impl("clef_rope_qkv_write_fp8", stream,
+                         KvWriteArgs{q, q_out, q_heads, k, v, cache_k, cache_v, k_scales, v_scales, nullptr, cos_table, sin_table,
+                                     seq_start, pos_base, pos_map, cache_map, cache_len, tokens, kv_heads, head_dim, rotary_dim,
+                                     cache_rows, 0.0f, FastDiv{}}, true, false, dtype);
+}
+
+int clef_qk_norm_rope_kv_write_fp8(clef_stream_t stream, uint8_t* cache_k, uint8_t* cache_v, float* k_scales,
+                                   float* v_scales, const void* k_raw, const void* v, const float* weight,
+                                   const float* cos_table, const float* sin_table, int tokens, int kv_heads, int head_dim,
+                                   int rotary_dim, float eps, const int32_t* seq_start, const int32_t* pos_base,
+                                   const int32_t* pos_map, const int32_t* cache_map, const int32_t* cache_len,
+                                   int cache_rows, int dtype) {
+    return kv_write_impl("clef_qk_norm_rope_kv_write_fp8", stream,
+                         KvWriteArgs{nullptr, nullptr, 0, k_raw, v, cache_k, cache_v, k_scales, v_scales, weight, cos_table, sin_table,
+                                     seq_start, pos_base, pos_map, cache_map, cache_len, tokens, kv_heads, head_dim, rotary_dim,
+                                     cache_rows, eps, FastDiv{}}, false, true, dtype);
+}
+
+int clef_kv_read_fp8(clef_stream_t stream, void* k_out, void* v_out, const uint8_t* cache_k, const uint8_t* cache_v,
+                     const float* k_scales, const float* v_scales, const int32_t* row_map, int rows, int cache_rows,
+                     int kv_heads, int head_dim, int dtype) {
+    const char* what = "clef_kv_read_fp8";
+    if (int r = check_dtype(dtype, what)) return r;
+    if (!k_out || !v_out || !cache_k || !cache_v || !k_scales || !v_scales) return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
+    if (rows < 0 || cache_rows < 0 || kv_heads <= 0 || head_dim <= 0 || head_dim % 8 != 0) {
+        return fail(CLEF_ERR_INVALID, "%s: rows %d cache_rows %d kv_heads %d head_dim %d (a multiple of 8)", what, rows, cache_rows,
+                    kv_heads, head_dim);
+    }
+    if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(cache_k, 8) || !aligned(cache_v, 8) || !aligned(k_scales, 4) ||
+        !aligned(v_scales, 4)) {
+        return fail(CLEF_ERR_INVALID, "%s: outputs must be 16-byte aligned, codes 8-byte", what);
+    }
+    const unsigned long long head_rows = (unsigned long long)rows * kv_heads;
+    if (head_rows >= 0x7fffffffull || head_rows * (head_dim / 8) >= 0x7fffffffull) {
+        return fail(CLEF_ERR_TOO_LARGE, "%s: %d rows of %d x %d", what, rows, kv_heads, head_dim);
+    }
+    if (rows == 0) return CLEF_OK;
+    DeviceInfo dev;
+    if (int r = device_info(dev)) return r;
+    cudaStream_t s = as_stream(stream);
+    const size_t pieces = (size_t)head_rows * (head_dim / 8);
+    const FastDiv piece_div = make_fast_div((uint32_t)(head_dim / 8)), heads_div = make_fast_div((uint32_t)kv_heads);
+    auto launch = [&](auto kernel, std::atomic<int>& occ, auto* k, auto* v) {
+        const int per_sm = ctas_per_sm(kernel, 0, occ);
+        launch_hot(kernel, balanced_grid((2 * pieces + kCtaThreads - 1) / kCtaThreads, (size_t)dev.sms * per_sm), 0, s, k, v, cache_k,
+                   cache_v, k_scales, v_scales, (const int*)row_map, pieces, cache_rows, kv_heads, piece_div, heads_div);
+    };
+    static std::atomic<int> occ[2];
+    if (dtype == CLEF_BF16) launch(kv_read_fp8_kernel<Bf16>, occ[0], (uint16_t*)k_out, (uint16_t*)v_out);
+    else launch(kv_read_fp8_kernel<F32>, occ[1], (float*)k_out, (float*)v_out);
+    return check_launch(what);
+}
+
+}  // extern "C"

@@ -151,6 +151,88 @@ fp8_rows_kernel(const typename T::storage* __restrict__ a, const typename T::sto
     }
 }
 
+// add_rms_norm_fp8_bf16 for any cols % 8 == 0: sum = a + b, rounded to T and stored (sum_out may be a or b), then
+// rms_norm_fp8_bf16 of the stored sum. One CTA of the reference's team of threads (kernels/elementwise.cu:8) owns a row;
+// thread t holds quads t, t + team, ... (QMAX of them at most) in registers from the one read on, in the order
+// team_sum_squares adds them.
+template <typename T, int QMAX>
+__global__ void __launch_bounds__(kCtaThreads)
+add_rms_norm_fp8_kernel(const typename T::storage* a, const typename T::storage* b, typename T::storage* sum_out,
+                        const float* __restrict__ weight, uint8_t* __restrict__ out, uint16_t* __restrict__ scales,
+                        uint16_t* __restrict__ bf_out, int rows, int cols, float eps) {
+    __shared__ float s_part[2][kCtaThreads / 32];
+    const int team = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = team >> 5, c4 = cols >> 2;
+    pdl_launch_dependents();
+    pdl_wait_prior_grids();
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        const size_t at = (size_t)row * cols;
+        float4 v[QMAX];
+#pragma unroll
+        for (int k = 0; k < QMAX; ++k) {
+            const int i = threadIdx.x + k * team;
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i < c4) {
+                const float4 p = load_quad<T>(a + at, i), q = load_quad<T>(b + at, i);
+                v[k] = make_float4(__fadd_rn(p.x, q.x), __fadd_rn(p.y, q.y), __fadd_rn(p.z, q.z), __fadd_rn(p.w, q.w));
+            }
+        }
+        float acc = 0.0f;
+#pragma unroll
+        for (int k = 0; k < QMAX; ++k) {
+            const int i = threadIdx.x + k * team;
+            if (i < c4) {
+                store_quad<T>(sum_out + at, i, v[k]);
+                if (T::kBytes == 2) {   // the norm sees the stored sum
+                    const uint32_t lo = pack_bf16x2(v[k].x, v[k].y), hi = pack_bf16x2(v[k].z, v[k].w);
+                    v[k] = make_float4(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi));
+                }
+                acc = __fadd_rn(acc, quad_sq(v[k]));
+            }
+        }
+        float total = warp_tree_sum(acc);
+        if (warps > 1) {
+            if (lane == 0) s_part[0][warp] = total;
+            __syncthreads();
+            total = lane < warps ? s_part[0][lane] : 0.0f;
+#pragma unroll
+            for (int off = 4; off > 0; off >>= 1) total = __fadd_rn(total, __shfl_xor_sync(kFullMask, total, off));
+            total = __shfl_sync(kFullMask, total, 0);
+        }
+        const float inv_norm = inv_rms(total, cols, eps);
+        float amax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < QMAX; ++k) {
+            const int i = threadIdx.x + k * team;
+            if (i < c4) {
+                const float4 w = *reinterpret_cast<const float4*>(weight + 4 * i);
+                v[k] = make_float4(v[k].x * inv_norm * (1.0f + w.x), v[k].y * inv_norm * (1.0f + w.y),
+                                   v[k].z * inv_norm * (1.0f + w.z), v[k].w * inv_norm * (1.0f + w.w));
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
+            }
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kFullMask, amax, off));
+        if (warps > 1) {
+            if (lane == 0) s_part[1][warp] = amax;
+            __syncthreads();
+            for (int w = 0; w < warps; ++w) amax = fmaxf(amax, s_part[1][w]);
+        }
+        const float scale = __fdiv_rn(amax, 448.0f);
+        if (threadIdx.x == 0) scales[row] = (uint16_t)(__float_as_uint(scale) >> 16);
+        const float inv = (scale > 0.0f) ? __fdiv_rn(1.0f, scale) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < QMAX; ++k) {
+            const int i = threadIdx.x + k * team;
+            if (i < c4) {
+                const uint32_t code = fp8_code(v[k].x, inv) | (fp8_code(v[k].y, inv) << 8) | (fp8_code(v[k].z, inv) << 16) |
+                                      (fp8_code(v[k].w, inv) << 24);
+                *reinterpret_cast<uint32_t*>(out + at + 4 * i) = code;
+                if (bf_out) store_quad<Bf16>(bf_out + at, i, v[k]);
+            }
+        }
+    }
+}
+
 // rms_norm_gated_quantise_fp8 (kernels/quantise.cu:123-191): one CTA per token; warp w normalises the
 // head rows w, w + 8, ... (< vh) of the token, a lane the quads lane, lane + 32 (cols <= 256) of a head
 // row in the reference's order; v = x * inv * weight * __fdividef(g, 1 + __expf(-g)); the token's amax
@@ -406,12 +488,15 @@ __device__ __forceinline__ float block_abs_max_ignoring_nan(const f32x2* v) {
 // quantise_fp8 (MODE plain) and rms_norm_fp8_bf16 (MODE RmsNorm, bf_out optional) for cols = NB * 512, one warp
 // per row: the row structure, prefetch and summation tree of rms_norm_quant_hot_kernel; the row maximum is a
 // 5-step butterfly, the row scale is computed by every lane, each lane encodes its NB blocks (16 bytes each).
-template <int NB, int MODE, typename T = Bf16>
+// ADD (MODE RmsNorm): the row is x + addend, rounded to T, written to sum_out (which may be x or addend: a row is read
+// whole by the warp that then writes it), and normalised as stored.
+template <int NB, int MODE, typename T = Bf16, bool ADD = false>
 __global__ void __launch_bounds__(kCtaThreads, (NB <= 4 ? 2 : 1))
 fp8_rows_hot_kernel(const typename T::storage* __restrict__ x, const float* __restrict__ weight, uint8_t* __restrict__ out,
-                    uint16_t* __restrict__ scales, uint16_t* __restrict__ bf_out, int rows, float eps) {
+                    uint16_t* __restrict__ scales, uint16_t* __restrict__ bf_out, int rows, float eps,
+                    const typename T::storage* addend = nullptr, typename T::storage* sum_out = nullptr) {
     constexpr int COLS = NB * 512;
-    constexpr bool NAT = T::kBytes == 4, REGPF = T::kBytes == 2;
+    constexpr bool NAT = T::kBytes == 4, REGPF = T::kBytes == 2 && !ADD;   // (a second prefetched row would spill)
     constexpr int LINE = 128 / T::kBytes;   // values per 128-byte line
     extern __shared__ float4 s_w[];   // (1 + w) in the pairs' order, as in rms_norm_quant_hot_kernel
     const int lane = threadIdx.x & 31;
@@ -429,15 +514,17 @@ fp8_rows_hot_kernel(const typename T::storage* __restrict__ x, const float* __re
 #pragma unroll
         for (int h = 0; h < NB * T::kBytes / 8; ++h) {
             prefetch_l2(x + (size_t)r * COLS + (size_t)(lane + 32 * h) * LINE);
+            if (ADD) prefetch_l2(addend + (size_t)r * COLS + (size_t)(lane + 32 * h) * LINE);
         }
     };
     if (row < rows) name_row_to_l2(row);   // this warp's first row towards L2; see prefetch_l2
     pdl_wait_prior_grids();
-    RawBlock16<T> d[NB];
+    RawBlock16<T> d[NB], e[ADD ? NB : 1];
     if (REGPF && row < rows) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             d[j] = ldg_block16<T>(x + (size_t)row * COLS + (size_t)(lane + 32 * j) * 16);
+            if (ADD) e[j] = ldg_block16<T>(addend + (size_t)row * COLS + (size_t)(lane + 32 * j) * 16);
         }
     }
     __syncthreads();
@@ -446,6 +533,7 @@ fp8_rows_hot_kernel(const typename T::storage* __restrict__ x, const float* __re
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
                 d[j] = ldg_block16<T>(x + (size_t)row * COLS + (size_t)(lane + 32 * j) * 16);
+                if (ADD) e[j] = ldg_block16<T>(addend + (size_t)row * COLS + (size_t)(lane + 32 * j) * 16);
             }
         }
         f32x2 v[NB][8];
@@ -453,6 +541,27 @@ fp8_rows_hot_kernel(const typename T::storage* __restrict__ x, const float* __re
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             unpack_block16<T>(d[j], v[j]);
+            if (ADD) {
+                f32x2 u[8];
+                unpack_block16<T>(e[j], u);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[j][i] = f2_add(v[j][i], u[i]);
+                typename T::storage* dst = sum_out + (size_t)row * COLS + (size_t)(lane + 32 * j) * 16;
+                if (NAT) {
+                    U8x32 w[2];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        w[0].w[2 * i] = __float_as_uint(v[j][i].x), w[0].w[2 * i + 1] = __float_as_uint(v[j][i].y);
+                        w[1].w[2 * i] = __float_as_uint(v[j][4 + i].x), w[1].w[2 * i + 1] = __float_as_uint(v[j][4 + i].y);
+                    }
+                    stg_v8(dst, w[0]);
+                    stg_v8(dst + 8, w[1]);
+                } else {
+                    const U8x32 w = pack16_bf16(v[j]);
+                    stg_v8(dst, w);
+                    unpack16_quadpairs(w, v[j]);   // the norm sees the stored sum
+                }
+            }
             if (MODE == kFp8RmsNorm) {
                 float quad[4];
                 quad_squares_of<NAT>(v[j], quad);
@@ -468,6 +577,7 @@ fp8_rows_hot_kernel(const typename T::storage* __restrict__ x, const float* __re
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     d[j] = ldg_block16<T>(x + (size_t)next * COLS + (size_t)(lane + 32 * j) * 16);
+                    if (ADD) e[j] = ldg_block16<T>(addend + (size_t)next * COLS + (size_t)(lane + 32 * j) * 16);
                 }
             } else {
                 name_row_to_l2(next);
@@ -527,7 +637,7 @@ fp8_rows_hot_kernel(const typename T::storage* __restrict__ x, const float* __re
             const float inv_scale = (scale > 0.0f) ? __fdiv_rn(1.0f, scale) : 0.0f;
             for (int j = 0; j < NB; ++j) {
                 const int b = lane + 32 * j;
-                fp8_block_cold<MODE, T>(x + (size_t)row * COLS + b * 16, nullptr, weight + b * 16, inv_norm, inv_scale,
+                fp8_block_cold<MODE, T>((ADD ? sum_out : x) + (size_t)row * COLS + b * 16, nullptr, weight + b * 16, inv_norm, inv_scale,
                                         reinterpret_cast<uint4*>(orow + (size_t)b * 16));
             }
         }

@@ -63,9 +63,14 @@ SYMBOLS = {
     "clef_embed_rms_norm_quantise_nvfp4_ex": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _F, _I, _I, _I, _I]),
     "clef_paged_attention_workspace": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(_SZ)]),
     "clef_paged_attention": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _SZ, _I, _I]),
+    "clef_rope_kv_write_fp8": (_I, [_P] * 9 + [_I] * 4 + [_P] * 5 + [_I, _I]),
+    "clef_rope_qkv_write_fp8": (_I, [_P, _P, _P, _I] + [_P] * 6 + [_I, _P, _P, _I, _I, _I] + [_P] * 5 + [_I, _I]),
+    "clef_qk_norm_rope_kv_write_fp8": (_I, [_P] * 10 + [_I] * 4 + [_F] + [_P] * 5 + [_I, _I]),
+    "clef_kv_read_fp8": (_I, [_P] * 8 + [_I] * 5),
     "clef_quantise_fp8": (_I, [_P, _P, _P, _P, _I, _I, _I]),
     "clef_swiglu_quantise_fp8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I]),
     "clef_rms_norm_fp8_bf16": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _F, _I]),
+    "clef_add_rms_norm_fp8_bf16": (_I, [_P] * 8 + [_I, _I, _F, _I]),
     "clef_rms_norm_gated_quantise_fp8": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _F, _I, _I, _I]),
     "clef_causal_conv_silu": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I]),
     "clef_conv_hist_save": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I]),
@@ -486,14 +491,12 @@ class Device:
         fp8 = cache_k.dtype in (torch.uint8, torch.float8_e4m3fn)
         if cache_v.dtype != cache_k.dtype or not (fp8 or cache_k.dtype == torch.bfloat16):
             raise ClefError(f"the caches must both be bfloat16 or E4M3 codes, got {cache_k.dtype} and {cache_v.dtype}")
-        cache_rows = cache_k.numel() // (kv_heads * head_dim)
-        if cache_v.numel() != cache_k.numel():
-            raise ClefError("cache_k and cache_v must have the same size")
         if fp8:
-            for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
-                if t is None or t.dtype != torch.float32 or t.numel() != cache_rows * kv_heads:
-                    raise ClefError(f"{name} must be float32 with one value per cache row and kv head")
-                _dev_tensor(t, name)
+            cache_rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
+        else:
+            cache_rows = cache_k.numel() // (kv_heads * head_dim)
+            if cache_v.numel() != cache_k.numel():
+                raise ClefError("cache_k and cache_v must have the same size")
         if out is None:
             out = torch.empty_like(q)
         elif _dev_tensor(out, "out").dtype != q.dtype or out.numel() != q.numel():
@@ -507,6 +510,70 @@ class Device:
                 page_table.shape[1], cache_rows // page_size, scale, _ptr(workspace), workspace.numel(),
                 CLEF_E4M3 if fp8 else CLEF_BF16, _dtype_code(q)), "clef_paged_attention")
         return out
+
+    # ==== the FP8 (E4M3) KV cache ================================================================
+
+    def _fp8_cache(self, cache_k, cache_v, k_scales, v_scales, kv_heads: int, head_dim: int) -> int:
+        """Checks the four buffers of an FP8 cache against each other; returns its rows."""
+        for t, name in ((cache_k, "cache_k"), (cache_v, "cache_v")):
+            if _dev_tensor(t, name).dtype not in (torch.uint8, torch.float8_e4m3fn):
+                raise ClefError(f"{name} must hold E4M3 codes (uint8 or float8_e4m3fn), got {t.dtype}")
+        rows = cache_k.numel() // (kv_heads * head_dim)
+        if cache_v.numel() != cache_k.numel():
+            raise ClefError("cache_k and cache_v must have the same size")
+        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+            if _dev_tensor(t, name).dtype != torch.float32 or t.numel() != rows * kv_heads:
+                raise ClefError(f"{name} must be float32 with one value per cache row and kv head")
+        return rows
+
+    def rope_kv_write_fp8_dev(self, cache_k, cache_v, k_scales, v_scales, k, v, cos, sin, tokens: int, kv_heads: int,
+                              head_dim: int, rotary_dim: int, seq_start=None, pos_base=None, pos_map=None, cache_map=None,
+                              cache_len=None):
+        """rope_apply_dev on k, then k and v into the FP8 caches and their scales (in place), one launch."""
+        _dev_tensor(k, "k"), _dev_tensor(v, "v")
+        rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
+        with torch.cuda.device(self.device):
+            _check(self.lib.clef_rope_kv_write_fp8(
+                _stream(), _ptr(cache_k), _ptr(cache_v), _ptr(k_scales), _ptr(v_scales), _ptr(k), _ptr(v), _ptr(cos), _ptr(sin),
+                tokens, kv_heads, head_dim, rotary_dim, _ptr(seq_start), _ptr(pos_base), _ptr(pos_map), _ptr(cache_map),
+                _ptr(cache_len), rows, _dtype_code(k)), "clef_rope_kv_write_fp8")
+
+    def rope_qkv_write_fp8_dev(self, q, cache_k, cache_v, k_scales, v_scales, k, v, cos, sin, tokens: int, q_heads: int,
+                               kv_heads: int, head_dim: int, rotary_dim: int, seq_start=None, pos_base=None, pos_map=None,
+                               cache_map=None, cache_len=None):
+        """rope_apply_dev on q (returned) and rope_kv_write_fp8_dev on k, v (caches written in place), one launch."""
+        _dev_tensor(q, "q"), _dev_tensor(k, "k"), _dev_tensor(v, "v")
+        rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
+        q_out = self._empty((tokens, q_heads, head_dim), q.dtype)
+        with torch.cuda.device(self.device):
+            _check(self.lib.clef_rope_qkv_write_fp8(
+                _stream(), _ptr(q_out), _ptr(q), q_heads, _ptr(cache_k), _ptr(cache_v), _ptr(k_scales), _ptr(v_scales), _ptr(k),
+                _ptr(v), kv_heads, _ptr(cos), _ptr(sin), tokens, head_dim, rotary_dim, _ptr(seq_start), _ptr(pos_base),
+                _ptr(pos_map), _ptr(cache_map), _ptr(cache_len), rows, _dtype_code(q)), "clef_rope_qkv_write_fp8")
+        return q_out
+
+    def qk_norm_rope_kv_write_fp8_dev(self, cache_k, cache_v, k_scales, v_scales, k_raw, v, weight, cos, sin, tokens: int,
+                                      kv_heads: int, head_dim: int, rotary_dim: int, eps: float, seq_start=None,
+                                      pos_base=None, pos_map=None, cache_map=None, cache_len=None):
+        """qk_norm_rope_dev on k_raw, then k and v into the FP8 caches and their scales (in place), one launch."""
+        _dev_tensor(k_raw, "k_raw"), _dev_tensor(v, "v")
+        rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
+        with torch.cuda.device(self.device):
+            _check(self.lib.clef_qk_norm_rope_kv_write_fp8(
+                _stream(), _ptr(cache_k), _ptr(cache_v), _ptr(k_scales), _ptr(v_scales), _ptr(k_raw), _ptr(v), _ptr(weight),
+                _ptr(cos), _ptr(sin), tokens, kv_heads, head_dim, rotary_dim, eps, _ptr(seq_start), _ptr(pos_base),
+                _ptr(pos_map), _ptr(cache_map), _ptr(cache_len), rows, _dtype_code(k_raw)), "clef_qk_norm_rope_kv_write_fp8")
+
+    def kv_read_fp8_dev(self, cache_k, cache_v, k_scales, v_scales, rows: int, kv_heads: int, head_dim: int, row_map=None,
+                        dtype=torch.bfloat16):
+        """(k, v) [rows, kv_heads, head_dim] of `dtype`: the cache rows row_map (0 .. rows - 1 without a map) read back."""
+        cache_rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
+        k, v = self._empty((rows, kv_heads, head_dim), dtype), self._empty((rows, kv_heads, head_dim), dtype)
+        with torch.cuda.device(self.device):
+            _check(self.lib.clef_kv_read_fp8(_stream(), _ptr(k), _ptr(v), _ptr(cache_k), _ptr(cache_v), _ptr(k_scales),
+                                             _ptr(v_scales), _ptr(row_map), rows, cache_rows, kv_heads, head_dim,
+                                             _dtype_code(k)), "clef_kv_read_fp8")
+        return k, v
 
     # ==== FP8 (E4M3) activation quantisers ======================================================
 
@@ -538,6 +605,20 @@ class Device:
             _check(self.lib.clef_rms_norm_fp8_bf16(_stream(), _ptr(x), _ptr(weight), _ptr(q), _ptr(qs), _ptr(bf), rows, cols,
                                                    eps, _dtype_code(x)), "clef_rms_norm_fp8_bf16")
         return q, qs, bf
+
+    def add_rms_norm_fp8_bf16_dev(self, a, b, weight, rows: int, cols: int, eps: float, sum_out=None):
+        """add_dev followed by rms_norm_fp8_bf16_dev on the stored sum, one pass; returns (sum, codes, row scales, bf16
+        copy)."""
+        _dev_tensor(a, "a"), _dev_tensor(b, "b")
+        if sum_out is None:
+            sum_out = self._empty((rows, cols), a.dtype)
+        q, qs = self._empty((rows, cols), torch.uint8), self._empty((rows,), torch.int16)
+        bf = self._empty((rows, cols), torch.bfloat16)
+        with torch.cuda.device(self.device):
+            _check(self.lib.clef_add_rms_norm_fp8_bf16(_stream(), _ptr(sum_out), _ptr(a), _ptr(b), _ptr(weight), _ptr(q),
+                                                       _ptr(qs), _ptr(bf), rows, cols, eps, _dtype_code(a)),
+                   "clef_add_rms_norm_fp8_bf16")
+        return sum_out, q, qs, bf
 
     # -- src/cuda/mod.rs:2304-2328 ------------------------------------------------------------
     def rms_norm_gated_quantise_fp8_dev(self, x, gate, weight, rows: int, cols: int, vh: int, eps: float):

@@ -270,6 +270,40 @@ int clef_paged_attention(clef_stream_t stream, void* out, const void* q, const v
                          int page_size, int table_width, int cache_pages, float scale, void* workspace,
                          size_t workspace_bytes, int cache_dtype, int dtype);
 
+/* The FP8 cache: rows of kv_heads * head_dim E4M3 codes, and one f32 scale per row and head ([cache_rows, kv_heads]). A
+ * head row is stored as scale = max |x| / 448 and codes of x / scale, rounded to nearest even, where x is the f32 value
+ * that the bf16 cache would round; code * scale is what it stands for. A head row whose maximum is below 2^-100 is
+ * stored as zeros (scale 0); one that holds an infinity or a NaN as scale NaN. Codes never hold a NaN. No counterpart in
+ * the reference, whose cache is bf16.
+ *
+ * clef_rope_kv_write_fp8, clef_rope_qkv_write_fp8 and clef_qk_norm_rope_kv_write_fp8 take the arguments of the bf16
+ * forms above (positions, cache_map, cache_len) with the scales beside the caches, and cache_rows: a token whose row is
+ * outside 0 .. cache_rows - 1 (a padding token, mapped to -1) is not written. The rows of the others must be distinct.
+ * One launch each. head_dim % 8 == 0 and at most 256, rotary_dim % 16 == 0. */
+int clef_rope_kv_write_fp8(clef_stream_t stream, uint8_t* cache_k, uint8_t* cache_v, float* k_scales, float* v_scales,
+                           const void* k, const void* v, const float* cos_table, const float* sin_table, int tokens,
+                           int kv_heads, int head_dim, int rotary_dim, const int32_t* seq_start, const int32_t* pos_base,
+                           const int32_t* pos_map, const int32_t* cache_map, const int32_t* cache_len, int cache_rows,
+                           int dtype);
+int clef_rope_qkv_write_fp8(clef_stream_t stream, void* q_out, const void* q, int q_heads, uint8_t* cache_k,
+                            uint8_t* cache_v, float* k_scales, float* v_scales, const void* k, const void* v, int kv_heads,
+                            const float* cos_table, const float* sin_table, int tokens, int head_dim, int rotary_dim,
+                            const int32_t* seq_start, const int32_t* pos_base, const int32_t* pos_map,
+                            const int32_t* cache_map, const int32_t* cache_len, int cache_rows, int dtype);
+int clef_qk_norm_rope_kv_write_fp8(clef_stream_t stream, uint8_t* cache_k, uint8_t* cache_v, float* k_scales,
+                                   float* v_scales, const void* k_raw, const void* v, const float* weight,
+                                   const float* cos_table, const float* sin_table, int tokens, int kv_heads, int head_dim,
+                                   int rotary_dim, float eps, const int32_t* seq_start, const int32_t* pos_base,
+                                   const int32_t* pos_map, const int32_t* cache_map, const int32_t* cache_len,
+                                   int cache_rows, int dtype);
+
+/* Reads an FP8 cache back into dense k_out, v_out [rows, kv_heads, head_dim] of the activation dtype: row i is cache row
+ * row_map[i], or i without a map; a row outside 0 .. cache_rows - 1 comes back as zeros. The same row may be read any
+ * number of times. */
+int clef_kv_read_fp8(clef_stream_t stream, void* k_out, void* v_out, const uint8_t* cache_k, const uint8_t* cache_v,
+                     const float* k_scales, const float* v_scales, const int32_t* row_map, int rows, int cache_rows,
+                     int kv_heads, int head_dim, int dtype);
+
 /* ------------------------------------------------------------------------------------------------
  * FP8 (E4M3) activation quantisers, for the FP8 projections of a mixed NVFP4 + FP8 checkpoint.
  * Per quantised row: scale = amax / 448, stored as the upper 16 bits of that f32 (one uint16 per row);
@@ -295,6 +329,14 @@ int clef_swiglu_quantise_fp8(clef_stream_t stream, const void* gate, const void*
  * The reference declines cols != 4096. */
 int clef_rms_norm_fp8_bf16(clef_stream_t stream, const void* x, const float* weight, uint8_t* q_out,
                            uint16_t* q_scales, uint16_t* bf_out, int rows, int cols, float eps, int dtype);
+
+/* The residual add and the next layer's norm + FP8 quantiser in one pass over the row: sum = a + b is written to sum_out
+ * (which may be a or b, and overlaps nothing else) in the activation dtype, and rms_norm_fp8_bf16 of that stored sum to
+ * q_out / q_scales / bf_out (may be NULL). Bytes equal clef_add followed by clef_rms_norm_fp8_bf16 on sum_out. No
+ * counterpart as ONE kernel in the reference. */
+int clef_add_rms_norm_fp8_bf16(clef_stream_t stream, void* sum_out, const void* a, const void* b, const float* weight,
+                               uint8_t* q_out, uint16_t* q_scales, uint16_t* bf_out, int rows, int cols, float eps,
+                               int dtype);
 
 /* rms_norm_gated_quantise_fp8_kernel (kernels/quantise.cu:123-191), Device::rms_norm_gated_quantise_fp8_dev
  * (src/cuda/mod.rs:2304-2328): `rows` head rows of width `cols` (vh per token, rows % vh == 0), one scale
