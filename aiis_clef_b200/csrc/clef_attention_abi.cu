@@ -9,6 +9,7 @@
 
 #include "abi_support.cuh"
 #include "kernels_attention.cuh"
+#include "kernels_attention_mma.cuh"
 
 using namespace clef;
 using namespace clef::abi;
@@ -20,6 +21,7 @@ constexpr int kAttnMaxGroup = 64;
 
 struct AttnPlan {
     int rows;            // R: rows of a row tile
+    bool chunk;          // attn_chunk_kernel, else attn_rows_kernel
     size_t items;        // bound on the (sequence, kv head, row tile) triples
     size_t bytes;        // of the workspace
 };
@@ -27,9 +29,11 @@ struct AttnPlan {
 AttnPlan attn_plan(int n_seqs, int total_q, int q_heads, int kv_heads, int head_dim) {
     AttnPlan p;
     const long long rows = (long long)total_q * (q_heads / kv_heads);
-    p.rows = rows > 8LL * n_seqs ? 16 : 8;
+    p.chunk = rows > 16LL * n_seqs;
+    p.rows = p.chunk ? (head_dim == 256 ? 128 : 256) : (rows > 8LL * n_seqs ? 16 : 8);
     p.items = ((size_t)(rows / p.rows) + n_seqs) * kv_heads;
-    p.bytes = (size_t)kAttnMaxCtas * 2 * (sizeof(int4) + (size_t)p.rows * (head_dim + 2) * sizeof(float));
+    const size_t ctas = p.chunk ? kAttnMaxCtas / 2 : kAttnMaxCtas;
+    p.bytes = (size_t)kAttnMaxCtas * 2 * sizeof(int4) + ctas * 2 * p.rows * (head_dim + 2) * sizeof(float);
     return p;
 }
 
@@ -45,6 +49,34 @@ int allow_smem(K kernel, size_t bytes, std::atomic<unsigned long long>& done, co
     return e == cudaSuccess ? CLEF_OK : fail(CLEF_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+template <typename K, typename... Args>
+void launch_pdl(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    (void)cudaLaunchKernelEx(&cfg, kernel, args...);   // errors surface in check_launch
+}
+
+// Launches `kernel` on the list of units, and the joining kernel where a row tile may have been cut.
+template <typename T, int D, int R, int WPR, typename K>
+int launch_units(K kernel, unsigned threads, size_t smem, size_t most, cudaStream_t s, const AttnArgs& a, const AttnPlan& plan,
+                 const char* what) {
+    const size_t key_tiles = ((size_t)a.table_width * a.page_size + kAttnKeys - 1) / kAttnKeys;
+    const unsigned ctas = clamp_grid(plan.items * key_tiles, most);
+    launch_pdl(kernel, dim3(ctas, 1, 1), threads, smem, s, a);
+    if (int r = check_launch(what)) return r;
+    if (key_tiles <= 1 || ctas <= 1) return CLEF_OK;
+    launch_pdl(attn_combine_kernel<T, D, R, WPR>, dim3(clamp_grid(plan.items, ctas), R * WPR / 8, 1), 256, 0, s, a, (int)ctas);
+    return check_launch(what);
+}
+
 template <typename T, bool FP8, int D, int NT>
 int launch_rows(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const AttnPlan& plan, const char* what) {
     constexpr int R = 8 * NT;
@@ -53,39 +85,33 @@ int launch_rows(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const 
     static std::atomic<int> occ{0};
     auto kernel = attn_rows_kernel<T, FP8, D, NT>;
     if (int r = allow_smem(kernel, smem, allowed, what)) return r;
-    const size_t key_tiles = ((size_t)a.table_width * a.page_size + kAttnKeys - 1) / kAttnKeys;
     size_t most = (size_t)dev.sms * ctas_per_sm(kernel, smem, occ);
     if (most > kAttnMaxCtas) most = kAttnMaxCtas;
-    const unsigned ctas = clamp_grid(plan.items * key_tiles, most);
-    launch_hot(kernel, ctas, smem, s, a);
-    if (int r = check_launch(what)) return r;
-    if (key_tiles <= 1 || ctas <= 1) return CLEF_OK;   // no row tile has been cut
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(clamp_grid(plan.items, ctas), R, 1);
-    cfg.blockDim = dim3(256, 1, 1);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    (void)cudaLaunchKernelEx(&cfg, attn_combine_kernel<T, D, R>, a, (int)ctas);
-    return check_launch(what);
+    return launch_units<T, D, R, 8>(kernel, kAttnThreads, smem, most, s, a, plan, what);
+}
+
+template <typename T, bool FP8, int D>
+int launch_chunk(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const AttnPlan& plan, const char* what) {
+    using Sh = ChunkShape<D>;
+    static std::atomic<unsigned long long> allowed{0};
+    auto kernel = attn_chunk_kernel<T, FP8, D>;
+    if (int r = allow_smem(kernel, Sh::SMEM, allowed, what)) return r;
+    const size_t most = dev.sms < kAttnMaxCtas / 2 ? dev.sms : kAttnMaxCtas / 2;
+    return launch_units<T, D, Sh::R, 1>(kernel, Sh::THREADS, Sh::SMEM, most, s, a, plan, what);
+}
+
+template <typename T, bool FP8, int D>
+int launch_for(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const AttnPlan& plan, const char* what) {
+    if (plan.chunk) return launch_chunk<T, FP8, D>(s, dev, a, plan, what);
+    return plan.rows == 8 ? launch_rows<T, FP8, D, 1>(s, dev, a, plan, what) : launch_rows<T, FP8, D, 2>(s, dev, a, plan, what);
 }
 
 template <typename T, bool FP8>
 int launch_attention(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const AttnPlan& plan, int head_dim,
                      const char* what) {
-#define CLEF_ATTN_ROWS(D) \
-    return plan.rows == 8 ? launch_rows<T, FP8, D, 1>(s, dev, a, plan, what) : launch_rows<T, FP8, D, 2>(s, dev, a, plan, what);
-    if (head_dim == 64) {
-        CLEF_ATTN_ROWS(64)
-    } else if (head_dim == 128) {
-        CLEF_ATTN_ROWS(128)
-    } else {
-        CLEF_ATTN_ROWS(256)
-    }
-#undef CLEF_ATTN_ROWS
+    if (head_dim == 64) return launch_for<T, FP8, 64>(s, dev, a, plan, what);
+    if (head_dim == 128) return launch_for<T, FP8, 128>(s, dev, a, plan, what);
+    return launch_for<T, FP8, 256>(s, dev, a, plan, what);
 }
 
 int check_attention_shape(const char* what, int n_seqs, int total_q, int q_heads, int kv_heads, int head_dim) {

@@ -522,15 +522,16 @@ attn_rows_kernel(AttnArgs a) {
 
 // ---------------------------------------------------------------------------------------------
 // Joins the partials of the row tiles that several CTAs shared: a tile is begun in slot 1 of one CTA and continued in
-// slot 0 of the CTAs after it, up to the one marked last. blockIdx.x takes a run of CTAs as possible beginnings,
-// blockIdx.y a row; the 8 warps split the partials and are joined in shared memory in a fixed order.
+// slot 0 of the CTAs after it, up to the one marked last. blockIdx.x takes a run of CTAs as possible beginnings. WPR
+// warps work on a row, one after the other every WPR-th partial, and are joined in shared memory in a fixed order: a
+// whole block per row where few rows have many partials (attn_rows_kernel), a warp where many rows have few.
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, int R>
+template <typename T, int D, int R, int WPR>
 __global__ void __launch_bounds__(256)
 attn_combine_kernel(AttnArgs a, int ctas) {
-    constexpr int WARPS = 8;
-    __shared__ float s_acc[WARPS][D + 2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int ROWS = 8 / WPR;   // of a block
+    __shared__ float s_acc[8][D + 2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
     pdl_launch_dependents();
     pdl_wait_prior_grids();
     const int from = (int)((long long)blockIdx.x * ctas / gridDim.x), to = (int)((long long)(blockIdx.x + 1) * ctas / gridDim.x);
@@ -538,8 +539,8 @@ attn_combine_kernel(AttnArgs a, int ctas) {
         const int4 d = a.desc[2 * first + 1];
         if (d.w != kAttnFirst) continue;
         const AttnSeq span = attn_seq(a, d.x);
-        const int x = blockIdx.y, row = d.z * R + x;
-        if (row >= span.n * a.group) continue;
+        const int x = blockIdx.y * ROWS + warp / WPR;
+        if (d.z * R + (int)blockIdx.y * ROWS >= span.n * a.group) continue;   // (the same for the whole block)
         int last = first + 1;
         while (last < ctas - 1 && a.desc[2 * last].w != kAttnLast) ++last;
         const int parts = last - first + 1;
@@ -554,7 +555,7 @@ attn_combine_kernel(AttnArgs a, int ctas) {
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) acc[e] = 0.0f;
 #pragma unroll 4
-        for (int i = warp; i < parts; i += WARPS) {
+        for (int i = sub; i < parts; i += WPR) {
             const float* p = part_of(i);
             const float f = fast_exp2(p[x] - ref);
             sum = fmaf(f, p[R + x], sum);
@@ -565,19 +566,22 @@ attn_combine_kernel(AttnArgs a, int ctas) {
         for (int e = 0; e < D / 32; ++e) s_acc[warp][lane + 32 * e] = acc[e];
         if (lane == 0) s_acc[warp][D] = sum;
         __syncthreads();
-        if (threadIdx.x < D / 4) {
+        for (int i = threadIdx.x; i < ROWS * (D / 4); i += 256) {
+            const int r = i / (D / 4), col = (i % (D / 4)) * 4;
+            const int mine = d.z * R + blockIdx.y * ROWS + r;
+            if (mine >= span.n * a.group) break;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             float total = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float* p = s_acc[w] + 4 * threadIdx.x;
-                v.x += p[0], v.y += p[1], v.z += p[2], v.w += p[3];
-                total += s_acc[w][D];
+            for (int w = 0; w < WPR; ++w) {
+                const float* p = s_acc[r * WPR + w];
+                v.x += p[col], v.y += p[col + 1], v.z += p[col + 2], v.w += p[col + 3];
+                total += p[D];
             }
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            const int token = (int)fast_div((uint32_t)row, a.group_div);
+            const int token = (int)fast_div((uint32_t)mine, a.group_div);
             typename T::storage* dst = static_cast<typename T::storage*>(a.out) +
-                ((size_t)(span.q0 + token) * a.q_heads + d.y * a.group + (row - token * a.group)) * D + 4 * threadIdx.x;
+                ((size_t)(span.q0 + token) * a.q_heads + d.y * a.group + (mine - token * a.group)) * D + col;
             store_quad<T>(dst, 0, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         }
         __syncthreads();

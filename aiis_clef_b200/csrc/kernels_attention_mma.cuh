@@ -1,0 +1,570 @@
+// Attention of chunks of new tokens, bound by the products: tcgen05 with accumulators in tensor memory.
+//
+// A CTA has the SM to itself. A row tile is TILES x 128 query rows; per key tile of N keys and per 128 rows
+//   S = Q K^T     [128 x N] f32, both operands K-major in shared memory (128-byte swizzle),
+//   P = exp2(...) bf16, written over S in tensor memory, one thread per row,
+//   O += P V      [128 x D] f32, P read from tensor memory, V [keys][dims] as it lies in the cache (MN-major).
+// Warps are specialised: one warpgroup of softmax per 128 rows, one warpgroup that gathers K and V rows from the pages
+// into a ring of four buffers (K, V, K, V ...), one thread that issues the products. For head_dim 64 and 128 the two
+// row blocks alternate, the products of one run under the softmax of the other; head_dim 256 has tensor memory for one
+// row block only and alternates two S buffers instead, with key tiles of 64 so that the ring fits.
+// The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (weights then stay
+// below 2^8, exact enough in f32 sums and bf16 weights alike), so the softmax rarely touches O.
+//
+// Every wait is bounded: after kWaitLimitNs it gives up, all later waits of the CTA return at once, and the rows the
+// CTA owns come out as NaN.
+#pragma once
+
+#include "kernels_attention.cuh"
+
+namespace clef {
+
+constexpr unsigned long long kWaitLimitNs = 2000000000ull;
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(smem_addr(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ unsigned long long global_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+// Waits for the phase of `parity`; gives up after kWaitLimitNs and raises *gave_up, which ends every later wait.
+__device__ __forceinline__ void mbar_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+    if (mbar_try(bar, parity)) return;
+    const unsigned long long from = global_ns();
+    for (int i = 1; !mbar_try(bar, parity); ++i) {
+        if (*gave_up) return;
+        if ((i & 63) == 0 && global_ns() - from > kWaitLimitNs) {
+            *gave_up = 1;
+            return;
+        }
+    }
+}
+
+// The same for a whole warp, which goes on together (the tensor memory instructions want it converged).
+__device__ __forceinline__ void mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+    mbar_wait(bar, parity, gave_up);
+    __syncwarp();
+}
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// D[128 x N] (tensor memory) (+)= A B^T; A from shared memory or from tensor memory.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+                 : "memory");
+}
+// 32 consecutive f32 columns of this thread's row.
+__device__ __forceinline__ void tc_ld32(uint32_t addr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+                   "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+                   "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const float* v) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+                 "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+                 "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+                 "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand descriptor, 128-byte swizzle: address, leading and stride byte offsets.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// Instruction descriptor: f32 accumulators, bf16 operands, A K-major; B K-major or MN-major.
+__host__ __device__ constexpr uint32_t mma_idesc(int n, bool b_mn_major) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+// Byte offset of 16-byte chunk `chunk` of row `row` in a tile of `rows` rows: 64 columns (128 bytes) side by side, the
+// chunks of a row permuted by the row's low three bits (the hardware's 128-byte swizzle).
+__device__ __forceinline__ uint32_t tile_offset(int row, int chunk, int rows) {
+    return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+template <int D>
+struct ChunkShape {
+    static constexpr int TILES = D == 256 ? 1 : 2;        // row blocks of 128
+    static constexpr int R = 128 * TILES;                 // rows of a row tile
+    static constexpr int N = D == 256 ? 64 : 128;         // keys of a step
+    static constexpr int SBUF = D == 256 ? 2 : 1;         // S buffers per row block
+    static constexpr int RING = 4;                        // K, V, K, V
+    static constexpr int THREADS = 128 * TILES + 128 + 32;
+    static constexpr int Q_BYTES = 128 * D * 2;
+    static constexpr int KV_BYTES = N * D * 2;
+    static constexpr int S_COL = 0;                       // tensor memory columns: S buffers, then O
+    static constexpr int O_COL = TILES * SBUF * N;
+    static constexpr int BAR_COUNT = 2 * RING + 10;
+    static constexpr int SMEM = 1024 + TILES * Q_BYTES + RING * KV_BYTES + 2 * TILES * 2 * N * 4 + 256;
+};
+
+// Steps of a segment [begin, end) of key tiles, the same for every role: whole tiles of N keys, none that lies past the
+// last key a row of the tile sees, one at least.
+template <int D>
+__device__ __forceinline__ void chunk_steps(const AttnArgs& a, const AttnCursor& c, int end, int& keys, int& from, int& to) {
+    constexpr int PER = kAttnKeys / ChunkShape<D>::N;
+    keys = attn_visible(a, c.span, min((c.tile + 1) * ChunkShape<D>::R, c.span.n * a.group));
+    from = c.key_tile * PER;
+    to = max(from + 1, min(end * PER, (keys + ChunkShape<D>::N - 1) / ChunkShape<D>::N));
+}
+
+template <typename T, bool FP8, int D>
+__global__ void __launch_bounds__(ChunkShape<D>::THREADS, 1)
+attn_chunk_kernel(AttnArgs a) {
+    using Sh = ChunkShape<D>;
+    constexpr int TILES = Sh::TILES, R = Sh::R, N = Sh::N, SBUF = Sh::SBUF, RING = Sh::RING;
+    extern __shared__ uint8_t s_raw[];
+    __shared__ uint64_t full[RING], empty[RING], q_ready[TILES], s_ready[TILES * SBUF], p_ready[TILES * SBUF], pv_done[TILES], drained;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_gave_up;
+    __shared__ AttnCursor s_cursor;
+    uint8_t* s_base = s_raw + ((1024 - (smem_addr(s_raw) & 1023)) & 1023);
+    uint8_t* s_q = s_base;
+    uint8_t* s_kv = s_q + TILES * Sh::Q_BYTES;
+    float* s_scale = reinterpret_cast<float*>(s_kv + RING * Sh::KV_BYTES);   // FP8: [TILES][2][k, v][N]
+    volatile int* gave_up = &s_gave_up;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < RING; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
+        for (int i = 0; i < TILES; ++i) mbar_init(&q_ready[i], 128), mbar_init(&pv_done[i], 1);
+        for (int i = 0; i < TILES * SBUF; ++i) mbar_init(&s_ready[i], 1), mbar_init(&p_ready[i], 128);
+        mbar_init(&drained, 1);
+        s_gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    pdl_launch_dependents();
+    pdl_wait_prior_grids();
+    if (warp == 0) {
+        const AttnCursor c = attn_locate<R>(a, blockIdx.x, gridDim.x);
+        if (lane == 0) s_cursor = c;
+    }
+    int4* desc = a.desc + 2 * blockIdx.x;
+    if (threadIdx.x < 2) desc[threadIdx.x].w = kAttnNone;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    AttnCursor cur = s_cursor;
+
+    if (warp < kProducerWarp) {
+        // ---- softmax: thread = row -------------------------------------------------------------------------------
+        const int t = warp >> 2;                                    // row block
+        const int x = threadIdx.x & 127;                            // row of the block = tensor memory lane
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;          // (32 (warp % 4)) << 16
+        const uint32_t o_addr = tmem + lanes + Sh::O_COL + t * D;
+        uint8_t* q_tile = s_q + t * Sh::Q_BYTES;
+        const float scale = fabsf(a.scale_log2);
+        const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale negates q instead
+        float* scales = s_scale + t * 4 * N;
+        int steps_done = 0;                                         // of this row block, over all segments
+        while (cur.left > 0) {
+            const int begin = cur.key_tile, end = (int)min((long long)cur.units, begin + cur.left);
+            const AttnSeq span = cur.span;
+            const int rows = span.n * a.group, row0 = cur.tile * R + t * 128;
+            int keys, from, to;
+            chunk_steps<D>(a, cur, end, keys, from, to);
+            if (row0 < rows) {
+                // q: 16-byte chunks, eight lanes to a 128-byte line, rounded to bf16, into the swizzled tile
+                for (int i = x; i < 128 * (D / 8); i += 128) {
+                    const int r = i / (D / 8), ch = i % (D / 8), y = row0 + r;
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (y < rows) {
+                        const int token = (int)fast_div((uint32_t)y, a.group_div);
+                        const size_t at = ((size_t)(span.q0 + token) * a.q_heads + cur.head * a.group + (y - token * a.group)) * D + ch * 8;
+                        float f[8];
+                        const float4 f0 = load_quad<T>(static_cast<const typename T::storage*>(a.q) + at, 0);
+                        const float4 f1 = load_quad<T>(static_cast<const typename T::storage*>(a.q) + at, 1);
+                        f[0] = f0.x, f[1] = f0.y, f[2] = f0.z, f[3] = f0.w, f[4] = f1.x, f[5] = f1.y, f[6] = f1.z, f[7] = f1.w;
+                        w = make_uint4(pack_bf16x2(f[0], f[1]) ^ flip, pack_bf16x2(f[2], f[3]) ^ flip, pack_bf16x2(f[4], f[5]) ^ flip,
+                                       pack_bf16x2(f[6], f[7]) ^ flip);
+                    }
+                    *reinterpret_cast<uint4*>(q_tile + tile_offset(r, ch, 128)) = w;
+                }
+                async_proxy_fence();
+                mbar_arrive(&q_ready[t]);
+                const int lim = row0 + x < rows ? attn_visible(a, span, row0 + x + 1) : 0;
+                float m = -INFINITY, l = 0.0f;
+                // FP8: thread x fetches the scales of key x of a step, one step ahead
+                float ks = 0.0f, vs = 0.0f;
+                auto fetch_scales = [&](int step) {
+                    const int key = step * N + x;
+                    const int row = x < N && step < to && key < keys ? attn_cache_row(a, cur.seq, key) : -1;
+                    const size_t at = (size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head;
+                    ks = row < 0 ? 0.0f : a.k_scales[at];
+                    vs = row < 0 ? 0.0f : a.v_scales[at];
+                };
+                if (FP8) fetch_scales(from);
+                for (int step = from; step < to; ++step, ++steps_done) {
+                    const int buf = SBUF == 1 ? 0 : (steps_done & 1);
+                    const uint32_t s_addr = tmem + lanes + Sh::S_COL + (t * SBUF + buf) * N;
+                    const uint32_t s_parity = (SBUF == 1 ? steps_done : steps_done >> 1) & 1;
+                    float* sc = scales + (steps_done & 1) * 2 * N;
+                    if (FP8) {
+                        if (x < N) sc[x] = ks * scale, sc[N + x] = vs;
+                        asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+                        fetch_scales(step + 1);
+                    }
+                    mbar_wait_warp(&s_ready[t * SBUF + buf], s_parity, gave_up);
+                    tc_fence_after();
+                    const int base = step * N;
+                    const bool edge = __any_sync(kFullMask, base + N > lim);   // some keys of the step are hidden from some row
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < N; c += 32) {
+                        float s[32];
+                        tc_ld32(s_addr + c, s);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            if (FP8) {
+                                const float4 k4 = *reinterpret_cast<const float4*>(sc + c + i);
+                                s[i] *= k4.x, s[i + 1] *= k4.y, s[i + 2] *= k4.z, s[i + 3] *= k4.w;
+                            }
+                        }
+                        if (edge) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) s[i] = base + c + i < lim ? s[i] : -INFINITY;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
+                    }
+                    if (!FP8) top = top == -INFINITY ? top : top * scale;
+                    const bool grown = top > m + 8.0f;   // (m = -inf: any key at all)
+                    if (__any_sync(kFullMask, grown)) {
+                        const float now = grown ? top : m;
+                        const float fix = now == m ? 1.0f : fast_exp2(m - now);
+                        l *= fix;
+                        m = now;
+                        if (step > from) {
+                            if (SBUF == 2) {   // S of this step was ready before the last product with P had ended
+                                mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
+                                tc_fence_after();
+                            }   // (with one S buffer its product came after that one)
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 32) {
+                                float o[32];
+                                tc_ld32(o_addr + c, o);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] *= fix;
+                                tc_st32(o_addr + c, o);
+                            }
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+                    for (int c = 0; c < N; c += 32) {
+                        float s[32];
+                        tc_ld32(s_addr + c, s);
+                        tc_wait_ld();
+                        uint32_t p[16];
+                        float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            float4 k4 = make_float4(scale, scale, scale, scale), v4 = make_float4(1.f, 1.f, 1.f, 1.f);
+                            if (FP8) {
+                                k4 = *reinterpret_cast<const float4*>(sc + c + i);
+                                v4 = *reinterpret_cast<const float4*>(sc + N + c + i);
+                            }
+                            float e0 = fmaf(s[i], k4.x, ref), e1 = fmaf(s[i + 1], k4.y, ref);
+                            float e2 = fmaf(s[i + 2], k4.z, ref), e3 = fmaf(s[i + 3], k4.w, ref);
+                            if (edge) {
+                                e0 = base + c + i < lim ? e0 : -INFINITY, e1 = base + c + i + 1 < lim ? e1 : -INFINITY;
+                                e2 = base + c + i + 2 < lim ? e2 : -INFINITY, e3 = base + c + i + 3 < lim ? e3 : -INFINITY;
+                            }
+                            e0 = fast_exp2(e0), e1 = fast_exp2(e1), e2 = fast_exp2(e2), e3 = fast_exp2(e3);
+                            sum0 += e0 + e1;
+                            sum1 += e2 + e3;
+                            if (FP8) {
+                                e0 *= v4.x, e1 *= v4.y, e2 *= v4.z, e3 *= v4.w;
+                                if (edge) {   // whatever scale a hidden key has, its weight is 0
+                                    e0 = base + c + i < lim ? e0 : 0.0f, e1 = base + c + i + 1 < lim ? e1 : 0.0f;
+                                    e2 = base + c + i + 2 < lim ? e2 : 0.0f, e3 = base + c + i + 3 < lim ? e3 : 0.0f;
+                                }
+                            }
+                            p[i / 2] = pack_bf16x2(e0, e1);
+                            p[i / 2 + 1] = pack_bf16x2(e2, e3);
+                        }
+                        l += sum0 + sum1;
+                        tc_st16(s_addr + c / 2, p);   // over columns of S that are read already
+                    }
+                    tc_wait_st();
+                    tc_fence_before();
+                    // pv_done is waited for once a step, so that its phase is never more than one ahead of the wait
+                    if (SBUF == 2 && steps_done > 0) mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
+                    mbar_arrive(&p_ready[t * SBUF + buf]);
+                }
+                mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
+                tc_fence_after();
+                const bool whole = begin == 0 && end == cur.units;
+                const bool live = row0 + x < rows;
+                const int slot = begin == 0 ? 1 : 0;
+                float* part = attn_slot(a, blockIdx.x, slot, R, D);
+                if (!whole) {
+                    if (threadIdx.x == 0) {
+                        desc[slot] = make_int4(cur.seq, cur.head, cur.tile, begin == 0 ? kAttnFirst : (end == cur.units ? kAttnLast : kAttnMiddle));
+                    }
+                    part[t * 128 + x] = m;
+                    part[R + t * 128 + x] = *gave_up ? __int_as_float(0x7fc00000) : l;
+                }
+                float f = 1.0f;
+                if (whole) f = l == 0.0f ? 0.0f : 1.0f / l;
+                if (*gave_up) f = __int_as_float(0x7fc00000);
+                const int token = (int)fast_div((uint32_t)(row0 + x), a.group_div);
+                typename T::storage* dst = static_cast<typename T::storage*>(a.out) +
+                    ((size_t)(span.q0 + token) * a.q_heads + cur.head * a.group + (row0 + x - token * a.group)) * D;
+                float* pdst = part + 2 * R + (size_t)(t * 128 + x) * D;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    tc_ld32(o_addr + c, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = f == 0.0f ? 0.0f : o[i] * f;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        if (!live) break;
+                        if (whole && T::kBytes == 2) {
+                            stg_v4(dst + c + i, make_uint4(pack_bf16x2(o[i], o[i + 1]), pack_bf16x2(o[i + 2], o[i + 3]),
+                                                           pack_bf16x2(o[i + 4], o[i + 5]), pack_bf16x2(o[i + 6], o[i + 7])));
+                        } else {
+                            float* to_f32 = whole ? reinterpret_cast<float*>(dst) : pdst;
+                            *reinterpret_cast<float4*>(to_f32 + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                            *reinterpret_cast<float4*>(to_f32 + c + i + 4) = make_float4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                tc_fence_before();
+            }
+            cur.left -= end - begin;
+            if (cur.left > 0) attn_advance<R>(a, cur);
+        }
+    } else if (warp < kMmaWarp) {
+        // ---- producers: a warp gathers N / 4 rows of each tile, lane l of it knows row l's place ----------------
+        constexpr int ROWS = N / 4;                       // rows per warp
+        const int w = warp - kProducerWarp;
+        using CacheT = typename std::conditional<FP8, uint8_t, uint16_t>::type;
+        constexpr int CPR = D * (FP8 ? 1 : 2) / 16;       // 16-byte pieces of a cache row
+        constexpr int RPI = 32 / (CPR < 8 ? CPR : 8);     // rows a warp touches at once
+        constexpr int LPR = 32 / RPI;                     // lanes per row
+        uint32_t item = 0;
+        while (cur.left > 0) {
+            const int end = (int)min((long long)cur.units, cur.key_tile + cur.left);
+            const int taken = end - cur.key_tile;
+            int keys, from, to;
+            chunk_steps<D>(a, cur, end, keys, from, to);
+            auto lookup = [&](int step) {
+                const int key = step * N + w * ROWS + (lane % ROWS);
+                return step < to && key < keys ? attn_cache_row(a, cur.seq, key) : -1;
+            };
+            int row32 = lookup(from);
+            for (int step = from; step < to; ++step) {
+                const int ahead = lookup(step + 1);
+#pragma unroll
+                for (int which = 0; which < 2; ++which, ++item) {
+                    const uint32_t slot = item % RING;
+                    uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
+                    const CacheT* src = static_cast<const CacheT*>(which == 0 ? a.k : a.v);
+                    if (!FP8) {
+                        mbar_wait(&empty[slot], ((item / RING) & 1) ^ 1, gave_up);
+#pragma unroll
+                        for (int i = 0; i < ROWS / RPI; ++i) {
+                            const int r = i * RPI + lane / LPR;
+                            const int row = __shfl_sync(kFullMask, row32, r);
+                            const uint8_t* p = reinterpret_cast<const uint8_t*>(src + ((size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head) * D);
+#pragma unroll
+                            for (int ch = lane % LPR; ch < CPR; ch += LPR) {
+                                const uint32_t dst = smem_addr(tile + tile_offset(w * ROWS + r, ch, N));
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p + 16 * ch), "r"(row < 0 ? 0 : 16)
+                                             : "memory");
+                            }
+                        }
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        if (item >= 2) {   // two items stay in flight; the one before them is complete: hand it over
+                            asm volatile("cp.async.wait_group 2;" ::: "memory");
+                            async_proxy_fence();
+                            mbar_arrive(&full[(item - 2) % RING]);
+                        }
+                    } else {
+                        uint4 code[ROWS / RPI][CPR / LPR];
+#pragma unroll
+                        for (int i = 0; i < ROWS / RPI; ++i) {
+                            const int row = __shfl_sync(kFullMask, row32, i * RPI + lane / LPR);
+                            const uint8_t* p = reinterpret_cast<const uint8_t*>(src + ((size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head) * D);
+#pragma unroll
+                            for (int j = 0; j < CPR / LPR; ++j) {
+                                code[i][j] = row < 0 ? make_uint4(0, 0, 0, 0) : ldg_stream_v4(p + 16 * (lane % LPR + j * LPR));
+                            }
+                        }
+                        mbar_wait(&empty[slot], ((item / RING) & 1) ^ 1, gave_up);
+#pragma unroll
+                        for (int i = 0; i < ROWS / RPI; ++i) {
+                            const int r = w * ROWS + i * RPI + lane / LPR;
+#pragma unroll
+                            for (int j = 0; j < CPR / LPR; ++j) {
+                                const int ch = 2 * (lane % LPR + j * LPR);
+                                uint4 lo, hi;
+                                e4m3x4_to_bf16(code[i][j].x, lo.x, lo.y);
+                                e4m3x4_to_bf16(code[i][j].y, lo.z, lo.w);
+                                e4m3x4_to_bf16(code[i][j].z, hi.x, hi.y);
+                                e4m3x4_to_bf16(code[i][j].w, hi.z, hi.w);
+                                *reinterpret_cast<uint4*>(tile + tile_offset(r, ch, N)) = lo;
+                                *reinterpret_cast<uint4*>(tile + tile_offset(r, ch + 1, N)) = hi;
+                            }
+                        }
+                        async_proxy_fence();
+                        mbar_arrive(&full[slot]);
+                    }
+                }
+                row32 = ahead;
+            }
+            cur.left -= taken;
+            if (cur.left > 0) attn_advance<R>(a, cur);
+        }
+        if (!FP8 && item > 0) {   // an even number of items, two at least: the last two are still to be handed over
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            async_proxy_fence();
+            mbar_arrive(&full[(item - 2) % RING]);
+            mbar_arrive(&full[(item - 1) % RING]);
+        }
+    } else if (lane == 0) {
+        // ---- products: one thread ----------------------------------------------------------------------------------
+        constexpr uint32_t s_idesc = mma_idesc(N, false), o_idesc = mma_idesc(D, true);
+        uint32_t item = 0;                // K and V tiles consumed so far
+        int segments[TILES] = {}, steps_done[TILES] = {};
+        auto scores = [&](int t, int nth, uint32_t k_item) {   // S of the nth step of row block t
+            const int buf = SBUF == 1 ? 0 : (nth & 1);
+            const uint32_t q_at = smem_addr(s_q + t * Sh::Q_BYTES), k_at = smem_addr(s_kv + (k_item % RING) * Sh::KV_BYTES);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                const uint64_t qa = smem_desc(q_at + (k >> 2) * 128 * 128 + (k & 3) * 32, 16, 1024);
+                const uint64_t kb = smem_desc(k_at + (k >> 2) * N * 128 + (k & 3) * 32, 16, 1024);
+                tc_mma_ss(tmem + Sh::S_COL + (t * SBUF + buf) * N, qa, kb, s_idesc, k > 0);
+            }
+            tc_commit(&s_ready[t * SBUF + buf]);
+        };
+        auto outputs = [&](int t, int nth, uint32_t v_item, bool add) {
+            const int buf = SBUF == 1 ? 0 : (nth & 1);
+            const uint32_t v_at = smem_addr(s_kv + (v_item % RING) * Sh::KV_BYTES);
+#pragma unroll
+            for (int k = 0; k < N / 16; ++k) {
+                const uint64_t vb = smem_desc(v_at + k * 2048, N * 128, 1024);
+                tc_mma_ts(tmem + Sh::O_COL + t * D, tmem + Sh::S_COL + (t * SBUF + buf) * N + 8 * k, vb, o_idesc, add || k > 0);
+            }
+            tc_commit(&pv_done[t]);
+        };
+        while (cur.left > 0) {
+            const int end = (int)min((long long)cur.units, cur.key_tile + cur.left);
+            const int taken = end - cur.key_tile;
+            int keys, from, to;
+            chunk_steps<D>(a, cur, end, keys, from, to);
+            const int blocks = cur.span.n * a.group - cur.tile * R > 128 ? TILES : 1;
+            const int count = to - from;
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                if (t < blocks) mbar_wait(&q_ready[t], segments[t]++ & 1, gave_up);
+            }
+            // the first SBUF steps' scores, then for each step its output and the scores SBUF steps later
+            for (int j = 0; j < SBUF && j < count; ++j) {
+                const uint32_t k_item = item + 2 * j;
+                mbar_wait(&full[k_item % RING], (k_item / RING) & 1, gave_up);
+                tc_fence_after();
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    if (t < blocks) scores(t, steps_done[t] + j, k_item);
+                }
+                tc_commit(&empty[k_item % RING]);
+            }
+            for (int j = 0; j < count; ++j) {
+                const uint32_t v_item = item + 2 * j + 1, k_item = item + 2 * (j + SBUF);
+                mbar_wait(&full[v_item % RING], (v_item / RING) & 1, gave_up);
+                const bool more = j + SBUF < count;
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    if (t >= blocks) break;
+                    const int nth = steps_done[t] + j;
+                    const int buf = SBUF == 1 ? 0 : (nth & 1);
+                    mbar_wait(&p_ready[t * SBUF + buf], (SBUF == 1 ? nth : nth >> 1) & 1, gave_up);
+                    tc_fence_after();
+                    outputs(t, nth, v_item, j > 0);
+                    if (t == blocks - 1) tc_commit(&empty[v_item % RING]);
+                    if (more) {
+                        if (t == 0) {
+                            mbar_wait(&full[k_item % RING], (k_item / RING) & 1, gave_up);
+                            tc_fence_after();
+                        }
+                        scores(t, nth + SBUF, k_item);
+                        if (t == blocks - 1) tc_commit(&empty[k_item % RING]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) steps_done[t] += t < blocks ? count : 0;
+            item += 2 * count;
+            cur.left -= taken;
+            if (cur.left > 0) attn_advance<R>(a, cur);
+        }
+        // every product and every arrival it triggers has landed before the CTA goes (also after a wait that gave up)
+        tc_commit(&drained);
+        for (int i = 0; i < (1 << 20) && !mbar_try(&drained, 0); ++i) {
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+}  // namespace clef
