@@ -33,7 +33,7 @@ AttnPlan attn_plan(int n_seqs, int total_q, int q_heads, int kv_heads, int head_
     p.rows = p.chunk ? (head_dim == 256 ? 128 : 256) : (rows > 8LL * n_seqs ? 16 : 8);
     p.items = ((size_t)(rows / p.rows) + n_seqs) * kv_heads;
     const size_t ctas = p.chunk ? kAttnMaxCtas / 2 : kAttnMaxCtas;
-    p.bytes = (size_t)kAttnMaxCtas * 2 * sizeof(int4) + ctas * 2 * p.rows * (head_dim + 2) * sizeof(float);
+    p.bytes = (size_t)kAttnMaxCtas * 2 * sizeof(AttnDesc) + ctas * 2 * p.rows * (head_dim + 2) * sizeof(float);
     return p;
 }
 
@@ -65,7 +65,7 @@ void launch_pdl(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t
 }
 
 // Launches `kernel` on the list of units, and the joining kernel where a row tile may have been cut.
-template <typename T, int D, int R, int WPR, typename K>
+template <typename T, int D, int R, bool ROWS, typename K>
 int launch_units(K kernel, unsigned threads, size_t smem, size_t most, cudaStream_t s, const AttnArgs& a, const AttnPlan& plan,
                  const char* what) {
     const size_t key_tiles = ((size_t)a.table_width * a.page_size + kAttnKeys - 1) / kAttnKeys;
@@ -73,7 +73,9 @@ int launch_units(K kernel, unsigned threads, size_t smem, size_t most, cudaStrea
     launch_pdl(kernel, dim3(ctas, 1, 1), threads, smem, s, a);
     if (int r = check_launch(what)) return r;
     if (key_tiles <= 1 || ctas <= 1) return CLEF_OK;
-    launch_pdl(attn_combine_kernel<T, D, R, WPR>, dim3(clamp_grid(plan.items, ctas), R * WPR / 8, 1), 256, 0, s, a, (int)ctas);
+    const unsigned runs = clamp_grid(plan.items, ctas);
+    if constexpr (ROWS) launch_pdl(attn_combine_rows_kernel<T, D, R>, dim3(runs, R / 32, 1), 256, 0, s, a, (int)ctas);
+    else launch_pdl(attn_combine_kernel<T, D, R>, dim3(runs, R, 1), 256, 0, s, a, (int)ctas);
     return check_launch(what);
 }
 
@@ -87,7 +89,7 @@ int launch_rows(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const 
     if (int r = allow_smem(kernel, smem, allowed, what)) return r;
     size_t most = (size_t)dev.sms * ctas_per_sm(kernel, smem, occ);
     if (most > kAttnMaxCtas) most = kAttnMaxCtas;
-    return launch_units<T, D, R, 8>(kernel, kAttnThreads, smem, most, s, a, plan, what);
+    return launch_units<T, D, R, false>(kernel, kAttnThreads, smem, most, s, a, plan, what);
 }
 
 template <typename T, bool FP8, int D>
@@ -97,7 +99,7 @@ int launch_chunk(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const
     auto kernel = attn_chunk_kernel<T, FP8, D>;
     if (int r = allow_smem(kernel, Sh::SMEM, allowed, what)) return r;
     const size_t most = dev.sms < kAttnMaxCtas / 2 ? dev.sms : kAttnMaxCtas / 2;
-    return launch_units<T, D, Sh::R, 1>(kernel, Sh::THREADS, Sh::SMEM, most, s, a, plan, what);
+    return launch_units<T, D, Sh::R, true>(kernel, Sh::THREADS, Sh::SMEM, most, s, a, plan, what);
 }
 
 template <typename T, bool FP8, int D>
@@ -183,7 +185,7 @@ int clef_paged_attention(clef_stream_t stream, void* out, const void* q, const v
     a.page_size = page_size, a.table_width = table_width, a.cache_pages = cache_pages;
     a.group_div = make_fast_div((uint32_t)group), a.page_div = make_fast_div((uint32_t)page_size);
     a.scale_log2 = scale * 1.44269504088896341f;
-    a.desc = static_cast<int4*>(workspace);
+    a.desc = static_cast<AttnDesc*>(workspace);
     a.part = reinterpret_cast<float*>(a.desc + 2 * kAttnMaxCtas);
     cudaStream_t s = as_stream(stream);
     if (dtype == CLEF_BF16) {

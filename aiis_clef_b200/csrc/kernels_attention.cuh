@@ -16,6 +16,7 @@
 
 #include "common.cuh"
 #include "f32x2.cuh"
+#include "kernels_generic.cuh"
 #include "kernels_hot.cuh"
 
 namespace clef {
@@ -37,13 +38,17 @@ struct AttnArgs {
     int page_size, table_width, cache_pages;
     FastDiv group_div, page_div;
     float scale_log2;           // scale * log2(e): the softmax runs on exp2
-    int4* desc;                 // workspace: two slots per CTA, {sequence, head, row tile, state}
-    float* part;                // workspace: per slot R maxima, R sums, R x head_dim outputs
+    struct AttnDesc* desc;      // workspace: what is in the two slots of each CTA
+    float* part;                // workspace: per slot R maxima, R sums, R x head_dim outputs (attn_chunk_kernel: [head_dim / 4][R][4])
 };
 
 // Slot states. Slot 0 of a CTA holds the end (or the middle) of a row tile begun by an earlier CTA, slot 1 the
 // beginning of one that a later CTA ends.
 enum AttnSlot { kAttnNone = 0, kAttnFirst = 1, kAttnMiddle = 2, kAttnLast = 3 };
+struct AttnDesc {
+    int state, tile, head, q0, rows;   // rows: of the sequence and kv head
+    int unused[3];
+};
 
 __device__ __forceinline__ float fast_exp2(float x) {
     float r;
@@ -67,75 +72,60 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int s) {
 __device__ __forceinline__ int attn_visible(const AttnArgs& a, const AttnSeq& q, int rows) {
     return max(0, q.kv - q.n + (int)fast_div((uint32_t)(rows - 1), a.group_div) + 1);
 }
-// Units of row tile `tile`: its key tiles, at least one (a row that sees nothing still has to be written).
+// Key tiles of row tile `tile`, at least one (a row that sees nothing still has to be written).
 template <int R>
-__device__ __forceinline__ int attn_tile_units(const AttnArgs& a, const AttnSeq& q, int tile) {
+__device__ __forceinline__ int attn_key_tiles(const AttnArgs& a, const AttnSeq& q, int tile) {
     const int rows = min((tile + 1) * R, q.n * a.group);
     return max(1, (attn_visible(a, q, rows) + kAttnKeys - 1) / kAttnKeys);
 }
 
-// sum over i < n of floor((step i + first) / m), all non-negative, m > 0: reduce step and first modulo m, then count
-// the lattice points under the line by columns of the exchanged axes (Euclid's algorithm on (step, m)).
-__device__ inline long long floor_sum(long long n, long long m, long long step, long long first) {
-    long long total = 0;
-    while (n > 0) {
-        if (step >= m) {
-            total += (n * (n - 1) / 2) * (step / m);
-            step %= m;
-        }
-        if (first >= m) {
-            total += n * (first / m);
-            first %= m;
-        }
-        const long long top = step * n + first;
-        if (top < m) break;
-        n = top / m;
-        first = top % m;
-        const long long t = m;
-        m = step;
-        step = t;
-    }
-    return total;
+// Work is shared out by a cost that is linear in the row tile's number, so that sums over row tiles need no loop and no
+// division: a row tile of a sequence with kv - n cached keys before its new ones costs
+//   OV * unit + max(0, (kv - n) * group + (tile + 1) R)      with unit = group * kAttnKeys the cost of a key tile,
+// which is `group` times the keys its last row sees, and OV key tiles' worth for its beginning and end.
+template <int R, int OV>
+__device__ __forceinline__ long long attn_tile_cost(const AttnArgs& a, const AttnSeq& q, int tile) {
+    return (long long)OV * a.group * kAttnKeys + max(0, (q.kv - q.n) * a.group + (tile + 1) * R);
 }
-
-// Units of all row tiles of one (sequence, kv head). A full tile i sees floor((A + i R) / (group keys)) + 1 key tiles
-// with A = (kv - n) group + R - 1 (1 where that is below 1), the last tile ceil(kv / keys).
-template <int R>
-__device__ inline long long attn_seq_units(const AttnArgs& a, const AttnSeq& q) {
+// Cost of all row tiles of one (sequence, kv head).
+template <int R, int OV>
+__device__ __forceinline__ long long attn_seq_cost(const AttnArgs& a, const AttnSeq& q) {
     const int tiles = (q.n * a.group + R - 1) / R;
-    if (tiles == 0) return 0;
-    const long long full = tiles - 1, m = (long long)a.group * kAttnKeys;
-    const long long A = (long long)(q.kv - q.n) * a.group + R - 1;
-    const long long skip = A >= 0 ? 0 : min(full, (-A + R - 1) / R);
-    return full + floor_sum(full - skip, m, R, A + skip * R) + max(1, (q.kv + kAttnKeys - 1) / kAttnKeys);
+    const int ahead = (q.kv - q.n) * a.group;
+    const int none = ahead >= 0 ? 0 : min(tiles, -ahead / R);   // row tiles whose linear part is 0
+    const long long some = tiles - none;
+    return (long long)tiles * OV * a.group * kAttnKeys + some * ahead + (long long)R * (some * (none + 1) + some * (some - 1) / 2);
 }
 
-// A CTA's place in the list of units: (sequence, kv head, row tile, key tile), and how many units are left to it.
+// A CTA's place in the list: (sequence, kv head, row tile), the row tile's cost, how much of it lies before the CTA's
+// share, and how much of the share is left.
 struct AttnCursor {
-    int seq, head, tile, key_tile, units;   // `units` of the row tile
+    int seq, head, tile, keys;   // `keys`: key tiles of the row tile
     AttnSeq span;
-    long long left;
+    long long cost, at, left;
 };
 
-// The cursor of CTA `cta` of `ctas`: unit floor(cta * total / ctas) on. One warp, all lanes; every lane has the result.
-template <int R>
+// The cursor of CTA `cta` of `ctas`. One warp, all lanes; every lane has the result.
+template <int R, int OV>
 __device__ inline AttnCursor attn_locate(const AttnArgs& a, int cta, int ctas) {
     const int lane = threadIdx.x & 31;
+    AttnCursor c;
+    c.seq = c.head = c.tile = c.keys = 0;
+    c.span = AttnSeq{0, 0, 0};
+    c.cost = c.at = 0;
     long long total = 0;
-    for (int s = lane; s < a.n_seqs; s += 32) total += a.kv_heads * attn_seq_units<R>(a, attn_seq(a, s));
+    for (int s = lane; s < a.n_seqs; s += 32) total += a.kv_heads * attn_seq_cost<R, OV>(a, attn_seq(a, s));
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(kFullMask, total, off);
-    AttnCursor c;
-    if (total < ctas) ctas = (int)total;   // the CTAs that work are the first ones, with a unit each at least
-    long long at = cta < ctas ? cta * total / ctas : 0;
-    c.left = cta < ctas ? (cta + 1) * total / ctas - at : 0;
-    c.seq = c.head = c.tile = c.key_tile = c.units = 0;
-    c.span = AttnSeq{0, 0, 0};
-    if (c.left == 0) return c;
+    // equal shares, but of a key tile at least: the CTAs that work are the first ones
+    const long long share = max((total + ctas - 1) / ctas, (long long)a.group * kAttnKeys);
+    long long at = cta * share;
+    c.left = min(share, total - at);
+    if (c.left <= 0) return c;
     long long per_head = 0;
     for (int base = 0; base < a.n_seqs; base += 32) {   // the sequence: scans of 32
         const int s = base + lane;
-        const long long mine = s < a.n_seqs ? attn_seq_units<R>(a, attn_seq(a, s)) : 0;
+        const long long mine = s < a.n_seqs ? attn_seq_cost<R, OV>(a, attn_seq(a, s)) : 0;
         long long upto = mine * a.kv_heads;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -153,34 +143,50 @@ __device__ inline AttnCursor attn_locate(const AttnArgs& a, int cta, int ctas) {
         at -= __shfl_sync(kFullMask, upto, 31);
     }
     c.span = attn_seq(a, c.seq);
-    c.head = (int)(at / per_head);
-    at -= c.head * per_head;
+    for (; at >= per_head; at -= per_head) ++c.head;
     const int tiles = (c.span.n * a.group + R - 1) / R;
     for (int base = 0; base < tiles; base += 32) {      // the row tile: scans of 32
-        const int mine = base + lane < tiles ? attn_tile_units<R>(a, c.span, base + lane) : 0;
-        int upto = mine;
+        const long long mine = base + lane < tiles ? attn_tile_cost<R, OV>(a, c.span, base + lane) : 0;
+        long long upto = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const int t = __shfl_up_sync(kFullMask, upto, off);
+            const long long t = __shfl_up_sync(kFullMask, upto, off);
             if (lane >= off) upto += t;
         }
-        const unsigned past = __ballot_sync(kFullMask, (long long)upto > at);
+        const unsigned past = __ballot_sync(kFullMask, upto > at);
         if (past) {
             const int hit = __ffs(past) - 1;
             c.tile = base + hit;
-            c.units = __shfl_sync(kFullMask, mine, hit);
-            c.key_tile = (int)at - (__shfl_sync(kFullMask, upto, hit) - c.units);
+            c.cost = __shfl_sync(kFullMask, mine, hit);
+            c.at = at - (__shfl_sync(kFullMask, upto, hit) - c.cost);
             break;
         }
         at -= __shfl_sync(kFullMask, upto, 31);
     }
+    c.keys = attn_key_tiles<R>(a, c.span, c.tile);
     return c;
 }
 
-// On to the next row tile (called with units left: there is one).
-template <int R>
+// The key tiles [begin, end) of the cursor's row tile that fall to its CTA: where a share ends at cost x of a row tile, the
+// key tiles before it are those of round((x - OV units) / unit); none, if it ends within the OV units (the next CTA then
+// begins the row tile), all, if the row tile ends in the share.
+template <int OV>
+__device__ __forceinline__ void attn_segment(const AttnArgs& a, const AttnCursor& c, int& begin, int& end) {
+    const int unit = a.group * kAttnKeys;
+    auto before = [&](long long x) {
+        const int y = (int)(x - (long long)OV * unit) + unit / 2;
+        return y <= 0 ? 0 : min(c.keys, y / unit);
+    };
+    begin = before(c.at);
+    end = c.at + c.left >= c.cost ? c.keys : before(c.at + c.left);
+}
+
+// On to the next row tile, if some of the share is left.
+template <int R, int OV>
 __device__ __forceinline__ void attn_advance(const AttnArgs& a, AttnCursor& c) {
-    c.key_tile = 0;
+    c.left -= c.cost - c.at;
+    if (c.left <= 0) return;
+    c.at = 0;
     if ((c.tile + 1) * R < c.span.n * a.group) {
         ++c.tile;
     } else {
@@ -193,7 +199,8 @@ __device__ __forceinline__ void attn_advance(const AttnArgs& a, AttnCursor& c) {
             } while (c.span.n == 0 && c.seq + 1 < a.n_seqs);
         }
     }
-    c.units = attn_tile_units<R>(a, c.span, c.tile);
+    c.cost = attn_tile_cost<R, OV>(a, c.span, c.tile);
+    c.keys = attn_key_tiles<R>(a, c.span, c.tile);
 }
 
 __device__ __forceinline__ float* attn_slot(const AttnArgs& a, int cta, int slot, int rows, int head_dim) {
@@ -241,7 +248,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 template <typename T, bool FP8, int D, int NT>
 __global__ void __launch_bounds__(kAttnThreads, (D == 256 || NT > 1 || !FP8) ? 1 : 2)
 attn_rows_kernel(AttnArgs a) {
-    constexpr int R = 8 * NT;
+    constexpr int R = 8 * NT, OV = 1;
     constexpr int WARPS = kAttnThreads / 32;
     constexpr int KSTEP = FP8 ? 64 : 32;             // head dims of one 16-byte load by the four lanes of a key
     constexpr int KL = D / KSTEP;                    // such loads per key
@@ -250,6 +257,7 @@ attn_rows_kernel(AttnArgs a) {
     constexpr int VW = VCH * (FP8 ? 1 : 2) / 4;      // words of a piece
     constexpr int PAD = 4;
     using CacheT = typename std::conditional<FP8, uint8_t, uint16_t>::type;
+    __shared__ AttnCursor s_cursor;
     extern __shared__ float s_o[];                   // [WARPS][R][D + PAD], then [WARPS][R] maxima and sums
     float* s_m = s_o + WARPS * R * (D + PAD);
     float* s_l = s_m + WARPS * R;
@@ -259,11 +267,18 @@ attn_rows_kernel(AttnArgs a) {
     pdl_wait_prior_grids();
     const CacheT* kc = static_cast<const CacheT*>(a.k);
     const CacheT* vc = static_cast<const CacheT*>(a.v);
-    AttnCursor cur = attn_locate<R>(a, blockIdx.x, gridDim.x);
-    int4* desc = a.desc + 2 * blockIdx.x;
-    if (threadIdx.x < 2) desc[threadIdx.x].w = kAttnNone;
-    while (cur.left > 0) {
-        const int begin = cur.key_tile, end = (int)min((long long)cur.units, begin + cur.left);
+    if (warp == 0) {
+        const AttnCursor at = attn_locate<R, OV>(a, blockIdx.x, gridDim.x);
+        if (lane == 0) s_cursor = at;
+    }
+    AttnDesc* desc = a.desc + 2 * blockIdx.x;
+    if (threadIdx.x < 2) desc[threadIdx.x].state = kAttnNone;
+    __syncthreads();
+    AttnCursor cur = s_cursor;
+    for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
+        int begin, end;
+        attn_segment<OV>(a, cur, begin, end);
+        if (begin == end) continue;
         const AttnSeq span = cur.span;
         const int row0 = cur.tile * R, rows = span.n * a.group;
         // q of this lane's row r (and r + 8): the columns that meet its K columns
@@ -477,11 +492,11 @@ attn_rows_kernel(AttnArgs a) {
             }
         }
         __syncthreads();
-        const bool whole = begin == 0 && end == cur.units;
+        const bool whole = begin == 0 && end == cur.keys;
         const int slot = begin == 0 ? 1 : 0;
         float* part = attn_slot(a, blockIdx.x, slot, R, D);
         if (!whole && threadIdx.x == 0) {
-            desc[slot] = make_int4(cur.seq, cur.head, cur.tile, begin == 0 ? kAttnFirst : (end == cur.units ? kAttnLast : kAttnMiddle));
+            desc[slot] = AttnDesc{begin == 0 ? kAttnFirst : (end == cur.keys ? kAttnLast : kAttnMiddle), cur.tile, cur.head, span.q0, rows};
         }
         for (int i = threadIdx.x; i < R * (D / 4); i += kAttnThreads) {
             const int x = i / (D / 4), col = (i % (D / 4)) * 4;
@@ -515,35 +530,45 @@ attn_rows_kernel(AttnArgs a) {
             }
         }
         __syncthreads();   // s_o is reused by the next segment
-        cur.left -= end - begin;
-        if (cur.left > 0) attn_advance<R>(a, cur);
     }
 }
 
 // ---------------------------------------------------------------------------------------------
 // Joins the partials of the row tiles that several CTAs shared: a tile is begun in slot 1 of one CTA and continued in
-// slot 0 of the CTAs after it, up to the one marked last. blockIdx.x takes a run of CTAs as possible beginnings. WPR
-// warps work on a row, one after the other every WPR-th partial, and are joined in shared memory in a fixed order: a
-// whole block per row where few rows have many partials (attn_rows_kernel), a warp where many rows have few.
+// slot 0 of the CTAs after it, up to the one marked last. blockIdx.x takes a run of CTAs as possible beginnings.
+// attn_combine_kernel: few rows with many partials (attn_rows_kernel), a block per row; the 8 warps take every eighth
+// partial and are joined in shared memory in a fixed order.
+// attn_combine_rows_kernel: many rows with few partials (attn_chunk_kernel), four rows per warp.
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, int R, int WPR>
+// Partials of the row tile that CTA `first` begins; a warp looks at the 32 CTAs after it at a time.
+__device__ __forceinline__ int attn_parts(const AttnArgs& a, int first, int ctas) {
+    for (int from = first + 1;; from += 32) {
+        const int at = from + (int)(threadIdx.x & 31);
+        const unsigned ends = __ballot_sync(kFullMask, at >= ctas - 1 || a.desc[2 * at].state == kAttnLast);
+        if (ends) return from + __ffs(ends) - first;
+    }
+}
+template <typename T>
+__device__ __forceinline__ typename T::storage* attn_out_row(const AttnArgs& a, const AttnDesc& d, int row, int head_dim) {
+    const int token = (int)fast_div((uint32_t)row, a.group_div);
+    return static_cast<typename T::storage*>(a.out) +
+           ((size_t)(d.q0 + token) * a.q_heads + d.head * a.group + (row - token * a.group)) * head_dim;
+}
+
+template <typename T, int D, int R>
 __global__ void __launch_bounds__(256)
 attn_combine_kernel(AttnArgs a, int ctas) {
-    constexpr int ROWS = 8 / WPR;   // of a block
-    __shared__ float s_acc[8][D + 2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
+    constexpr int WARPS = 8;
+    __shared__ float s_acc[WARPS][D + 2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_launch_dependents();
     pdl_wait_prior_grids();
     const int from = (int)((long long)blockIdx.x * ctas / gridDim.x), to = (int)((long long)(blockIdx.x + 1) * ctas / gridDim.x);
     for (int first = from; first < to; ++first) {
-        const int4 d = a.desc[2 * first + 1];
-        if (d.w != kAttnFirst) continue;
-        const AttnSeq span = attn_seq(a, d.x);
-        const int x = blockIdx.y * ROWS + warp / WPR;
-        if (d.z * R + (int)blockIdx.y * ROWS >= span.n * a.group) continue;   // (the same for the whole block)
-        int last = first + 1;
-        while (last < ctas - 1 && a.desc[2 * last].w != kAttnLast) ++last;
-        const int parts = last - first + 1;
+        const AttnDesc d = a.desc[2 * first + 1];
+        const int x = blockIdx.y, row = d.tile * R + x;
+        if (d.state != kAttnFirst || row >= d.rows) continue;
+        const int parts = attn_parts(a, first, ctas);
         auto part_of = [&](int i) { return attn_slot(a, first + i, i == 0 ? 1 : 0, R, D); };
         float top = -INFINITY;
         for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_of(i)[x]);
@@ -555,7 +580,7 @@ attn_combine_kernel(AttnArgs a, int ctas) {
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) acc[e] = 0.0f;
 #pragma unroll 4
-        for (int i = sub; i < parts; i += WPR) {
+        for (int i = warp; i < parts; i += WARPS) {
             const float* p = part_of(i);
             const float f = fast_exp2(p[x] - ref);
             sum = fmaf(f, p[R + x], sum);
@@ -566,25 +591,66 @@ attn_combine_kernel(AttnArgs a, int ctas) {
         for (int e = 0; e < D / 32; ++e) s_acc[warp][lane + 32 * e] = acc[e];
         if (lane == 0) s_acc[warp][D] = sum;
         __syncthreads();
-        for (int i = threadIdx.x; i < ROWS * (D / 4); i += 256) {
-            const int r = i / (D / 4), col = (i % (D / 4)) * 4;
-            const int mine = d.z * R + blockIdx.y * ROWS + r;
-            if (mine >= span.n * a.group) break;
+        if (threadIdx.x < D / 4) {
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             float total = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WPR; ++w) {
-                const float* p = s_acc[r * WPR + w];
-                v.x += p[col], v.y += p[col + 1], v.z += p[col + 2], v.w += p[col + 3];
-                total += p[D];
+            for (int w = 0; w < WARPS; ++w) {
+                const float* p = s_acc[w] + 4 * threadIdx.x;
+                v.x += p[0], v.y += p[1], v.z += p[2], v.w += p[3];
+                total += s_acc[w][D];
             }
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            const int token = (int)fast_div((uint32_t)mine, a.group_div);
-            typename T::storage* dst = static_cast<typename T::storage*>(a.out) +
-                ((size_t)(span.q0 + token) * a.q_heads + d.y * a.group + (mine - token * a.group)) * D + col;
-            store_quad<T>(dst, 0, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+            store_quad<T>(attn_out_row<T>(a, d, row, D), threadIdx.x, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         }
         __syncthreads();
+    }
+}
+
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(256)
+attn_combine_rows_kernel(AttnArgs a, int ctas) {
+    constexpr int Q = D / 32;   // column quads of a lane: lane / 4, lane / 4 + 8, ... of row lane % 4 of the warp's four
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_launch_dependents();
+    pdl_wait_prior_grids();
+    const int from = (int)((long long)blockIdx.x * ctas / gridDim.x), to = (int)((long long)(blockIdx.x + 1) * ctas / gridDim.x);
+    for (int first = from; first < to; ++first) {
+        const AttnDesc d = a.desc[2 * first + 1];
+        const int x0 = (blockIdx.y * 8 + warp) * 4, x = x0 + (lane & 3);
+        if (d.state != kAttnFirst || d.tile * R + x0 >= d.rows) continue;
+        const int parts = attn_parts(a, first, ctas);
+        // one pass with a running maximum: the statistics and outputs of a partial are requested together
+        float top = -INFINITY, sum = 0.0f;
+        float4 acc[Q];
+#pragma unroll
+        for (int e = 0; e < Q; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (int i = 0; i < parts; ++i) {
+            const float* p = attn_slot(a, first + i, i == 0 ? 1 : 0, R, D);
+            const float4* src = reinterpret_cast<const float4*>(p + 2 * R) + (lane >> 2) * R + x;
+            float4 o[Q];
+            const float m = p[x], l = p[R + x];
+#pragma unroll
+            for (int e = 0; e < Q; ++e) o[e] = src[8 * e * R];
+            const float now = fmaxf(top, m), ref = now == -INFINITY ? 0.0f : now;
+            const float f = fast_exp2(m - ref), g = fast_exp2(top - ref);
+            top = now;
+            sum = fmaf(f, l, sum * g);
+#pragma unroll
+            for (int e = 0; e < Q; ++e) {
+                acc[e].x = fmaf(f, o[e].x, acc[e].x * g), acc[e].y = fmaf(f, o[e].y, acc[e].y * g);
+                acc[e].z = fmaf(f, o[e].z, acc[e].z * g), acc[e].w = fmaf(f, o[e].w, acc[e].w * g);
+            }
+        }
+        if (d.tile * R + x < d.rows) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            typename T::storage* dst = attn_out_row<T>(a, d, d.tile * R + x, D);
+#pragma unroll
+            for (int e = 0; e < Q; ++e) {
+                store_quad<T>(dst, (lane >> 2) + 8 * e, make_float4(acc[e].x * inv, acc[e].y * inv, acc[e].z * inv, acc[e].w * inv));
+            }
+        }
     }
 }
 

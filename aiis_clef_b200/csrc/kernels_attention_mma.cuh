@@ -15,6 +15,10 @@
 // CTA owns come out as NaN.
 #pragma once
 
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
 #include "kernels_attention.cuh"
 
 namespace clef {
@@ -70,6 +74,16 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
 }
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Four E4M3 codes times their row's scale, rounded to bf16 (what a bf16 cache would hold: half a step of 2^-8 per value,
+// next to the codes' own 2^-4; it frees the softmax of two products per key).
+__device__ __forceinline__ void e4m3x4_scaled(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
+    uint32_t a, b;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    lo = pack_bf16x2(x.x * scale, x.y * scale);
+    hi = pack_bf16x2(y.x * scale, y.y * scale);
+}
+
 // D[128 x N] (tensor memory) (+)= A B^T; A from shared memory or from tensor memory.
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
@@ -111,9 +125,15 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Shared-memory operand descriptor, 128-byte swizzle: address, leading and stride byte offsets.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// Shared-memory operand descriptor, 128-byte swizzle. Low word: address / 16 and leading byte offset / 16 in the upper half;
+// high word: stride byte offset / 16 (1,024: eight rows of 128 bytes), version, swizzle mode.
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t leading) {
+    uint32_t low = (addr >> 4) | ((leading >> 4) << 16);
+    asm volatile("" : "+r"(low));   // keeps the descriptors of an unrolled loop from being computed, and kept, all at once
+    return low;
+}
+__device__ __forceinline__ uint64_t smem_desc(uint32_t low, uint32_t bytes_on) {
+    return ((uint64_t)((1024 >> 4) | (1u << 14) | (2u << 29)) << 32) | (low + (bytes_on >> 4));
 }
 // Instruction descriptor: f32 accumulators, bf16 operands, A K-major; B K-major or MN-major.
 __host__ __device__ constexpr uint32_t mma_idesc(int n, bool b_mn_major) {
@@ -126,6 +146,50 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int chunk, int rows) {
     return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
+// Eight q values as they are loaded, and as bf16.
+template <typename T>
+struct RawQ {
+    uint4 w[T::kBytes / 2];
+    __device__ __forceinline__ void load(const typename T::storage* p) {
+#pragma unroll
+        for (int i = 0; i < T::kBytes / 2; ++i) w[i] = ldg_stream_v4(reinterpret_cast<const uint8_t*>(p) + 16 * i);
+    }
+    __device__ __forceinline__ uint4 bf16() const {
+        if (T::kBytes == 2) return w[0];
+        const uint4 b = w[T::kBytes / 2 - 1];
+        return make_uint4(pack_bf16x2(__uint_as_float(w[0].x), __uint_as_float(w[0].y)), pack_bf16x2(__uint_as_float(w[0].z), __uint_as_float(w[0].w)),
+                          pack_bf16x2(__uint_as_float(b.x), __uint_as_float(b.y)), pack_bf16x2(__uint_as_float(b.z), __uint_as_float(b.w)));
+    }
+};
+
+template <int REGS, bool UP>
+__device__ __forceinline__ void set_registers() {
+    if (UP) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x of a pair on the FMA pipe, for -126 <= x < 127 after clamping from below: x = n + f with n the nearest integer
+// (adding 1.5 * 2^23 leaves n in the low mantissa bits), 2^f by a polynomial of degree 4 that is minimax in relative error
+// on [-1/2, 1/2] (2.7e-6), n added to the exponent. The multi-function unit does 16 exponentials a clock and SM, which
+// would bound the softmax; three pairs in eight are computed here instead.
+__device__ __forceinline__ f32x2 exp2_poly(f32x2 x) {
+    x = f2_pack(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+    const f32x2 t = f2_add(x, f2_splat(12582912.0f));
+    const f32x2 f = f2_fma(f2_add(t, f2_splat(-12582912.0f)), f2_splat(-1.0f), x);
+    f32x2 p = f2_fma(f2_splat(0.009570105001330376f), f, f2_splat(0.05591785907745361f));
+    p = f2_fma(p, f, f2_splat(0.240247443318367f));
+    p = f2_fma(p, f, f2_splat(0.6931217908859253f));
+    p = f2_fma(p, f, f2_splat(0.9999992847442627f));
+    return f2_pack(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                   __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
 template <int D>
 struct ChunkShape {
     static constexpr int TILES = D == 256 ? 1 : 2;        // row blocks of 128
@@ -133,30 +197,41 @@ struct ChunkShape {
     static constexpr int N = D == 256 ? 64 : 128;         // keys of a step
     static constexpr int SBUF = D == 256 ? 2 : 1;         // S buffers per row block
     static constexpr int RING = 4;                        // K, V, K, V
-    static constexpr int THREADS = 128 * TILES + 128 + 32;
+    static constexpr int OV = 2;                          // a row tile's beginning and end cost about two units
+    static constexpr int THREADS = 128 * TILES + 256;     // softmax, producers, products (one thread of a warpgroup)
+    // Registers: 512 threads start with 128 each; the softmax keeps a row of S in registers.
+    static constexpr bool SPLIT = TILES == 2;
+    static constexpr int SOFTMAX_REGS = 184, PRODUCER_REGS = 80, MMA_REGS = 64;
+    static_assert(!SPLIT || 2 * SOFTMAX_REGS + PRODUCER_REGS + MMA_REGS <= 512, "more than the block was launched with");
     static constexpr int Q_BYTES = 128 * D * 2;
     static constexpr int KV_BYTES = N * D * 2;
     static constexpr int S_COL = 0;                       // tensor memory columns: S buffers, then O
     static constexpr int O_COL = TILES * SBUF * N;
     static constexpr int BAR_COUNT = 2 * RING + 10;
-    static constexpr int SMEM = 1024 + TILES * Q_BYTES + RING * KV_BYTES + 2 * TILES * 2 * N * 4 + 256;
+    static constexpr int SMEM = 1024 + TILES * Q_BYTES + RING * KV_BYTES;
 };
 
 // Steps of a segment [begin, end) of key tiles, the same for every role: whole tiles of N keys, none that lies past the
 // last key a row of the tile sees, one at least.
 template <int D>
-__device__ __forceinline__ void chunk_steps(const AttnArgs& a, const AttnCursor& c, int end, int& keys, int& from, int& to) {
+__device__ __forceinline__ void chunk_steps(const AttnArgs& a, const AttnCursor& c, int begin, int end, int& keys, int& from, int& to) {
     constexpr int PER = kAttnKeys / ChunkShape<D>::N;
     keys = attn_visible(a, c.span, min((c.tile + 1) * ChunkShape<D>::R, c.span.n * a.group));
-    from = c.key_tile * PER;
+    from = begin * PER;
     to = max(from + 1, min(end * PER, (keys + ChunkShape<D>::N - 1) / ChunkShape<D>::N));
+}
+
+// The 128 threads of row block t.
+__device__ __forceinline__ void block_barrier(int t) {
+    if (t == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+    else asm volatile("bar.sync 2, 128;" ::: "memory");
 }
 
 template <typename T, bool FP8, int D>
 __global__ void __launch_bounds__(ChunkShape<D>::THREADS, 1)
 attn_chunk_kernel(AttnArgs a) {
     using Sh = ChunkShape<D>;
-    constexpr int TILES = Sh::TILES, R = Sh::R, N = Sh::N, SBUF = Sh::SBUF, RING = Sh::RING;
+    constexpr int TILES = Sh::TILES, R = Sh::R, N = Sh::N, SBUF = Sh::SBUF, RING = Sh::RING, OV = Sh::OV;
     extern __shared__ uint8_t s_raw[];
     __shared__ uint64_t full[RING], empty[RING], q_ready[TILES], s_ready[TILES * SBUF], p_ready[TILES * SBUF], pv_done[TILES], drained;
     __shared__ uint32_t s_tmem;
@@ -165,7 +240,6 @@ attn_chunk_kernel(AttnArgs a) {
     uint8_t* s_base = s_raw + ((1024 - (smem_addr(s_raw) & 1023)) & 1023);
     uint8_t* s_q = s_base;
     uint8_t* s_kv = s_q + TILES * Sh::Q_BYTES;
-    float* s_scale = reinterpret_cast<float*>(s_kv + RING * Sh::KV_BYTES);   // FP8: [TILES][2][k, v][N]
     volatile int* gave_up = &s_gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4;
@@ -184,19 +258,20 @@ attn_chunk_kernel(AttnArgs a) {
     pdl_launch_dependents();
     pdl_wait_prior_grids();
     if (warp == 0) {
-        const AttnCursor c = attn_locate<R>(a, blockIdx.x, gridDim.x);
+        const AttnCursor c = attn_locate<R, OV>(a, blockIdx.x, gridDim.x);
         if (lane == 0) s_cursor = c;
     }
-    int4* desc = a.desc + 2 * blockIdx.x;
-    if (threadIdx.x < 2) desc[threadIdx.x].w = kAttnNone;
+    AttnDesc* desc = a.desc + 2 * blockIdx.x;
+    if (threadIdx.x < 2) desc[threadIdx.x].state = kAttnNone;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    AttnCursor cur = s_cursor;
 
     if (warp < kProducerWarp) {
         // ---- softmax: thread = row -------------------------------------------------------------------------------
+        if (Sh::SPLIT) set_registers<Sh::SOFTMAX_REGS, true>();
+        AttnCursor cur = s_cursor;
         const int t = warp >> 2;                                    // row block
         const int x = threadIdx.x & 127;                            // row of the block = tensor memory lane
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;          // (32 (warp % 4)) << 16
@@ -204,205 +279,214 @@ attn_chunk_kernel(AttnArgs a) {
         uint8_t* q_tile = s_q + t * Sh::Q_BYTES;
         const float scale = fabsf(a.scale_log2);
         const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale negates q instead
-        float* scales = s_scale + t * 4 * N;
         int steps_done = 0;                                         // of this row block, over all segments
-        while (cur.left > 0) {
-            const int begin = cur.key_tile, end = (int)min((long long)cur.units, begin + cur.left);
+        for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
+            int begin, end;
+            attn_segment<OV>(a, cur, begin, end);
             const AttnSeq span = cur.span;
             const int rows = span.n * a.group, row0 = cur.tile * R + t * 128;
+            if (begin == end || row0 >= rows) continue;
             int keys, from, to;
-            chunk_steps<D>(a, cur, end, keys, from, to);
-            if (row0 < rows) {
-                // q: 16-byte chunks, eight lanes to a 128-byte line, rounded to bf16, into the swizzled tile
-                for (int i = x; i < 128 * (D / 8); i += 128) {
-                    const int r = i / (D / 8), ch = i % (D / 8), y = row0 + r;
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (y < rows) {
-                        const int token = (int)fast_div((uint32_t)y, a.group_div);
-                        const size_t at = ((size_t)(span.q0 + token) * a.q_heads + cur.head * a.group + (y - token * a.group)) * D + ch * 8;
-                        float f[8];
-                        const float4 f0 = load_quad<T>(static_cast<const typename T::storage*>(a.q) + at, 0);
-                        const float4 f1 = load_quad<T>(static_cast<const typename T::storage*>(a.q) + at, 1);
-                        f[0] = f0.x, f[1] = f0.y, f[2] = f0.z, f[3] = f0.w, f[4] = f1.x, f[5] = f1.y, f[6] = f1.z, f[7] = f1.w;
-                        w = make_uint4(pack_bf16x2(f[0], f[1]) ^ flip, pack_bf16x2(f[2], f[3]) ^ flip, pack_bf16x2(f[4], f[5]) ^ flip,
-                                       pack_bf16x2(f[6], f[7]) ^ flip);
-                    }
-                    *reinterpret_cast<uint4*>(q_tile + tile_offset(r, ch, 128)) = w;
-                }
-                async_proxy_fence();
-                mbar_arrive(&q_ready[t]);
-                const int lim = row0 + x < rows ? attn_visible(a, span, row0 + x + 1) : 0;
-                float m = -INFINITY, l = 0.0f;
-                // FP8: thread x fetches the scales of key x of a step, one step ahead
-                float ks = 0.0f, vs = 0.0f;
-                auto fetch_scales = [&](int step) {
-                    const int key = step * N + x;
-                    const int row = x < N && step < to && key < keys ? attn_cache_row(a, cur.seq, key) : -1;
-                    const size_t at = (size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head;
-                    ks = row < 0 ? 0.0f : a.k_scales[at];
-                    vs = row < 0 ? 0.0f : a.v_scales[at];
-                };
-                if (FP8) fetch_scales(from);
-                for (int step = from; step < to; ++step, ++steps_done) {
-                    const int buf = SBUF == 1 ? 0 : (steps_done & 1);
-                    const uint32_t s_addr = tmem + lanes + Sh::S_COL + (t * SBUF + buf) * N;
-                    const uint32_t s_parity = (SBUF == 1 ? steps_done : steps_done >> 1) & 1;
-                    float* sc = scales + (steps_done & 1) * 2 * N;
-                    if (FP8) {
-                        if (x < N) sc[x] = ks * scale, sc[N + x] = vs;
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
-                        fetch_scales(step + 1);
-                    }
-                    mbar_wait_warp(&s_ready[t * SBUF + buf], s_parity, gave_up);
-                    tc_fence_after();
-                    const int base = step * N;
-                    const bool edge = __any_sync(kFullMask, base + N > lim);   // some keys of the step are hidden from some row
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < N; c += 32) {
-                        float s[32];
-                        tc_ld32(s_addr + c, s);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            if (FP8) {
-                                const float4 k4 = *reinterpret_cast<const float4*>(sc + c + i);
-                                s[i] *= k4.x, s[i + 1] *= k4.y, s[i + 2] *= k4.z, s[i + 3] *= k4.w;
-                            }
-                        }
-                        if (edge) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) s[i] = base + c + i < lim ? s[i] : -INFINITY;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
-                    }
-                    if (!FP8) top = top == -INFINITY ? top : top * scale;
-                    const bool grown = top > m + 8.0f;   // (m = -inf: any key at all)
-                    if (__any_sync(kFullMask, grown)) {
-                        const float now = grown ? top : m;
-                        const float fix = now == m ? 1.0f : fast_exp2(m - now);
-                        l *= fix;
-                        m = now;
-                        if (step > from) {
-                            if (SBUF == 2) {   // S of this step was ready before the last product with P had ended
-                                mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
-                                tc_fence_after();
-                            }   // (with one S buffer its product came after that one)
+            chunk_steps<D>(a, cur, begin, end, keys, from, to);
+            // q: 16-byte chunks, eight lanes to a 128-byte line, rounded to bf16, into the swizzled tile; eight requests in
+            // flight (rows past the last repeat it, and are stored as zeros)
 #pragma unroll 1
-                            for (int c = 0; c < D; c += 32) {
-                                float o[32];
-                                tc_ld32(o_addr + c, o);
-                                tc_wait_ld();
+            for (int i0 = 0; i0 < D / 8; i0 += 8) {
+                RawQ<T> raw[8];
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] *= fix;
-                                tc_st32(o_addr + c, o);
-                            }
-                        }
-                    }
-                    const float ref = m == -INFINITY ? 0.0f : -m;
-#pragma unroll
-                    for (int c = 0; c < N; c += 32) {
-                        float s[32];
-                        tc_ld32(s_addr + c, s);
-                        tc_wait_ld();
-                        uint32_t p[16];
-                        float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            float4 k4 = make_float4(scale, scale, scale, scale), v4 = make_float4(1.f, 1.f, 1.f, 1.f);
-                            if (FP8) {
-                                k4 = *reinterpret_cast<const float4*>(sc + c + i);
-                                v4 = *reinterpret_cast<const float4*>(sc + N + c + i);
-                            }
-                            float e0 = fmaf(s[i], k4.x, ref), e1 = fmaf(s[i + 1], k4.y, ref);
-                            float e2 = fmaf(s[i + 2], k4.z, ref), e3 = fmaf(s[i + 3], k4.w, ref);
-                            if (edge) {
-                                e0 = base + c + i < lim ? e0 : -INFINITY, e1 = base + c + i + 1 < lim ? e1 : -INFINITY;
-                                e2 = base + c + i + 2 < lim ? e2 : -INFINITY, e3 = base + c + i + 3 < lim ? e3 : -INFINITY;
-                            }
-                            e0 = fast_exp2(e0), e1 = fast_exp2(e1), e2 = fast_exp2(e2), e3 = fast_exp2(e3);
-                            sum0 += e0 + e1;
-                            sum1 += e2 + e3;
-                            if (FP8) {
-                                e0 *= v4.x, e1 *= v4.y, e2 *= v4.z, e3 *= v4.w;
-                                if (edge) {   // whatever scale a hidden key has, its weight is 0
-                                    e0 = base + c + i < lim ? e0 : 0.0f, e1 = base + c + i + 1 < lim ? e1 : 0.0f;
-                                    e2 = base + c + i + 2 < lim ? e2 : 0.0f, e3 = base + c + i + 3 < lim ? e3 : 0.0f;
-                                }
-                            }
-                            p[i / 2] = pack_bf16x2(e0, e1);
-                            p[i / 2 + 1] = pack_bf16x2(e2, e3);
-                        }
-                        l += sum0 + sum1;
-                        tc_st16(s_addr + c / 2, p);   // over columns of S that are read already
-                    }
-                    tc_wait_st();
-                    tc_fence_before();
-                    // pv_done is waited for once a step, so that its phase is never more than one ahead of the wait
-                    if (SBUF == 2 && steps_done > 0) mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
-                    mbar_arrive(&p_ready[t * SBUF + buf]);
+                for (int j = 0; j < 8; ++j) {
+                    const int i = (i0 + j) * 128 + x, y = min(row0 + i / (D / 8), rows - 1);
+                    const int token = (int)fast_div((uint32_t)y, a.group_div);
+                    raw[j].load(static_cast<const typename T::storage*>(a.q) +
+                                ((size_t)(span.q0 + token) * a.q_heads + cur.head * a.group + (y - token * a.group)) * D + i % (D / 8) * 8);
                 }
-                mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = (i0 + j) * 128 + x, r = i / (D / 8);
+                    uint4 w = raw[j].bf16();
+                    w = row0 + r < rows ? make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip) : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(q_tile + tile_offset(r, i % (D / 8), 128)) = w;
+                }
+            }
+            async_proxy_fence();
+            mbar_arrive(&q_ready[t]);
+            const int lim = row0 + x < rows ? attn_visible(a, span, row0 + x + 1) : 0;
+            float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
+            for (int step = from; step < to; ++step, ++steps_done) {
+                const int buf = SBUF == 1 ? 0 : (steps_done & 1);
+                const uint32_t s_addr = tmem + lanes + Sh::S_COL + (t * SBUF + buf) * N;
+                const uint32_t s_parity = (SBUF == 1 ? steps_done : steps_done >> 1) & 1;
+                mbar_wait_warp(&s_ready[t * SBUF + buf], s_parity, gave_up);
                 tc_fence_after();
-                const bool whole = begin == 0 && end == cur.units;
-                const bool live = row0 + x < rows;
-                const int slot = begin == 0 ? 1 : 0;
-                float* part = attn_slot(a, blockIdx.x, slot, R, D);
-                if (!whole) {
-                    if (threadIdx.x == 0) {
-                        desc[slot] = make_int4(cur.seq, cur.head, cur.tile, begin == 0 ? kAttnFirst : (end == cur.units ? kAttnLast : kAttnMiddle));
+                f32x2 s[N / 2];
+#pragma unroll
+                for (int c = 0; c < N; c += 32) tc_ld32(s_addr + c, reinterpret_cast<float*>(s + c / 2));
+                tc_wait_ld();
+                const int base = step * N;
+                const bool edge = __any_sync(kFullMask, base + N > lim);   // some keys of the step are hidden from some row
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < N / 2; ++i) {
+                        s[i].x = base + 2 * i < lim ? s[i].x : -INFINITY;
+                        s[i].y = base + 2 * i + 1 < lim ? s[i].y : -INFINITY;
                     }
-                    part[t * 128 + x] = m;
-                    part[R + t * 128 + x] = *gave_up ? __int_as_float(0x7fc00000) : l;
                 }
-                float f = 1.0f;
-                if (whole) f = l == 0.0f ? 0.0f : 1.0f / l;
-                if (*gave_up) f = __int_as_float(0x7fc00000);
-                const int token = (int)fast_div((uint32_t)(row0 + x), a.group_div);
-                typename T::storage* dst = static_cast<typename T::storage*>(a.out) +
-                    ((size_t)(span.q0 + token) * a.q_heads + cur.head * a.group + (row0 + x - token * a.group)) * D;
-                float* pdst = part + 2 * R + (size_t)(t * 128 + x) * D;
+                float top0 = s[0].x, top1 = s[0].y;
+#pragma unroll
+                for (int i = 1; i < N / 2 - 1; i += 2) {
+                    top0 = max3(top0, s[i].x, s[i].y);
+                    top1 = max3(top1, s[i + 1].x, s[i + 1].y);
+                }
+                float top = fmaxf(max3(top0, top1, s[N / 2 - 1].x), s[N / 2 - 1].y);
+                top = top == -INFINITY ? top : top * scale;
+                const bool grown = top > m + 8.0f;   // (m = -inf: any key at all)
+                if (__any_sync(kFullMask, grown)) {
+                    const float now = grown ? top : m;
+                    const float fix = now == m ? 1.0f : fast_exp2(m - now);
+                    l *= fix;
+                    m = now;
+                    if (step > from) {
+                        if (SBUF == 2) {   // S of this step was ready before the last product with P had ended
+                            mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
+                            tc_fence_after();
+                        }   // (with one S buffer its product came after that one)
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            float o[32];
+                            tc_ld32(o_addr + c, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] *= fix;
+                            tc_st32(o_addr + c, o);
+                        }
+                    }
+                }
+                const f32x2 ref = f2_splat(m == -INFINITY ? 0.0f : -m);
+                const f32x2 by = f2_splat(scale);
+                f32x2 sum0 = f2_splat(0.0f), sum1 = f2_splat(0.0f);
+                auto weights = [&](auto with_edge) {   // (compiled twice: a test per pair would cost more than the pair)
+                    constexpr bool EDGE = decltype(with_edge)::value;
+#pragma unroll
+                    for (int c = 0; c < N / 2; c += 16) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            f32x2 e = f2_fma(s[c + i], by, ref);
+                            if (EDGE) {   // hidden keys: a weight of exactly 0 (and scale 0 would make NaN of their -inf)
+                                e.x = base + 2 * (c + i) < lim ? fast_exp2(e.x) : 0.0f;
+                                e.y = base + 2 * (c + i) + 1 < lim ? fast_exp2(e.y) : 0.0f;
+                            } else if (i % 8 == 2 || i % 8 == 5 || i % 8 == 7) {
+                                e = exp2_poly(e);
+                            } else {
+                                e = f2_pack(fast_exp2(e.x), fast_exp2(e.y));
+                            }
+                            if (i % 2 == 0) sum0 = f2_add(sum0, e);
+                            else sum1 = f2_add(sum1, e);
+                            p[i] = pack_bf16x2(e.x, e.y);
+                        }
+                        tc_st16(s_addr + c, p);   // over columns of S that are in registers
+                    }
+                };
+                if (edge) weights(std::true_type{});
+                else weights(std::false_type{});
+                sum0 = f2_add(sum0, sum1);
+                l += sum0.x + sum0.y;
+                tc_wait_st();
+                tc_fence_before();
+                // pv_done is waited for once a step, so that its phase is never more than one ahead of the wait
+                if (SBUF == 2 && steps_done > 0) mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
+                mbar_arrive(&p_ready[t * SBUF + buf]);
+            }
+            mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
+            tc_fence_after();
+            const bool whole = begin == 0 && end == cur.keys;
+            const int slot = begin == 0 ? 1 : 0;
+            float* part = attn_slot(a, blockIdx.x, slot, R, D);
+            if (!whole) {
+                if (threadIdx.x == 0) {
+                    desc[slot] = AttnDesc{begin == 0 ? kAttnFirst : (end == cur.keys ? kAttnLast : kAttnMiddle), cur.tile, cur.head, span.q0, rows};
+                }
+                part[t * 128 + x] = m;
+                part[R + t * 128 + x] = *gave_up ? __int_as_float(0x7fc00000) : l;
+            }
+            float f = 1.0f;
+            if (whole) f = l == 0.0f ? 0.0f : 1.0f / l;
+            if (*gave_up) f = __int_as_float(0x7fc00000);
+            if (!whole) {
+                // partials: [D / 4][R][4], so that the 32 rows of a warp are 512 consecutive bytes
+                float4* dst = reinterpret_cast<float4*>(part + 2 * R) + t * 128 + x;
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     float o[32];
                     tc_ld32(o_addr + c, o);
                     tc_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = f == 0.0f ? 0.0f : o[i] * f;
+                    for (int i = 0; i < 32; i += 4) dst[(c + i) / 4 * R] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            } else {
+                // rows of `whole` columns at a time through the q tile (its products are done), then out in whole lines
+                constexpr int COLS = T::kBytes == 2 ? D : D / 2;     // as many as the q tile holds
+                constexpr int PIECES = COLS * T::kBytes / 16;        // 16-byte pieces of a row
+#pragma unroll 1
+                for (int c0 = 0; c0 < D; c0 += COLS) {
+#pragma unroll 1
+                    for (int c = 0; c < COLS; c += 32) {
+                        float o[32];
+                        tc_ld32(o_addr + c0 + c, o);
+                        tc_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        if (!live) break;
-                        if (whole && T::kBytes == 2) {
-                            stg_v4(dst + c + i, make_uint4(pack_bf16x2(o[i], o[i + 1]), pack_bf16x2(o[i + 2], o[i + 3]),
-                                                           pack_bf16x2(o[i + 4], o[i + 5]), pack_bf16x2(o[i + 6], o[i + 7])));
-                        } else {
-                            float* to_f32 = whole ? reinterpret_cast<float*>(dst) : pdst;
-                            *reinterpret_cast<float4*>(to_f32 + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                            *reinterpret_cast<float4*>(to_f32 + c + i + 4) = make_float4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
+                        for (int i = 0; i < 32; ++i) o[i] = f == 0.0f ? 0.0f : o[i] * f;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 16 / T::kBytes) {
+                            const uint4 w = T::kBytes == 2
+                                ? make_uint4(pack_bf16x2(o[i], o[i + 1]), pack_bf16x2(o[i + 2], o[i + 3]), pack_bf16x2(o[i + 4 & 31], o[i + 5 & 31]),
+                                             pack_bf16x2(o[i + 6 & 31], o[i + 7 & 31]))
+                                : make_uint4(__float_as_uint(o[i]), __float_as_uint(o[i + 1]), __float_as_uint(o[i + 2]), __float_as_uint(o[i + 3]));
+                            *reinterpret_cast<uint4*>(q_tile + tile_offset(x, (c + i) * T::kBytes / 16, 128)) = w;
                         }
                     }
-                    __syncwarp();
+                    block_barrier(t);
+#pragma unroll 4
+                    for (int i = x; i < 128 * PIECES; i += 128) {
+                        const int r = i / PIECES, y = row0 + r;
+                        if (y < rows) {
+                            const int token = (int)fast_div((uint32_t)y, a.group_div);
+                            typename T::storage* dst = static_cast<typename T::storage*>(a.out) +
+                                ((size_t)(span.q0 + token) * a.q_heads + cur.head * a.group + (y - token * a.group)) * D + c0;
+                            stg_v4(reinterpret_cast<uint8_t*>(dst) + i % PIECES * 16,
+                                   *reinterpret_cast<const uint4*>(q_tile + tile_offset(r, i % PIECES, 128)));
+                        }
+                    }
+                    block_barrier(t);   // the tile is written again, with the next columns or the next q
                 }
-                tc_fence_before();
             }
-            cur.left -= end - begin;
-            if (cur.left > 0) attn_advance<R>(a, cur);
+            tc_fence_before();
         }
     } else if (warp < kMmaWarp) {
         // ---- producers: a warp gathers N / 4 rows of each tile, lane l of it knows row l's place ----------------
         constexpr int ROWS = N / 4;                       // rows per warp
+        if (Sh::SPLIT) set_registers<Sh::PRODUCER_REGS, false>();
+        AttnCursor cur = s_cursor;
         const int w = warp - kProducerWarp;
         using CacheT = typename std::conditional<FP8, uint8_t, uint16_t>::type;
         constexpr int CPR = D * (FP8 ? 1 : 2) / 16;       // 16-byte pieces of a cache row
         constexpr int RPI = 32 / (CPR < 8 ? CPR : 8);     // rows a warp touches at once
         constexpr int LPR = 32 / RPI;                     // lanes per row
-        uint32_t item = 0;
-        while (cur.left > 0) {
-            const int end = (int)min((long long)cur.units, cur.key_tile + cur.left);
-            const int taken = end - cur.key_tile;
-            int keys, from, to;
-            chunk_steps<D>(a, cur, end, keys, from, to);
+        uint32_t item = 0;      // K and V tiles asked for so far
+        uint32_t issued = 0, in_flight = 0;   // (cp.async) asked for, and the last of them that are not handed over
+        auto hand_over = [&](uint32_t but) {   // all but the last `but` (0 or 2) of those in flight
+            if (in_flight <= but) return;
+            if (but == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+            else asm volatile("cp.async.wait_group 2;" ::: "memory");
+            async_proxy_fence();
+            for (; in_flight > but; --in_flight) mbar_arrive(&full[(issued - in_flight) % RING]);
+        };
+        for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
+            int begin, end, keys, from, to;
+            attn_segment<OV>(a, cur, begin, end);
+            if (begin == end) continue;
+            chunk_steps<D>(a, cur, begin, end, keys, from, to);
             auto lookup = [&](int step) {
                 const int key = step * N + w * ROWS + (lane % ROWS);
                 return step < to && key < keys ? attn_cache_row(a, cur.seq, key) : -1;
@@ -412,11 +496,17 @@ attn_chunk_kernel(AttnArgs a) {
                 const int ahead = lookup(step + 1);
 #pragma unroll
                 for (int which = 0; which < 2; ++which, ++item) {
-                    const uint32_t slot = item % RING;
+                    const uint32_t slot = item % RING, parity = ((item / RING) & 1) ^ 1;
                     uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
                     const CacheT* src = static_cast<const CacheT*>(which == 0 ? a.k : a.v);
                     if (!FP8) {
-                        mbar_wait(&empty[slot], ((item / RING) & 1) ^ 1, gave_up);
+                        // While its buffer is still being read, the warp lets the rows it has asked for arrive, and hands
+                        // them over; otherwise two items stay in flight.
+                        if (!mbar_try(&empty[slot], parity)) {
+                            hand_over(0);
+                            mbar_wait(&empty[slot], parity, gave_up);
+                        }
+                        __syncwarp();
 #pragma unroll
                         for (int i = 0; i < ROWS / RPI; ++i) {
                             const int r = i * RPI + lane / LPR;
@@ -430,12 +520,11 @@ attn_chunk_kernel(AttnArgs a) {
                             }
                         }
                         asm volatile("cp.async.commit_group;" ::: "memory");
-                        if (item >= 2) {   // two items stay in flight; the one before them is complete: hand it over
-                            asm volatile("cp.async.wait_group 2;" ::: "memory");
-                            async_proxy_fence();
-                            mbar_arrive(&full[(item - 2) % RING]);
-                        }
+                        ++issued, ++in_flight;
+                        if (in_flight > 2) hand_over(2);
                     } else {
+                        const float* by = which == 0 ? a.k_scales : a.v_scales;
+                        const float scale32 = row32 < 0 ? 0.0f : by[(size_t)row32 * a.kv_heads + cur.head];
                         uint4 code[ROWS / RPI][CPR / LPR];
 #pragma unroll
                         for (int i = 0; i < ROWS / RPI; ++i) {
@@ -446,20 +535,21 @@ attn_chunk_kernel(AttnArgs a) {
                                 code[i][j] = row < 0 ? make_uint4(0, 0, 0, 0) : ldg_stream_v4(p + 16 * (lane % LPR + j * LPR));
                             }
                         }
-                        mbar_wait(&empty[slot], ((item / RING) & 1) ^ 1, gave_up);
+                        mbar_wait_warp(&empty[slot], parity, gave_up);
 #pragma unroll
                         for (int i = 0; i < ROWS / RPI; ++i) {
-                            const int r = w * ROWS + i * RPI + lane / LPR;
+                            const int r = i * RPI + lane / LPR;
+                            const float scale = __shfl_sync(kFullMask, scale32, i * RPI + lane / LPR);
 #pragma unroll
                             for (int j = 0; j < CPR / LPR; ++j) {
                                 const int ch = 2 * (lane % LPR + j * LPR);
                                 uint4 lo, hi;
-                                e4m3x4_to_bf16(code[i][j].x, lo.x, lo.y);
-                                e4m3x4_to_bf16(code[i][j].y, lo.z, lo.w);
-                                e4m3x4_to_bf16(code[i][j].z, hi.x, hi.y);
-                                e4m3x4_to_bf16(code[i][j].w, hi.z, hi.w);
-                                *reinterpret_cast<uint4*>(tile + tile_offset(r, ch, N)) = lo;
-                                *reinterpret_cast<uint4*>(tile + tile_offset(r, ch + 1, N)) = hi;
+                                e4m3x4_scaled(code[i][j].x, scale, lo.x, lo.y);
+                                e4m3x4_scaled(code[i][j].y, scale, lo.z, lo.w);
+                                e4m3x4_scaled(code[i][j].z, scale, hi.x, hi.y);
+                                e4m3x4_scaled(code[i][j].w, scale, hi.z, hi.w);
+                                *reinterpret_cast<uint4*>(tile + tile_offset(w * ROWS + r, ch, N)) = lo;
+                                *reinterpret_cast<uint4*>(tile + tile_offset(w * ROWS + r, ch + 1, N)) = hi;
                             }
                         }
                         async_proxy_fence();
@@ -468,46 +558,43 @@ attn_chunk_kernel(AttnArgs a) {
                 }
                 row32 = ahead;
             }
-            cur.left -= taken;
-            if (cur.left > 0) attn_advance<R>(a, cur);
         }
-        if (!FP8 && item > 0) {   // an even number of items, two at least: the last two are still to be handed over
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            async_proxy_fence();
-            mbar_arrive(&full[(item - 2) % RING]);
-            mbar_arrive(&full[(item - 1) % RING]);
-        }
-    } else if (lane == 0) {
+        if (!FP8) hand_over(0);
+    } else {
+        if (Sh::SPLIT) set_registers<Sh::MMA_REGS, false>();
+        AttnCursor cur = s_cursor;
+        if (threadIdx.x == kMmaWarp * 32) {
         // ---- products: one thread ----------------------------------------------------------------------------------
         constexpr uint32_t s_idesc = mma_idesc(N, false), o_idesc = mma_idesc(D, true);
         uint32_t item = 0;                // K and V tiles consumed so far
         int segments[TILES] = {}, steps_done[TILES] = {};
         auto scores = [&](int t, int nth, uint32_t k_item) {   // S of the nth step of row block t
             const int buf = SBUF == 1 ? 0 : (nth & 1);
-            const uint32_t q_at = smem_addr(s_q + t * Sh::Q_BYTES), k_at = smem_addr(s_kv + (k_item % RING) * Sh::KV_BYTES);
+            const uint32_t q_low = desc_low(smem_addr(s_q + t * Sh::Q_BYTES), 16);
+            const uint32_t k_low = desc_low(smem_addr(s_kv + (k_item % RING) * Sh::KV_BYTES), 16);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-                const uint64_t qa = smem_desc(q_at + (k >> 2) * 128 * 128 + (k & 3) * 32, 16, 1024);
-                const uint64_t kb = smem_desc(k_at + (k >> 2) * N * 128 + (k & 3) * 32, 16, 1024);
+                const uint64_t qa = smem_desc(q_low, (k >> 2) * 128 * 128 + (k & 3) * 32);
+                const uint64_t kb = smem_desc(k_low, (k >> 2) * N * 128 + (k & 3) * 32);
                 tc_mma_ss(tmem + Sh::S_COL + (t * SBUF + buf) * N, qa, kb, s_idesc, k > 0);
             }
             tc_commit(&s_ready[t * SBUF + buf]);
         };
         auto outputs = [&](int t, int nth, uint32_t v_item, bool add) {
             const int buf = SBUF == 1 ? 0 : (nth & 1);
-            const uint32_t v_at = smem_addr(s_kv + (v_item % RING) * Sh::KV_BYTES);
+            const uint32_t v_low = desc_low(smem_addr(s_kv + (v_item % RING) * Sh::KV_BYTES), N * 128);
 #pragma unroll
             for (int k = 0; k < N / 16; ++k) {
-                const uint64_t vb = smem_desc(v_at + k * 2048, N * 128, 1024);
+                const uint64_t vb = smem_desc(v_low, k * 2048);
                 tc_mma_ts(tmem + Sh::O_COL + t * D, tmem + Sh::S_COL + (t * SBUF + buf) * N + 8 * k, vb, o_idesc, add || k > 0);
             }
             tc_commit(&pv_done[t]);
         };
-        while (cur.left > 0) {
-            const int end = (int)min((long long)cur.units, cur.key_tile + cur.left);
-            const int taken = end - cur.key_tile;
-            int keys, from, to;
-            chunk_steps<D>(a, cur, end, keys, from, to);
+        for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
+            int begin, end, keys, from, to;
+            attn_segment<OV>(a, cur, begin, end);
+            if (begin == end) continue;
+            chunk_steps<D>(a, cur, begin, end, keys, from, to);
             const int blocks = cur.span.n * a.group - cur.tile * R > 128 ? TILES : 1;
             const int count = to - from;
 #pragma unroll
@@ -551,12 +638,11 @@ attn_chunk_kernel(AttnArgs a) {
 #pragma unroll
             for (int t = 0; t < TILES; ++t) steps_done[t] += t < blocks ? count : 0;
             item += 2 * count;
-            cur.left -= taken;
-            if (cur.left > 0) attn_advance<R>(a, cur);
         }
         // every product and every arrival it triggers has landed before the CTA goes (also after a wait that gave up)
         tc_commit(&drained);
         for (int i = 0; i < (1 << 20) && !mbar_try(&drained, 0); ++i) {
+        }
         }
     }
     tc_fence_before();
