@@ -174,29 +174,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// 2^x of a pair on the FMA pipe, for -126 <= x < 127 after clamping from below: x = n + f with n the nearest integer
-// (adding 1.5 * 2^23 leaves n in the low mantissa bits), 2^f by a polynomial of degree 4 that is minimax in relative error
-// on [-1/2, 1/2] (2.7e-6), n added to the exponent. The multi-function unit does 16 exponentials a clock and SM, which
-// would bound the softmax; three pairs in eight are computed here instead.
-__device__ __forceinline__ f32x2 exp2_poly(f32x2 x) {
-    x = f2_pack(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
-    const f32x2 t = f2_add(x, f2_splat(12582912.0f));
-    const f32x2 f = f2_fma(f2_add(t, f2_splat(-12582912.0f)), f2_splat(-1.0f), x);
-    f32x2 p = f2_fma(f2_splat(0.009570105001330376f), f, f2_splat(0.05591785907745361f));
-    p = f2_fma(p, f, f2_splat(0.240247443318367f));
-    p = f2_fma(p, f, f2_splat(0.6931217908859253f));
-    p = f2_fma(p, f, f2_splat(0.9999992847442627f));
-    return f2_pack(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                   __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
-
 template <int D>
 struct ChunkShape {
     static constexpr int TILES = D == 256 ? 1 : 2;        // row blocks of 128
     static constexpr int R = 128 * TILES;                 // rows of a row tile
-    static constexpr int N = D == 256 ? 64 : 128;         // keys of a step
-    static constexpr int SBUF = D == 256 ? 2 : 1;         // S buffers per row block
-    static constexpr int RING = 4;                        // K, V, K, V
+    static constexpr int N = 64;                          // keys of a step
+    static constexpr int SBUF = 2;                        // S buffers per row block
+    static constexpr int SLOTS = D == 256 ? 2 : 4;        // buffers of K tiles, and as many of V tiles
     static constexpr int OV = 2;                          // a row tile's beginning and end cost about two units
     static constexpr int THREADS = 128 * TILES + 256;     // softmax, producers, products (one thread of a warpgroup)
     // Registers: 512 threads start with 128 each; the softmax keeps a row of S in registers.
@@ -207,8 +191,7 @@ struct ChunkShape {
     static constexpr int KV_BYTES = N * D * 2;
     static constexpr int S_COL = 0;                       // tensor memory columns: S buffers, then O
     static constexpr int O_COL = TILES * SBUF * N;
-    static constexpr int BAR_COUNT = 2 * RING + 10;
-    static constexpr int SMEM = 1024 + TILES * Q_BYTES + RING * KV_BYTES;
+    static constexpr int SMEM = 1024 + TILES * Q_BYTES + 2 * SLOTS * KV_BYTES;
 };
 
 // Steps of a segment [begin, end) of key tiles, the same for every role: whole tiles of N keys, none that lies past the
@@ -231,9 +214,9 @@ template <typename T, bool FP8, int D>
 __global__ void __launch_bounds__(ChunkShape<D>::THREADS, 1)
 attn_chunk_kernel(AttnArgs a) {
     using Sh = ChunkShape<D>;
-    constexpr int TILES = Sh::TILES, R = Sh::R, N = Sh::N, SBUF = Sh::SBUF, RING = Sh::RING, OV = Sh::OV;
+    constexpr int TILES = Sh::TILES, R = Sh::R, N = Sh::N, SBUF = Sh::SBUF, SLOTS = Sh::SLOTS, OV = Sh::OV;
     extern __shared__ uint8_t s_raw[];
-    __shared__ uint64_t full[RING], empty[RING], q_ready[TILES], s_ready[TILES * SBUF], p_ready[TILES * SBUF], pv_done[TILES], drained;
+    __shared__ uint64_t full[2 * SLOTS], empty[2 * SLOTS], q_ready[TILES], s_ready[TILES * SBUF], p_ready[TILES * SBUF], pv_done[TILES], drained;
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ AttnCursor s_cursor;
@@ -244,7 +227,7 @@ attn_chunk_kernel(AttnArgs a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < RING; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
+        for (int i = 0; i < 2 * SLOTS; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
         for (int i = 0; i < TILES; ++i) mbar_init(&q_ready[i], 128), mbar_init(&pv_done[i], 1);
         for (int i = 0; i < TILES * SBUF; ++i) mbar_init(&s_ready[i], 1), mbar_init(&p_ready[i], 128);
         mbar_init(&drained, 1);
@@ -376,8 +359,6 @@ attn_chunk_kernel(AttnArgs a) {
                             if (EDGE) {   // hidden keys: a weight of exactly 0 (and scale 0 would make NaN of their -inf)
                                 e.x = base + 2 * (c + i) < lim ? fast_exp2(e.x) : 0.0f;
                                 e.y = base + 2 * (c + i) + 1 < lim ? fast_exp2(e.y) : 0.0f;
-                            } else if (i % 8 == 2 || i % 8 == 5 || i % 8 == 7) {
-                                e = exp2_poly(e);
                             } else {
                                 e = f2_pack(fast_exp2(e.x), fast_exp2(e.y));
                             }
@@ -473,14 +454,75 @@ attn_chunk_kernel(AttnArgs a) {
         constexpr int CPR = D * (FP8 ? 1 : 2) / 16;       // 16-byte pieces of a cache row
         constexpr int RPI = 32 / (CPR < 8 ? CPR : 8);     // rows a warp touches at once
         constexpr int LPR = 32 / RPI;                     // lanes per row
-        uint32_t item = 0;      // K and V tiles asked for so far
-        uint32_t issued = 0, in_flight = 0;   // (cp.async) asked for, and the last of them that are not handed over
-        auto hand_over = [&](uint32_t but) {   // all but the last `but` (0 or 2) of those in flight
+        uint32_t asked[2] = {0, 0};           // K and V tiles so far
+        uint32_t pending = 0, in_flight = 0;  // cp.async: the slots not handed over, four bits each, the oldest on top
+        auto hand_over = [&](uint32_t but) {  // all but the last `but` (0 or 2) of those in flight
             if (in_flight <= but) return;
             if (but == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
             else asm volatile("cp.async.wait_group 2;" ::: "memory");
             async_proxy_fence();
-            for (; in_flight > but; --in_flight) mbar_arrive(&full[(issued - in_flight) % RING]);
+            for (; in_flight > but; --in_flight) mbar_arrive(&full[pending >> (4 * (in_flight - 1)) & 15]);
+        };
+        // tile `which` (0: K, 1: V) of the step whose cache rows are row32
+        auto fetch = [&](int which, int row32) {
+            const uint32_t nth = asked[which]++, slot = which * SLOTS + nth % SLOTS, parity = ((nth / SLOTS) & 1) ^ 1;
+            uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
+            const CacheT* src = static_cast<const CacheT*>(which == 0 ? a.k : a.v);
+            if (!FP8) {
+                // While its buffer is still being read, the warp lets the rows it has asked for arrive, and hands them
+                // over; otherwise two tiles stay in flight.
+                if (!mbar_try(&empty[slot], parity)) {
+                    hand_over(0);
+                    mbar_wait(&empty[slot], parity, gave_up);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < ROWS / RPI; ++i) {
+                    const int r = i * RPI + lane / LPR;
+                    const int row = __shfl_sync(kFullMask, row32, r);
+                    const uint8_t* p = reinterpret_cast<const uint8_t*>(src + ((size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head) * D);
+#pragma unroll
+                    for (int ch = lane % LPR; ch < CPR; ch += LPR) {
+                        const uint32_t dst = smem_addr(tile + tile_offset(w * ROWS + r, ch, N));
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p + 16 * ch), "r"(row < 0 ? 0 : 16) : "memory");
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                pending = pending << 4 | slot;
+                if (++in_flight > 2) hand_over(2);
+            } else {
+                const float* by = which == 0 ? a.k_scales : a.v_scales;
+                const float scale32 = row32 < 0 ? 0.0f : by[(size_t)row32 * a.kv_heads + cur.head];
+                uint4 code[ROWS / RPI][CPR / LPR];
+#pragma unroll
+                for (int i = 0; i < ROWS / RPI; ++i) {
+                    const int row = __shfl_sync(kFullMask, row32, i * RPI + lane / LPR);
+                    const uint8_t* p = reinterpret_cast<const uint8_t*>(src + ((size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head) * D);
+#pragma unroll
+                    for (int j = 0; j < CPR / LPR; ++j) {
+                        code[i][j] = row < 0 ? make_uint4(0, 0, 0, 0) : ldg_stream_v4(p + 16 * (lane % LPR + j * LPR));
+                    }
+                }
+                mbar_wait_warp(&empty[slot], parity, gave_up);
+#pragma unroll
+                for (int i = 0; i < ROWS / RPI; ++i) {
+                    const int r = i * RPI + lane / LPR;
+                    const float scale = __shfl_sync(kFullMask, scale32, r);
+#pragma unroll
+                    for (int j = 0; j < CPR / LPR; ++j) {
+                        const int ch = 2 * (lane % LPR + j * LPR);
+                        uint4 lo, hi;
+                        e4m3x4_scaled(code[i][j].x, scale, lo.x, lo.y);
+                        e4m3x4_scaled(code[i][j].y, scale, lo.z, lo.w);
+                        e4m3x4_scaled(code[i][j].z, scale, hi.x, hi.y);
+                        e4m3x4_scaled(code[i][j].w, scale, hi.z, hi.w);
+                        *reinterpret_cast<uint4*>(tile + tile_offset(w * ROWS + r, ch, N)) = lo;
+                        *reinterpret_cast<uint4*>(tile + tile_offset(w * ROWS + r, ch + 1, N)) = hi;
+                    }
+                }
+                async_proxy_fence();
+                mbar_arrive(&full[slot]);
+            }
         };
         for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
             int begin, end, keys, from, to;
@@ -491,72 +533,21 @@ attn_chunk_kernel(AttnArgs a) {
                 const int key = step * N + w * ROWS + (lane % ROWS);
                 return step < to && key < keys ? attn_cache_row(a, cur.seq, key) : -1;
             };
-            int row32 = lookup(from);
+            // in the order the products want them: SBUF tiles of K, then V and the K of SBUF steps later
+            int rows_of[SBUF + 1];   // cache rows of steps `step` on
+#pragma unroll
+            for (int j = 0; j <= SBUF; ++j) rows_of[j] = lookup(from + j);
+#pragma unroll
+            for (int j = 0; j < SBUF; ++j) {
+                if (from + j < to) fetch(0, rows_of[j]);
+            }
             for (int step = from; step < to; ++step) {
-                const int ahead = lookup(step + 1);
+                const int ahead = lookup(step + SBUF + 1);
+                fetch(1, rows_of[0]);
+                if (step + SBUF < to) fetch(0, rows_of[SBUF]);
 #pragma unroll
-                for (int which = 0; which < 2; ++which, ++item) {
-                    const uint32_t slot = item % RING, parity = ((item / RING) & 1) ^ 1;
-                    uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
-                    const CacheT* src = static_cast<const CacheT*>(which == 0 ? a.k : a.v);
-                    if (!FP8) {
-                        // While its buffer is still being read, the warp lets the rows it has asked for arrive, and hands
-                        // them over; otherwise two items stay in flight.
-                        if (!mbar_try(&empty[slot], parity)) {
-                            hand_over(0);
-                            mbar_wait(&empty[slot], parity, gave_up);
-                        }
-                        __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < ROWS / RPI; ++i) {
-                            const int r = i * RPI + lane / LPR;
-                            const int row = __shfl_sync(kFullMask, row32, r);
-                            const uint8_t* p = reinterpret_cast<const uint8_t*>(src + ((size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head) * D);
-#pragma unroll
-                            for (int ch = lane % LPR; ch < CPR; ch += LPR) {
-                                const uint32_t dst = smem_addr(tile + tile_offset(w * ROWS + r, ch, N));
-                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p + 16 * ch), "r"(row < 0 ? 0 : 16)
-                                             : "memory");
-                            }
-                        }
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        ++issued, ++in_flight;
-                        if (in_flight > 2) hand_over(2);
-                    } else {
-                        const float* by = which == 0 ? a.k_scales : a.v_scales;
-                        const float scale32 = row32 < 0 ? 0.0f : by[(size_t)row32 * a.kv_heads + cur.head];
-                        uint4 code[ROWS / RPI][CPR / LPR];
-#pragma unroll
-                        for (int i = 0; i < ROWS / RPI; ++i) {
-                            const int row = __shfl_sync(kFullMask, row32, i * RPI + lane / LPR);
-                            const uint8_t* p = reinterpret_cast<const uint8_t*>(src + ((size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head) * D);
-#pragma unroll
-                            for (int j = 0; j < CPR / LPR; ++j) {
-                                code[i][j] = row < 0 ? make_uint4(0, 0, 0, 0) : ldg_stream_v4(p + 16 * (lane % LPR + j * LPR));
-                            }
-                        }
-                        mbar_wait_warp(&empty[slot], parity, gave_up);
-#pragma unroll
-                        for (int i = 0; i < ROWS / RPI; ++i) {
-                            const int r = i * RPI + lane / LPR;
-                            const float scale = __shfl_sync(kFullMask, scale32, i * RPI + lane / LPR);
-#pragma unroll
-                            for (int j = 0; j < CPR / LPR; ++j) {
-                                const int ch = 2 * (lane % LPR + j * LPR);
-                                uint4 lo, hi;
-                                e4m3x4_scaled(code[i][j].x, scale, lo.x, lo.y);
-                                e4m3x4_scaled(code[i][j].y, scale, lo.z, lo.w);
-                                e4m3x4_scaled(code[i][j].z, scale, hi.x, hi.y);
-                                e4m3x4_scaled(code[i][j].w, scale, hi.z, hi.w);
-                                *reinterpret_cast<uint4*>(tile + tile_offset(w * ROWS + r, ch, N)) = lo;
-                                *reinterpret_cast<uint4*>(tile + tile_offset(w * ROWS + r, ch + 1, N)) = hi;
-                            }
-                        }
-                        async_proxy_fence();
-                        mbar_arrive(&full[slot]);
-                    }
-                }
-                row32 = ahead;
+                for (int j = 0; j < SBUF; ++j) rows_of[j] = rows_of[j + 1];
+                rows_of[SBUF] = ahead;
             }
         }
         if (!FP8) hand_over(0);
@@ -566,12 +557,12 @@ attn_chunk_kernel(AttnArgs a) {
         if (threadIdx.x == kMmaWarp * 32) {
         // ---- products: one thread ----------------------------------------------------------------------------------
         constexpr uint32_t s_idesc = mma_idesc(N, false), o_idesc = mma_idesc(D, true);
-        uint32_t item = 0;                // K and V tiles consumed so far
+        uint32_t used = 0;                // K tiles, and V tiles, consumed so far
         int segments[TILES] = {}, steps_done[TILES] = {};
-        auto scores = [&](int t, int nth, uint32_t k_item) {   // S of the nth step of row block t
+        auto scores = [&](int t, int nth, uint32_t k_slot) {   // S of the nth step of row block t
             const int buf = SBUF == 1 ? 0 : (nth & 1);
             const uint32_t q_low = desc_low(smem_addr(s_q + t * Sh::Q_BYTES), 16);
-            const uint32_t k_low = desc_low(smem_addr(s_kv + (k_item % RING) * Sh::KV_BYTES), 16);
+            const uint32_t k_low = desc_low(smem_addr(s_kv + k_slot * Sh::KV_BYTES), 16);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
                 const uint64_t qa = smem_desc(q_low, (k >> 2) * 128 * 128 + (k & 3) * 32);
@@ -580,9 +571,9 @@ attn_chunk_kernel(AttnArgs a) {
             }
             tc_commit(&s_ready[t * SBUF + buf]);
         };
-        auto outputs = [&](int t, int nth, uint32_t v_item, bool add) {
+        auto outputs = [&](int t, int nth, uint32_t v_slot, bool add) {
             const int buf = SBUF == 1 ? 0 : (nth & 1);
-            const uint32_t v_low = desc_low(smem_addr(s_kv + (v_item % RING) * Sh::KV_BYTES), N * 128);
+            const uint32_t v_low = desc_low(smem_addr(s_kv + v_slot * Sh::KV_BYTES), N * 128);
 #pragma unroll
             for (int k = 0; k < N / 16; ++k) {
                 const uint64_t vb = smem_desc(v_low, k * 2048);
@@ -602,19 +593,20 @@ attn_chunk_kernel(AttnArgs a) {
                 if (t < blocks) mbar_wait(&q_ready[t], segments[t]++ & 1, gave_up);
             }
             // the first SBUF steps' scores, then for each step its output and the scores SBUF steps later
+            auto k_slot_of = [&](int j) { return (used + j) % SLOTS; };
+            auto tile_parity = [&](int j) { return ((used + j) / SLOTS) & 1; };
             for (int j = 0; j < SBUF && j < count; ++j) {
-                const uint32_t k_item = item + 2 * j;
-                mbar_wait(&full[k_item % RING], (k_item / RING) & 1, gave_up);
+                mbar_wait(&full[k_slot_of(j)], tile_parity(j), gave_up);
                 tc_fence_after();
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
-                    if (t < blocks) scores(t, steps_done[t] + j, k_item);
+                    if (t < blocks) scores(t, steps_done[t] + j, k_slot_of(j));
                 }
-                tc_commit(&empty[k_item % RING]);
+                tc_commit(&empty[k_slot_of(j)]);
             }
             for (int j = 0; j < count; ++j) {
-                const uint32_t v_item = item + 2 * j + 1, k_item = item + 2 * (j + SBUF);
-                mbar_wait(&full[v_item % RING], (v_item / RING) & 1, gave_up);
+                const uint32_t v_slot = SLOTS + k_slot_of(j), k_slot = k_slot_of(j + SBUF);
+                mbar_wait(&full[v_slot], tile_parity(j), gave_up);
                 const bool more = j + SBUF < count;
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
@@ -623,21 +615,21 @@ attn_chunk_kernel(AttnArgs a) {
                     const int buf = SBUF == 1 ? 0 : (nth & 1);
                     mbar_wait(&p_ready[t * SBUF + buf], (SBUF == 1 ? nth : nth >> 1) & 1, gave_up);
                     tc_fence_after();
-                    outputs(t, nth, v_item, j > 0);
-                    if (t == blocks - 1) tc_commit(&empty[v_item % RING]);
+                    outputs(t, nth, v_slot, j > 0);
+                    if (t == blocks - 1) tc_commit(&empty[v_slot]);
                     if (more) {
                         if (t == 0) {
-                            mbar_wait(&full[k_item % RING], (k_item / RING) & 1, gave_up);
+                            mbar_wait(&full[k_slot], tile_parity(j + SBUF), gave_up);
                             tc_fence_after();
                         }
-                        scores(t, nth + SBUF, k_item);
-                        if (t == blocks - 1) tc_commit(&empty[k_item % RING]);
+                        scores(t, nth + SBUF, k_slot);
+                        if (t == blocks - 1) tc_commit(&empty[k_slot]);
                     }
                 }
             }
 #pragma unroll
             for (int t = 0; t < TILES; ++t) steps_done[t] += t < blocks ? count : 0;
-            item += 2 * count;
+            used += count;
         }
         // every product and every arrival it triggers has landed before the CTA goes (also after a wait that gave up)
         tc_commit(&drained);
