@@ -69,9 +69,19 @@ __device__ __forceinline__ void mbar_wait_warp(uint64_t* bar, uint32_t parity, v
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+// Products and commits are issued by the one lane whose `leader` is set, as predicated instructions of a converged warp:
+// their descriptors then stay in uniform registers. (Issued inside a branch that one thread takes, each product cost
+// about 75 cycles to issue, more than most take to execute.)
+__device__ __forceinline__ void tc_commit(uint64_t* bar, uint32_t leader) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)), "r"(leader) : "memory");
 }
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(kFullMask, x, 0); }
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Four E4M3 codes times their row's scale, rounded to bf16 (what a bf16 cache would hold: half a step of 2^-8 per value,
@@ -85,14 +95,14 @@ __device__ __forceinline__ void e4m3x4_scaled(uint32_t w, float scale, uint32_t&
 }
 
 // D[128 x N] (tensor memory) (+)= A B^T; A from shared memory or from tensor memory.
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, uint32_t leader) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
                  : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add, uint32_t leader) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
                  : "memory");
 }
 // 32 consecutive f32 columns of this thread's row.
@@ -128,9 +138,7 @@ __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sy
 // Shared-memory operand descriptor, 128-byte swizzle. Low word: address / 16 and leading byte offset / 16 in the upper half;
 // high word: stride byte offset / 16 (1,024: eight rows of 128 bytes), version, swizzle mode.
 __device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t leading) {
-    uint32_t low = (addr >> 4) | ((leading >> 4) << 16);
-    asm volatile("" : "+r"(low));   // keeps the descriptors of an unrolled loop from being computed, and kept, all at once
-    return low;
+    return (addr >> 4) | ((leading >> 4) << 16);
 }
 __device__ __forceinline__ uint64_t smem_desc(uint32_t low, uint32_t bytes_on) {
     return ((uint64_t)((1024 >> 4) | (1u << 14) | (2u << 29)) << 32) | (low + (bytes_on >> 4));
@@ -216,7 +224,7 @@ attn_chunk_kernel(AttnArgs a) {
     using Sh = ChunkShape<D>;
     constexpr int TILES = Sh::TILES, R = Sh::R, N = Sh::N, SBUF = Sh::SBUF, SLOTS = Sh::SLOTS, OV = Sh::OV;
     extern __shared__ uint8_t s_raw[];
-    __shared__ uint64_t full[2 * SLOTS], empty[2 * SLOTS], q_ready[TILES], s_ready[TILES * SBUF], p_ready[TILES * SBUF], pv_done[TILES], drained;
+    __shared__ uint64_t full[2 * SLOTS], empty[2 * SLOTS], q_ready[TILES], s_ready[TILES * SBUF], p_ready[TILES * SBUF], pv_done[TILES * 2], drained;
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ AttnCursor s_cursor;
@@ -228,8 +236,9 @@ attn_chunk_kernel(AttnArgs a) {
     constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2 * SLOTS; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
-        for (int i = 0; i < TILES; ++i) mbar_init(&q_ready[i], 128), mbar_init(&pv_done[i], 1);
+        for (int i = 0; i < TILES; ++i) mbar_init(&q_ready[i], 128);
         for (int i = 0; i < TILES * SBUF; ++i) mbar_init(&s_ready[i], 1), mbar_init(&p_ready[i], 128);
+        for (int i = 0; i < TILES * 2; ++i) mbar_init(&pv_done[i], 1);
         mbar_init(&drained, 1);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -263,6 +272,12 @@ attn_chunk_kernel(AttnArgs a) {
         const float scale = fabsf(a.scale_log2);
         const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale negates q instead
         int steps_done = 0;                                         // of this row block, over all segments
+        // The product with P of the nth step. Even and odd steps have a barrier each: a wait may be left out, as that for
+        // the step after the next one on the same barrier cannot end before this block's softmax has come that far.
+        auto wait_outputs = [&](int nth) {
+            mbar_wait_warp(&pv_done[2 * t + (nth & 1)], (nth >> 1) & 1, gave_up);
+            tc_fence_after();
+        };
         for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
             int begin, end;
             attn_segment<OV>(a, cur, begin, end);
@@ -330,10 +345,8 @@ attn_chunk_kernel(AttnArgs a) {
                     l *= fix;
                     m = now;
                     if (step > from) {
-                        if (SBUF == 2) {   // S of this step was ready before the last product with P had ended
-                            mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
-                            tc_fence_after();
-                        }   // (with one S buffer its product came after that one)
+                        // O may still be in the last step's product (S of this step came after the one before it)
+                        wait_outputs(steps_done - 1);
 #pragma unroll 1
                         for (int c = 0; c < D; c += 32) {
                             float o[32];
@@ -375,12 +388,9 @@ attn_chunk_kernel(AttnArgs a) {
                 l += sum0.x + sum0.y;
                 tc_wait_st();
                 tc_fence_before();
-                // pv_done is waited for once a step, so that its phase is never more than one ahead of the wait
-                if (SBUF == 2 && steps_done > 0) mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
                 mbar_arrive(&p_ready[t * SBUF + buf]);
             }
-            mbar_wait_warp(&pv_done[t], (steps_done - 1) & 1, gave_up);
-            tc_fence_after();
+            wait_outputs(steps_done - 1);
             const bool whole = begin == 0 && end == cur.keys;
             const int slot = begin == 0 ? 1 : 0;
             float* part = attn_slot(a, blockIdx.x, slot, R, D);
@@ -554,76 +564,78 @@ attn_chunk_kernel(AttnArgs a) {
     } else {
         if (Sh::SPLIT) set_registers<Sh::MMA_REGS, false>();
         AttnCursor cur = s_cursor;
-        if (threadIdx.x == kMmaWarp * 32) {
-        // ---- products: one thread ----------------------------------------------------------------------------------
+        if (warp == kMmaWarp) {
+        // ---- products: one warp, one lane of which issues ----------------------------------------------------------
+        const uint32_t leader = elect_lane();
+        const uint32_t q_base = uniform((int)smem_addr(s_q)), kv_base = uniform((int)smem_addr(s_kv)), acc = uniform((int)tmem);
         constexpr uint32_t s_idesc = mma_idesc(N, false), o_idesc = mma_idesc(D, true);
         uint32_t used = 0;                // K tiles, and V tiles, consumed so far
         int segments[TILES] = {}, steps_done[TILES] = {};
         auto scores = [&](int t, int nth, uint32_t k_slot) {   // S of the nth step of row block t
             const int buf = SBUF == 1 ? 0 : (nth & 1);
-            const uint32_t q_low = desc_low(smem_addr(s_q + t * Sh::Q_BYTES), 16);
-            const uint32_t k_low = desc_low(smem_addr(s_kv + k_slot * Sh::KV_BYTES), 16);
+            const uint32_t q_low = desc_low(q_base + t * Sh::Q_BYTES, 16);
+            const uint32_t k_low = desc_low(kv_base + k_slot * Sh::KV_BYTES, 16);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
                 const uint64_t qa = smem_desc(q_low, (k >> 2) * 128 * 128 + (k & 3) * 32);
                 const uint64_t kb = smem_desc(k_low, (k >> 2) * N * 128 + (k & 3) * 32);
-                tc_mma_ss(tmem + Sh::S_COL + (t * SBUF + buf) * N, qa, kb, s_idesc, k > 0);
+                tc_mma_ss(acc + Sh::S_COL + (t * SBUF + buf) * N, qa, kb, s_idesc, k > 0, leader);
             }
-            tc_commit(&s_ready[t * SBUF + buf]);
+            tc_commit(&s_ready[t * SBUF + buf], leader);
         };
         auto outputs = [&](int t, int nth, uint32_t v_slot, bool add) {
             const int buf = SBUF == 1 ? 0 : (nth & 1);
-            const uint32_t v_low = desc_low(smem_addr(s_kv + v_slot * Sh::KV_BYTES), N * 128);
+            const uint32_t v_low = desc_low(kv_base + v_slot * Sh::KV_BYTES, N * 128);
 #pragma unroll
             for (int k = 0; k < N / 16; ++k) {
                 const uint64_t vb = smem_desc(v_low, k * 2048);
-                tc_mma_ts(tmem + Sh::O_COL + t * D, tmem + Sh::S_COL + (t * SBUF + buf) * N + 8 * k, vb, o_idesc, add || k > 0);
+                tc_mma_ts(acc + Sh::O_COL + t * D, acc + Sh::S_COL + (t * SBUF + buf) * N + 8 * k, vb, o_idesc, add || k > 0, leader);
             }
-            tc_commit(&pv_done[t]);
+            tc_commit(&pv_done[2 * t + (nth & 1)], leader);
         };
-        for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
+        for (; uniform(cur.left > 0); attn_advance<R, OV>(a, cur)) {
             int begin, end, keys, from, to;
             attn_segment<OV>(a, cur, begin, end);
-            if (begin == end) continue;
+            if (uniform(begin == end)) continue;
             chunk_steps<D>(a, cur, begin, end, keys, from, to);
-            const int blocks = cur.span.n * a.group - cur.tile * R > 128 ? TILES : 1;
-            const int count = to - from;
+            const int blocks = uniform(cur.span.n * a.group - cur.tile * R > 128 ? TILES : 1);
+            const int count = uniform(to - from);
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
-                if (t < blocks) mbar_wait(&q_ready[t], segments[t]++ & 1, gave_up);
+                if (t < blocks) mbar_wait_warp(&q_ready[t], segments[t]++ & 1, gave_up);
             }
             // the first SBUF steps' scores, then for each step its output and the scores SBUF steps later
             auto k_slot_of = [&](int j) { return (used + j) % SLOTS; };
             auto tile_parity = [&](int j) { return ((used + j) / SLOTS) & 1; };
             for (int j = 0; j < SBUF && j < count; ++j) {
-                mbar_wait(&full[k_slot_of(j)], tile_parity(j), gave_up);
+                mbar_wait_warp(&full[k_slot_of(j)], tile_parity(j), gave_up);
                 tc_fence_after();
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
                     if (t < blocks) scores(t, steps_done[t] + j, k_slot_of(j));
                 }
-                tc_commit(&empty[k_slot_of(j)]);
+                tc_commit(&empty[k_slot_of(j)], leader);
             }
             for (int j = 0; j < count; ++j) {
                 const uint32_t v_slot = SLOTS + k_slot_of(j), k_slot = k_slot_of(j + SBUF);
-                mbar_wait(&full[v_slot], tile_parity(j), gave_up);
+                mbar_wait_warp(&full[v_slot], tile_parity(j), gave_up);
                 const bool more = j + SBUF < count;
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
                     if (t >= blocks) break;
                     const int nth = steps_done[t] + j;
                     const int buf = SBUF == 1 ? 0 : (nth & 1);
-                    mbar_wait(&p_ready[t * SBUF + buf], (SBUF == 1 ? nth : nth >> 1) & 1, gave_up);
+                    mbar_wait_warp(&p_ready[t * SBUF + buf], (SBUF == 1 ? nth : nth >> 1) & 1, gave_up);
                     tc_fence_after();
                     outputs(t, nth, v_slot, j > 0);
-                    if (t == blocks - 1) tc_commit(&empty[v_slot]);
+                    if (t == blocks - 1) tc_commit(&empty[v_slot], leader);
                     if (more) {
                         if (t == 0) {
-                            mbar_wait(&full[k_slot], tile_parity(j + SBUF), gave_up);
+                            mbar_wait_warp(&full[k_slot], tile_parity(j + SBUF), gave_up);
                             tc_fence_after();
                         }
                         scores(t, nth + SBUF, k_slot);
-                        if (t == blocks - 1) tc_commit(&empty[k_slot]);
+                        if (t == blocks - 1) tc_commit(&empty[k_slot], leader);
                     }
                 }
             }
@@ -632,7 +644,7 @@ attn_chunk_kernel(AttnArgs a) {
             used += count;
         }
         // every product and every arrival it triggers has landed before the CTA goes (also after a wait that gave up)
-        tc_commit(&drained);
+        tc_commit(&drained, leader);
         for (int i = 0; i < (1 << 20) && !mbar_try(&drained, 0); ++i) {
         }
         }
