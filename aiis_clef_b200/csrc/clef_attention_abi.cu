@@ -33,7 +33,7 @@ AttnPlan attn_plan(int n_seqs, int total_q, int q_heads, int kv_heads, int head_
     p.rows = p.chunk ? (head_dim == 256 ? 128 : 256) : (rows > 8LL * n_seqs ? 16 : 8);
     p.items = ((size_t)(rows / p.rows) + n_seqs) * kv_heads;
     const size_t ctas = p.chunk ? kAttnMaxCtas / 2 : kAttnMaxCtas;
-    p.bytes = (size_t)kAttnMaxCtas * 2 * sizeof(AttnDesc) + ctas * 2 * p.rows * (head_dim + 2) * sizeof(float);
+    p.bytes = (size_t)kAttnMaxCtas * sizeof(AttnDesc) + ctas * 2 * p.rows * (head_dim + 2) * sizeof(float);
     return p;
 }
 
@@ -65,7 +65,7 @@ void launch_pdl(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t
 }
 
 // Launches `kernel` on the list of units, and the joining kernel where a row tile may have been cut.
-template <typename T, int D, int R, bool ROWS, typename K>
+template <typename T, int D, int R, bool CHUNK, typename K>
 int launch_units(K kernel, unsigned threads, size_t smem, size_t most, cudaStream_t s, const AttnArgs& a, const AttnPlan& plan,
                  const char* what) {
     const size_t key_tiles = ((size_t)a.table_width * a.page_size + kAttnKeys - 1) / kAttnKeys;
@@ -73,9 +73,11 @@ int launch_units(K kernel, unsigned threads, size_t smem, size_t most, cudaStrea
     launch_pdl(kernel, dim3(ctas, 1, 1), threads, smem, s, a);
     if (int r = check_launch(what)) return r;
     if (key_tiles <= 1 || ctas <= 1) return CLEF_OK;
-    const unsigned runs = clamp_grid(plan.items, ctas);
-    if constexpr (ROWS) launch_pdl(attn_combine_rows_kernel<T, D, R>, dim3(runs, R / 32, 1), 256, 0, s, a, (int)ctas);
-    else launch_pdl(attn_combine_kernel<T, D, R>, dim3(runs, R, 1), 256, 0, s, a, (int)ctas);
+    // a run of 32 possible beginnings at most, fewer where more row tiles may begin
+    const unsigned runs = clamp_grid(plan.items > (ctas + 31) / 32 ? plan.items : (ctas + 31) / 32, ctas);
+    if constexpr (CHUNK) launch_pdl(attn_combine_rows_kernel<T, D, R>, dim3(runs, R / 32, 1), 256, 0, s, a, (int)ctas);
+    else if (ctas > 8 * plan.items) launch_pdl(attn_combine_kernel<T, D, R, 8>, dim3(runs, R, D / 64), 256, 0, s, a, (int)ctas);
+    else launch_pdl(attn_combine_kernel<T, D, R, 1>, dim3(runs, R / 8, 1), 256, 0, s, a, (int)ctas);
     return check_launch(what);
 }
 
@@ -186,7 +188,7 @@ int clef_paged_attention(clef_stream_t stream, void* out, const void* q, const v
     a.group_div = make_fast_div((uint32_t)group), a.page_div = make_fast_div((uint32_t)page_size);
     a.scale_log2 = scale * 1.44269504088896341f;
     a.desc = static_cast<AttnDesc*>(workspace);
-    a.part = reinterpret_cast<float*>(a.desc + 2 * kAttnMaxCtas);
+    a.part = reinterpret_cast<float*>(a.desc + kAttnMaxCtas);
     cudaStream_t s = as_stream(stream);
     if (dtype == CLEF_BF16) {
         return cache_dtype == CLEF_BF16 ? launch_attention<Bf16, false>(s, dev, a, plan, head_dim, what)

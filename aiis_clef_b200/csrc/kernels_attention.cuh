@@ -38,15 +38,15 @@ struct AttnArgs {
     int page_size, table_width, cache_pages;
     FastDiv group_div, page_div;
     float scale_log2;           // scale * log2(e): the softmax runs on exp2
-    struct AttnDesc* desc;      // workspace: what is in the two slots of each CTA
+    struct AttnDesc* desc;      // workspace: what is in slot 1 of each CTA
     float* part;                // workspace: per slot R maxima, R sums, R x head_dim outputs (attn_chunk_kernel: [head_dim / 4][R][4])
 };
 
-// Slot states. Slot 0 of a CTA holds the end (or the middle) of a row tile begun by an earlier CTA, slot 1 the
-// beginning of one that a later CTA ends.
-enum AttnSlot { kAttnNone = 0, kAttnFirst = 1, kAttnMiddle = 2, kAttnLast = 3 };
+// Slot 1 of a CTA holds the beginning of a row tile that later CTAs go on with, slot 0 its CTA's share of a row tile
+// begun by an earlier one. What is in slot 1:
 struct AttnDesc {
-    int state, tile, head, q0, rows;   // rows: of the sequence and kv head
+    int parts;                    // CTAs that share the row tile, this one first; 0: the slot is empty
+    int tile, head, q0, rows;     // rows: of the sequence and kv head
     int unused[3];
 };
 
@@ -102,7 +102,7 @@ __device__ __forceinline__ long long attn_seq_cost(const AttnArgs& a, const Attn
 struct AttnCursor {
     int seq, head, tile, keys;   // `keys`: key tiles of the row tile
     AttnSeq span;
-    long long cost, at, left;
+    long long cost, at, left, share;
 };
 
 // The cursor of CTA `cta` of `ctas`. One warp, all lanes; every lane has the result.
@@ -118,9 +118,9 @@ __device__ inline AttnCursor attn_locate(const AttnArgs& a, int cta, int ctas) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(kFullMask, total, off);
     // equal shares, but of a key tile at least: the CTAs that work are the first ones
-    const long long share = max((total + ctas - 1) / ctas, (long long)a.group * kAttnKeys);
-    long long at = cta * share;
-    c.left = min(share, total - at);
+    c.share = max((total + ctas - 1) / ctas, (long long)a.group * kAttnKeys);
+    long long at = cta * c.share;
+    c.left = min(c.share, total - at);
     if (c.left <= 0) return c;
     long long per_head = 0;
     for (int base = 0; base < a.n_seqs; base += 32) {   // the sequence: scans of 32
@@ -171,14 +171,23 @@ __device__ inline AttnCursor attn_locate(const AttnArgs& a, int cta, int ctas) {
 // key tiles before it are those of round((x - OV units) / unit); none, if it ends within the OV units (the next CTA then
 // begins the row tile), all, if the row tile ends in the share.
 template <int OV>
+__device__ __forceinline__ int attn_tiles_before(const AttnArgs& a, const AttnCursor& c, long long x) {
+    const int unit = a.group * kAttnKeys, y = (int)(x - (long long)OV * unit) + unit / 2;
+    return y <= 0 ? 0 : min(c.keys, y / unit);
+}
+template <int OV>
 __device__ __forceinline__ void attn_segment(const AttnArgs& a, const AttnCursor& c, int& begin, int& end) {
-    const int unit = a.group * kAttnKeys;
-    auto before = [&](long long x) {
-        const int y = (int)(x - (long long)OV * unit) + unit / 2;
-        return y <= 0 ? 0 : min(c.keys, y / unit);
-    };
-    begin = before(c.at);
-    end = c.at + c.left >= c.cost ? c.keys : before(c.at + c.left);
+    begin = attn_tiles_before<OV>(a, c, c.at);
+    end = c.at + c.left >= c.cost ? c.keys : attn_tiles_before<OV>(a, c, c.at + c.left);
+}
+// The description of a row tile that begins in this CTA's share and goes on after it: the shares that follow, up to the
+// row tile's end or the one that finds no key tile left.
+template <int OV>
+__device__ __forceinline__ AttnDesc attn_describe(const AttnArgs& a, const AttnCursor& c) {
+    const long long rest = c.cost - (c.at + c.left);
+    int more = (int)((rest + c.share - 1) / c.share);
+    while (more > 0 && attn_tiles_before<OV>(a, c, c.at + c.left + (more - 1) * c.share) >= c.keys) --more;
+    return AttnDesc{1 + more, c.tile, c.head, c.span.q0, c.span.n * a.group};
 }
 
 // On to the next row tile, if some of the share is left.
@@ -214,19 +223,27 @@ __device__ __forceinline__ int attn_cache_row(const AttnArgs& a, int seq, int t)
     return (unsigned)at < (unsigned)a.cache_pages ? at * a.page_size + (t - page * a.page_size) : -1;
 }
 
-// Four E4M3 codes -> two bf16 pairs, exactly: sign, exponent and mantissa bits moved into a bf16 pattern read 2^120 too
-// small (the biases are 7 and 127), and one multiplication by 2^120, which also normalises the subnormal codes.
-__device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
-    const uint32_t x = (a & 0x80008000u) | ((a >> 4) & 0x07f007f0u), y = (b & 0x80008000u) | ((b >> 4) & 0x07f007f0u);
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(0x7b807b80u));
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(y), "r"(0x7b807b80u));
+// Four E4M3 codes -> two f16 pairs, exactly.
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 
-__device__ __forceinline__ void mma_bf16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+template <bool F16>
+__device__ __forceinline__ void mma_16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if (F16) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t r;
@@ -244,6 +261,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // and 16 bytes at column 16 r of keys 2c, 2c + 1, 2c + 8, 2c + 9 for O^T, where a byte permute pairs two keys. Warps
 // take 16 keys each, keep their own softmax statistics, and are joined in shared memory at the end of a row tile.
 // The next keys are requested as soon as the registers of the current ones are free.
+// An FP8 cache is multiplied in f16, which holds every E4M3 code and which one conversion instruction gives for two
+// codes (bf16 takes five). What else enters the products is brought into f16's range by powers of two: a q row is
+// divided by one so that its largest element is in [1, 2), and weight times value scale by the running maximum of the
+// value scales; both are multiplied back in f32. f16 then rounds finer than bf16 (2^-11), down to 2^-14 of the maximum.
 // ---------------------------------------------------------------------------------------------
 template <typename T, bool FP8, int D, int NT>
 __global__ void __launch_bounds__(kAttnThreads, (D == 256 || NT > 1 || !FP8) ? 1 : 2)
@@ -271,8 +292,7 @@ attn_rows_kernel(AttnArgs a) {
         const AttnCursor at = attn_locate<R, OV>(a, blockIdx.x, gridDim.x);
         if (lane == 0) s_cursor = at;
     }
-    AttnDesc* desc = a.desc + 2 * blockIdx.x;
-    if (threadIdx.x < 2) desc[threadIdx.x].state = kAttnNone;
+    if (threadIdx.x == 0) a.desc[blockIdx.x].parts = 0;
     __syncthreads();
     AttnCursor cur = s_cursor;
     for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
@@ -283,21 +303,45 @@ attn_rows_kernel(AttnArgs a) {
         const int row0 = cur.tile * R, rows = span.n * a.group;
         // q of this lane's row r (and r + 8): the columns that meet its K columns
         uint32_t qf[NT][D / 16][2];
-        int lim[NT][2];   // keys seen by rows 2c and 2c + 1 of each 8
+        int lim[NT][2];     // keys seen by rows 2c and 2c + 1 of each 8
+        float back[NT][2];  // FP8: score scale of those rows
+        float v_most = 0.0f;   // FP8: a power of two no value scale so far is above; o is that much too small
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int x = row0 + nt * 8 + r;
             const int token = (int)fast_div((uint32_t)x, a.group_div);
             const size_t at = ((size_t)(span.q0 + token) * a.q_heads + cur.head * a.group + (x - token * a.group)) * D;
             const typename T::storage* qr = static_cast<const typename T::storage*>(a.q) + at;
+            float4 f[D / 16];
+            float most = 0.0f;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 // bf16: 8 columns (two steps) at 32 (i / 2) + 8 c; FP8: 16 columns (four steps) at 64 (i / 4) + 16 c
                 const int col = FP8 ? 64 * (i >> 2) + 16 * c + 4 * (i & 3) : 32 * (i >> 1) + 8 * c + 4 * (i & 1);
-                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (x < rows) f = load_quad<T>(qr + col, 0);
-                qf[nt][i][0] = pack_bf16x2(f.x, f.y);
-                qf[nt][i][1] = pack_bf16x2(f.z, f.w);
+                f[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (x < rows) f[i] = load_quad<T>(qr + col, 0);
+                if (FP8) most = fmaxf(fmaxf(fmaxf(most, fabsf(f[i].x)), fmaxf(fabsf(f[i].y), fabsf(f[i].z))), fabsf(f[i].w));
+            }
+            if (FP8) {
+                most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
+                // the power of two below it, kept where it and its reciprocal are normal numbers
+                const int exponent = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100);
+                const float down = __uint_as_float((uint32_t)(127 - exponent) << 23), up = __uint_as_float((uint32_t)(127 + exponent) << 23);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    qf[nt][i][0] = pack_f16x2(f[i].x * down, f[i].y * down);
+                    qf[nt][i][1] = pack_f16x2(f[i].z * down, f[i].w * down);
+                }
+                // row r's factor to the lanes whose columns of S^T are rows 2c and 2c + 1
+                back[nt][0] = a.scale_log2 * __shfl_sync(kFullMask, up, 8 * c);
+                back[nt][1] = a.scale_log2 * __shfl_sync(kFullMask, up, 8 * c + 4);
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    qf[nt][i][0] = pack_bf16x2(f[i].x, f[i].y);
+                    qf[nt][i][1] = pack_bf16x2(f[i].z, f[i].w);
+                }
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -371,22 +415,43 @@ attn_rows_kernel(AttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         uint32_t f[4];
-                        e4m3x4_to_bf16(w0[e], f[0], f[2]);
-                        e4m3x4_to_bf16(w1[e], f[1], f[3]);
+                        e4m3x4_to_f16(w0[e], f[0], f[2]);
+                        e4m3x4_to_f16(w1[e], f[1], f[3]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_bf16(s[nt], f, qf[nt][4 * i + e][0], qf[nt][4 * i + e][1]);
+                        for (int nt = 0; nt < NT; ++nt) mma_16816<FP8>(s[nt], f, qf[nt][4 * i + e][0], qf[nt][4 * i + e][1]);
                     }
                 } else {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const uint32_t f[4] = {w0[2 * e], w1[2 * e], w0[2 * e + 1], w1[2 * e + 1]};
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_bf16(s[nt], f, qf[nt][2 * i + e][0], qf[nt][2 * i + e][1]);
+                        for (int nt = 0; nt < NT; ++nt) mma_16816<FP8>(s[nt], f, qf[nt][2 * i + e][0], qf[nt][2 * i + e][1]);
                     }
                 }
             }
-            const float ks0 = FP8 ? ks[0] * a.scale_log2 : a.scale_log2, ks1 = FP8 ? ks[1] * a.scale_log2 : a.scale_log2;
-            const float vs0 = FP8 ? vs[0] : 1.0f, vs1 = FP8 ? vs[1] : 1.0f;
+            float ks0 = 0.0f, ks1 = 0.0f, vs0 = 0.0f, vs1 = 0.0f;
+            if (FP8) {
+                ks0 = ks[0], ks1 = ks[1];
+                const float most = fmaxf(vs[0], vs[1]);
+                if (__any_sync(kFullMask, most > v_most)) {
+                    float now = most;
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) now = fmaxf(now, __shfl_xor_sync(kFullMask, now, off));
+                    now = __uint_as_float((__float_as_uint(fmaxf(now, 1e-37f)) + 0x007fffffu) & 0x7f800000u);   // up to a power of two
+                    const float fix = v_most / now;   // 0 at first
+                    v_most = now;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int b = 0; b < VL; ++b) {
+#pragma unroll
+                            for (int i = 0; i < VCH / 2; ++i) o[nt][b][i][0] *= fix, o[nt][b][i][1] *= fix, o[nt][b][i][2] *= fix, o[nt][b][i][3] *= fix;
+                        }
+                    }
+                }
+                const float inv = v_most > 0.0f ? 1.0f / v_most : 0.0f;
+                vs0 = vs[0] * inv, vs1 = vs[1] * inv;
+            }
             const bool more = tile + 1 < end;
             if (more) load_k(row16);
             uint32_t pf[NT][2];
@@ -395,8 +460,9 @@ attn_rows_kernel(AttnArgs a) {
                 float top[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    s[nt][e] = t0 + r < lim[nt][e] ? s[nt][e] * ks0 : -INFINITY;
-                    s[nt][2 + e] = t0 + r + 8 < lim[nt][e] ? s[nt][2 + e] * ks1 : -INFINITY;
+                    const float k0 = FP8 ? ks0 * back[nt][e] : a.scale_log2, k1 = FP8 ? ks1 * back[nt][e] : a.scale_log2;
+                    s[nt][e] = t0 + r < lim[nt][e] ? s[nt][e] * k0 : -INFINITY;
+                    s[nt][2 + e] = t0 + r + 8 < lim[nt][e] ? s[nt][2 + e] * k1 : -INFINITY;
                     top[e] = fmaxf(s[nt][e], s[nt][2 + e]);
                 }
 #pragma unroll
@@ -430,7 +496,7 @@ attn_rows_kernel(AttnArgs a) {
                     p[2 + e] = fast_exp2(s[nt][2 + e] - ref);
                     l[nt][e] += p[e] + p[2 + e];
                 }
-                // weights rounded to bf16 for the product (the sum above keeps them in f32); masked keys stay exactly 0
+                // weights rounded to bf16 or f16 for the product (the sum above keeps them in f32); masked keys stay exactly 0
                 if (FP8) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -438,8 +504,8 @@ attn_rows_kernel(AttnArgs a) {
                         p[2 + e] = p[2 + e] == 0.0f ? 0.0f : p[2 + e] * vs1;
                     }
                 }
-                pf[nt][0] = transpose8x8(pack_bf16x2(p[0], p[1]));
-                pf[nt][1] = transpose8x8(pack_bf16x2(p[2], p[3]));
+                pf[nt][0] = transpose8x8(FP8 ? pack_f16x2(p[0], p[1]) : pack_bf16x2(p[0], p[1]));
+                pf[nt][1] = transpose8x8(FP8 ? pack_f16x2(p[2], p[3]) : pack_bf16x2(p[2], p[3]));
             }
 #pragma unroll
             for (int b = 0; b < VL; ++b) {
@@ -447,20 +513,20 @@ attn_rows_kernel(AttnArgs a) {
                 for (int w = 0; w < VW; ++w) {
                     if (FP8) {   // a word is 4 dims: pair keys (0, 1) and (2, 3) dim by dim, then widen
                         uint32_t f[2][4];
-                        e4m3x4_to_bf16(__byte_perm(vr[0][b][w], vr[1][b][w], 0x5140), f[0][0], f[0][1]);
-                        e4m3x4_to_bf16(__byte_perm(vr[2][b][w], vr[3][b][w], 0x5140), f[0][2], f[0][3]);
-                        e4m3x4_to_bf16(__byte_perm(vr[0][b][w], vr[1][b][w], 0x7362), f[1][0], f[1][1]);
-                        e4m3x4_to_bf16(__byte_perm(vr[2][b][w], vr[3][b][w], 0x7362), f[1][2], f[1][3]);
+                        e4m3x4_to_f16(__byte_perm(vr[0][b][w], vr[1][b][w], 0x5140), f[0][0], f[0][1]);
+                        e4m3x4_to_f16(__byte_perm(vr[2][b][w], vr[3][b][w], 0x5140), f[0][2], f[0][3]);
+                        e4m3x4_to_f16(__byte_perm(vr[0][b][w], vr[1][b][w], 0x7362), f[1][0], f[1][1]);
+                        e4m3x4_to_f16(__byte_perm(vr[2][b][w], vr[3][b][w], 0x7362), f[1][2], f[1][3]);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_bf16(o[nt][b][2 * w + h], f[h], pf[nt][0], pf[nt][1]);
+                            for (int nt = 0; nt < NT; ++nt) mma_16816<FP8>(o[nt][b][2 * w + h], f[h], pf[nt][0], pf[nt][1]);
                         }
                     } else {     // a word is 2 dims
                         const uint32_t f[4] = {__byte_perm(vr[0][b][w], vr[1][b][w], 0x5410), __byte_perm(vr[0][b][w], vr[1][b][w], 0x7632),
                                                __byte_perm(vr[2][b][w], vr[3][b][w], 0x5410), __byte_perm(vr[2][b][w], vr[3][b][w], 0x7632)};
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_bf16(o[nt][b][w], f, pf[nt][0], pf[nt][1]);
+                        for (int nt = 0; nt < NT; ++nt) mma_16816<FP8>(o[nt][b][w], f, pf[nt][0], pf[nt][1]);
                     }
                 }
             }
@@ -486,7 +552,8 @@ attn_rows_kernel(AttnArgs a) {
                 for (int b = 0; b < VL; ++b) {
 #pragma unroll
                     for (int i = 0; i < VCH / 2; ++i) {
-                        *reinterpret_cast<float2*>(dst + 8 * VCH * b + 2 * i) = make_float2(o[nt][b][i][e], o[nt][b][i][2 + e]);
+                        const float by = FP8 ? v_most : 1.0f;
+                        *reinterpret_cast<float2*>(dst + 8 * VCH * b + 2 * i) = make_float2(o[nt][b][i][e] * by, o[nt][b][i][2 + e] * by);
                     }
                 }
             }
@@ -495,9 +562,7 @@ attn_rows_kernel(AttnArgs a) {
         const bool whole = begin == 0 && end == cur.keys;
         const int slot = begin == 0 ? 1 : 0;
         float* part = attn_slot(a, blockIdx.x, slot, R, D);
-        if (!whole && threadIdx.x == 0) {
-            desc[slot] = AttnDesc{begin == 0 ? kAttnFirst : (end == cur.keys ? kAttnLast : kAttnMiddle), cur.tile, cur.head, span.q0, rows};
-        }
+        if (!whole && begin == 0 && threadIdx.x == 0) a.desc[blockIdx.x] = attn_describe<OV>(a, cur);
         for (int i = threadIdx.x; i < R * (D / 4); i += kAttnThreads) {
             const int x = i / (D / 4), col = (i % (D / 4)) * 4;
             float top = -INFINITY;
@@ -534,19 +599,21 @@ attn_rows_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins the partials of the row tiles that several CTAs shared: a tile is begun in slot 1 of one CTA and continued in
-// slot 0 of the CTAs after it, up to the one marked last. blockIdx.x takes a run of CTAs as possible beginnings.
-// attn_combine_kernel: few rows with many partials (attn_rows_kernel), a block per row; the 8 warps take every eighth
-// partial and are joined in shared memory in a fixed order.
-// attn_combine_rows_kernel: many rows with few partials (attn_chunk_kernel), four rows per warp.
+// Joins the partials of the row tiles that several CTAs shared: slot 1 of the CTA that began one, slot 0 of the CTAs after
+// it. blockIdx.x takes a run of CTAs as possible beginnings, 32 at a time. One pass with a running maximum, the statistics
+// and outputs of several partials requested together: the time is a chain of memory latencies.
+// attn_combine_kernel (partials of attn_rows_kernel): WARPS = 8, few row tiles with many partials: a block per row and 64
+// columns, warp w takes every eighth partial, joined in shared memory in a fixed order; WARPS = 1: a warp per row.
+// attn_combine_rows_kernel (of attn_chunk_kernel): many rows with few partials, four rows per warp.
 // ---------------------------------------------------------------------------------------------
-// Partials of the row tile that CTA `first` begins; a warp looks at the 32 CTAs after it at a time.
-__device__ __forceinline__ int attn_parts(const AttnArgs& a, int first, int ctas) {
-    for (int from = first + 1;; from += 32) {
+// The next CTA from `from` on, before `to`, that begins a row tile others go on with; `to` if there is none.
+__device__ __forceinline__ int attn_next_first(const AttnArgs& a, int from, int to) {
+    for (; from < to; from += 32) {
         const int at = from + (int)(threadIdx.x & 31);
-        const unsigned ends = __ballot_sync(kFullMask, at >= ctas - 1 || a.desc[2 * at].state == kAttnLast);
-        if (ends) return from + __ffs(ends) - first;
+        const unsigned begins = __ballot_sync(kFullMask, at < to && a.desc[at].parts > 0);
+        if (begins) return from + __ffs(begins) - 1;
     }
+    return to;
 }
 template <typename T>
 __device__ __forceinline__ typename T::storage* attn_out_row(const AttnArgs& a, const AttnDesc& d, int row, int head_dim) {
@@ -555,55 +622,96 @@ __device__ __forceinline__ typename T::storage* attn_out_row(const AttnArgs& a, 
            ((size_t)(d.q0 + token) * a.q_heads + d.head * a.group + (row - token * a.group)) * head_dim;
 }
 
-template <typename T, int D, int R>
+template <typename T, int D, int R, int WARPS>
 __global__ void __launch_bounds__(256)
 attn_combine_kernel(AttnArgs a, int ctas) {
-    constexpr int WARPS = 8;
-    __shared__ float s_acc[WARPS][D + 2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int COLS = WARPS == 1 ? D : 64, V = COLS / 32, AHEAD = 8 / (V / 2 > 2 ? 2 : 1);
+    __shared__ float s_acc[WARPS == 1 ? 1 : 8][COLS + 2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = WARPS == 1 ? 0 : warp;
+    const int x = WARPS == 1 ? blockIdx.y * 8 + warp : blockIdx.y, col = blockIdx.z * COLS + lane * V;
     pdl_launch_dependents();
     pdl_wait_prior_grids();
     const int from = (int)((long long)blockIdx.x * ctas / gridDim.x), to = (int)((long long)(blockIdx.x + 1) * ctas / gridDim.x);
-    for (int first = from; first < to; ++first) {
-        const AttnDesc d = a.desc[2 * first + 1];
-        const int x = blockIdx.y, row = d.tile * R + x;
-        if (d.state != kAttnFirst || row >= d.rows) continue;
-        const int parts = attn_parts(a, first, ctas);
-        auto part_of = [&](int i) { return attn_slot(a, first + i, i == 0 ? 1 : 0, R, D); };
-        float top = -INFINITY;
-        for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_of(i)[x]);
+    for (int first = attn_next_first(a, from, to); first < to; first = attn_next_first(a, first + 1, to)) {
+        const AttnDesc d = a.desc[first];
+        const int row = d.tile * R + x;
+        if (row >= d.rows) continue;   // (the same for the whole block, or a warp of its own)
+        float top = -INFINITY, sum = 0.0f, acc[V];
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f;
-        float acc[D / 32];
+        for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+        for (int i0 = sub; i0 < d.parts; i0 += WARPS * AHEAD) {
+            float m[AHEAD], l[AHEAD];
+            float2 o[AHEAD][V / 2];
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-        for (int i = warp; i < parts; i += WARPS) {
-            const float* p = part_of(i);
-            const float f = fast_exp2(p[x] - ref);
-            sum = fmaf(f, p[R + x], sum);
+            for (int j = 0; j < AHEAD; ++j) {
+                const int i = i0 + j * WARPS;
+                if (i < d.parts) {
+                    const float* p = attn_slot(a, first + i, i == 0 ? 1 : 0, R, D);
+                    m[j] = p[x], l[j] = p[R + x];
 #pragma unroll
-            for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(f, p[2 * R + (size_t)x * D + lane + 32 * e], acc[e]);
+                    for (int e = 0; e < V / 2; ++e) o[j][e] = reinterpret_cast<const float2*>(p + 2 * R + (size_t)x * D + col)[e];
+                }
+            }
+            float now = top;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) now = fmaxf(now, i0 + j * WARPS < d.parts ? m[j] : -INFINITY);
+            const float ref = now == -INFINITY ? 0.0f : now, g = fast_exp2(top - ref);
+            top = now;
+            sum *= g;
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] *= g;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                if (i0 + j * WARPS < d.parts) {
+                    const float f = fast_exp2(m[j] - ref);
+                    sum = fmaf(f, l[j], sum);
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) {
+                        acc[2 * e] = fmaf(f, o[j][e].x, acc[2 * e]);
+                        acc[2 * e + 1] = fmaf(f, o[j][e].y, acc[2 * e + 1]);
+                    }
+                }
+            }
         }
+        float2 out[V / 2];
+        if (WARPS == 1) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) s_acc[warp][lane + 32 * e] = acc[e];
-        if (lane == 0) s_acc[warp][D] = sum;
-        __syncthreads();
-        if (threadIdx.x < D / 4) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            float total = 0.0f;
+            for (int e = 0; e < V / 2; ++e) out[e] = make_float2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+        } else {
+            __syncthreads();   // the last row tile's join is over
+#pragma unroll
+            for (int e = 0; e < V; ++e) s_acc[warp][lane * V + e] = acc[e];
+            if (lane == 0) s_acc[warp][COLS] = sum, s_acc[warp][COLS + 1] = top;
+            __syncthreads();
+            float most = -INFINITY, total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) most = fmaxf(most, s_acc[w][COLS + 1]);
+            if (most == -INFINITY) most = 0.0f;
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) out[e] = make_float2(0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                const float* p = s_acc[w] + 4 * threadIdx.x;
-                v.x += p[0], v.y += p[1], v.z += p[2], v.w += p[3];
-                total += s_acc[w][D];
+                const float f = fast_exp2(s_acc[w][COLS + 1] - most);
+                total = fmaf(f, s_acc[w][COLS], total);
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    out[e].x = fmaf(f, s_acc[w][lane * V + 2 * e], out[e].x);
+                    out[e].y = fmaf(f, s_acc[w][lane * V + 2 * e + 1], out[e].y);
+                }
             }
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            store_quad<T>(attn_out_row<T>(a, d, row, D), threadIdx.x, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) out[e] = make_float2(out[e].x * inv, out[e].y * inv);
         }
-        __syncthreads();
+        if (sub == 0) {
+            typename T::storage* dst = attn_out_row<T>(a, d, row, D) + col;
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) {
+                if (T::kBytes == 2) reinterpret_cast<uint32_t*>(dst)[e] = pack_bf16x2(out[e].x, out[e].y);
+                else reinterpret_cast<float2*>(dst)[e] = out[e];
+            }
+        }
     }
 }
 
@@ -615,18 +723,16 @@ attn_combine_rows_kernel(AttnArgs a, int ctas) {
     pdl_launch_dependents();
     pdl_wait_prior_grids();
     const int from = (int)((long long)blockIdx.x * ctas / gridDim.x), to = (int)((long long)(blockIdx.x + 1) * ctas / gridDim.x);
-    for (int first = from; first < to; ++first) {
-        const AttnDesc d = a.desc[2 * first + 1];
+    for (int first = attn_next_first(a, from, to); first < to; first = attn_next_first(a, first + 1, to)) {
+        const AttnDesc d = a.desc[first];
         const int x0 = (blockIdx.y * 8 + warp) * 4, x = x0 + (lane & 3);
-        if (d.state != kAttnFirst || d.tile * R + x0 >= d.rows) continue;
-        const int parts = attn_parts(a, first, ctas);
-        // one pass with a running maximum: the statistics and outputs of a partial are requested together
+        if (d.tile * R + x0 >= d.rows) continue;
         float top = -INFINITY, sum = 0.0f;
         float4 acc[Q];
 #pragma unroll
         for (int e = 0; e < Q; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
-        for (int i = 0; i < parts; ++i) {
+        for (int i = 0; i < d.parts; ++i) {
             const float* p = attn_slot(a, first + i, i == 0 ? 1 : 0, R, D);
             const float4* src = reinterpret_cast<const float4*>(p + 2 * R) + (lane >> 2) * R + x;
             float4 o[Q];

@@ -253,8 +253,7 @@ attn_chunk_kernel(AttnArgs a) {
         const AttnCursor c = attn_locate<R, OV>(a, blockIdx.x, gridDim.x);
         if (lane == 0) s_cursor = c;
     }
-    AttnDesc* desc = a.desc + 2 * blockIdx.x;
-    if (threadIdx.x < 2) desc[threadIdx.x].state = kAttnNone;
+    if (threadIdx.x == 0) a.desc[blockIdx.x].parts = 0;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -395,9 +394,7 @@ attn_chunk_kernel(AttnArgs a) {
             const int slot = begin == 0 ? 1 : 0;
             float* part = attn_slot(a, blockIdx.x, slot, R, D);
             if (!whole) {
-                if (threadIdx.x == 0) {
-                    desc[slot] = AttnDesc{begin == 0 ? kAttnFirst : (end == cur.keys ? kAttnLast : kAttnMiddle), cur.tile, cur.head, span.q0, rows};
-                }
+                if (begin == 0 && threadIdx.x == 0) a.desc[blockIdx.x] = attn_describe<OV>(a, cur);
                 part[t * 128 + x] = m;
                 part[R + t * 128 + x] = *gave_up ? __int_as_float(0x7fc00000) : l;
             }
