@@ -199,7 +199,10 @@ struct ChunkShape {
     static constexpr int KV_BYTES = N * D * 2;
     static constexpr int S_COL = 0;                       // tensor memory columns: S buffers, then O
     static constexpr int O_COL = TILES * SBUF * N;
+    static constexpr int STAGES = D == 256 ? 2 : 4;       // FP8: tiles of codes on their way, beside the widened ones
+    static constexpr int STAGE_BYTES = N * D + N * 4;     // codes and row scales
     static constexpr int SMEM = 1024 + TILES * Q_BYTES + 2 * SLOTS * KV_BYTES;
+    static constexpr int SMEM_FP8 = SMEM + STAGES * STAGE_BYTES;
 };
 
 // Steps of a segment [begin, end) of key tiles, the same for every role: whole tiles of N keys, none that lies past the
@@ -231,6 +234,7 @@ attn_chunk_kernel(AttnArgs a) {
     uint8_t* s_base = s_raw + ((1024 - (smem_addr(s_raw) & 1023)) & 1023);
     uint8_t* s_q = s_base;
     uint8_t* s_kv = s_q + TILES * Sh::Q_BYTES;
+    uint8_t* s_stage = s_kv + 2 * SLOTS * Sh::KV_BYTES;   // FP8 only
     volatile int* gave_up = &s_gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4;
@@ -461,75 +465,92 @@ attn_chunk_kernel(AttnArgs a) {
         constexpr int CPR = D * (FP8 ? 1 : 2) / 16;       // 16-byte pieces of a cache row
         constexpr int RPI = 32 / (CPR < 8 ? CPR : 8);     // rows a warp touches at once
         constexpr int LPR = 32 / RPI;                     // lanes per row
+        constexpr int DEPTH = FP8 ? Sh::STAGES : 3;   // tiles on their way
         uint32_t asked[2] = {0, 0};           // K and V tiles so far
-        uint32_t pending = 0, in_flight = 0;  // cp.async: the slots not handed over, four bits each, the oldest on top
-        auto hand_over = [&](uint32_t but) {  // all but the last `but` (0 or 2) of those in flight
-            if (in_flight <= but) return;
-            if (but == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-            else asm volatile("cp.async.wait_group 2;" ::: "memory");
+        uint32_t pending = 0, in_flight = 0;  // the slots not handed over yet, four bits each, the oldest on top
+        uint32_t used_slots[2] = {0, 0}, taken = 0;
+        auto arrived = [&](bool all) {        // the oldest tile on its way (with `all`, every one)
+            if (all) asm volatile("cp.async.wait_group 0;" ::: "memory");
+            else asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+        };
+        auto oldest = [&]() { return pending >> (4 * (in_flight - 1)) & 15; };
+        // bf16: rows go straight into their slot, and are handed over once there
+        auto hand_over = [&](bool all) {
+            if (in_flight == 0) return;
+            arrived(all);
             async_proxy_fence();
-            for (; in_flight > but; --in_flight) mbar_arrive(&full[pending >> (4 * (in_flight - 1)) & 15]);
+            for (; in_flight > (all ? 0u : DEPTH - 1u); --in_flight) mbar_arrive(&full[oldest()]);
+        };
+        // FP8: the oldest staged tile is widened into its slot. A thread reads the codes that it copied itself; the row scales
+        // are the warp's.
+        auto widen = [&](bool all) {
+            arrived(all);
+            __syncwarp();
+            const uint32_t slot = oldest(), which = slot / SLOTS, parity = ((used_slots[which]++ / SLOTS) & 1) ^ 1;
+            const uint8_t* stage = s_stage + taken % Sh::STAGES * Sh::STAGE_BYTES;
+            uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
+            mbar_wait_warp(&empty[slot], parity, gave_up);
+#pragma unroll
+            for (int i = 0; i < ROWS / RPI; ++i) {
+                const int r = w * ROWS + i * RPI + lane / LPR;
+                const float scale = *reinterpret_cast<const float*>(stage + N * D + r * 4);
+#pragma unroll
+                for (int j = 0; j < CPR / LPR; ++j) {
+                    const uint4 code = *reinterpret_cast<const uint4*>(stage + (((i * (CPR / LPR) + j) * 4 + w) * 32 + lane) * 16);
+                    const int ch = 2 * (lane % LPR + j * LPR);
+                    uint4 lo, hi;
+                    e4m3x4_scaled(code.x, scale, lo.x, lo.y);
+                    e4m3x4_scaled(code.y, scale, lo.z, lo.w);
+                    e4m3x4_scaled(code.z, scale, hi.x, hi.y);
+                    e4m3x4_scaled(code.w, scale, hi.z, hi.w);
+                    *reinterpret_cast<uint4*>(tile + tile_offset(r, ch, N)) = lo;
+                    *reinterpret_cast<uint4*>(tile + tile_offset(r, ch + 1, N)) = hi;
+                }
+            }
+            async_proxy_fence();
+            mbar_arrive(&full[slot]);
+            --in_flight, ++taken;
+            __syncwarp();
         };
         // tile `which` (0: K, 1: V) of the step whose cache rows are row32
         auto fetch = [&](int which, int row32) {
-            const uint32_t nth = asked[which]++, slot = which * SLOTS + nth % SLOTS, parity = ((nth / SLOTS) & 1) ^ 1;
-            uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
-            const CacheT* src = static_cast<const CacheT*>(which == 0 ? a.k : a.v);
+            const uint32_t nth = asked[which]++, slot = which * SLOTS + nth % SLOTS;
+            uint8_t* to;
             if (!FP8) {
-                // While its buffer is still being read, the warp lets the rows it has asked for arrive, and hands them
-                // over; otherwise two tiles stay in flight.
+                // While its slot is still being read, the warp lets the rows it has asked for arrive, and hands them over.
+                const uint32_t parity = ((nth / SLOTS) & 1) ^ 1;
                 if (!mbar_try(&empty[slot], parity)) {
-                    hand_over(0);
+                    hand_over(true);
                     mbar_wait(&empty[slot], parity, gave_up);
                 }
                 __syncwarp();
-#pragma unroll
-                for (int i = 0; i < ROWS / RPI; ++i) {
-                    const int r = i * RPI + lane / LPR;
-                    const int row = __shfl_sync(kFullMask, row32, r);
-                    const uint8_t* p = reinterpret_cast<const uint8_t*>(src + ((size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head) * D);
-#pragma unroll
-                    for (int ch = lane % LPR; ch < CPR; ch += LPR) {
-                        const uint32_t dst = smem_addr(tile + tile_offset(w * ROWS + r, ch, N));
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p + 16 * ch), "r"(row < 0 ? 0 : 16) : "memory");
-                    }
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                pending = pending << 4 | slot;
-                if (++in_flight > 2) hand_over(2);
+                to = s_kv + slot * Sh::KV_BYTES;
             } else {
-                const float* by = which == 0 ? a.k_scales : a.v_scales;
-                const float scale32 = row32 < 0 ? 0.0f : by[(size_t)row32 * a.kv_heads + cur.head];
-                uint4 code[ROWS / RPI][CPR / LPR];
-#pragma unroll
-                for (int i = 0; i < ROWS / RPI; ++i) {
-                    const int row = __shfl_sync(kFullMask, row32, i * RPI + lane / LPR);
-                    const uint8_t* p = reinterpret_cast<const uint8_t*>(src + ((size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head) * D);
-#pragma unroll
-                    for (int j = 0; j < CPR / LPR; ++j) {
-                        code[i][j] = row < 0 ? make_uint4(0, 0, 0, 0) : ldg_stream_v4(p + 16 * (lane % LPR + j * LPR));
-                    }
+                if (in_flight == DEPTH) widen(false);
+                to = s_stage + (taken + in_flight) % Sh::STAGES * Sh::STAGE_BYTES;
+                if (lane < ROWS) {
+                    const float* by = (which == 0 ? a.k_scales : a.v_scales) + (size_t)(row32 < 0 ? 0 : row32) * a.kv_heads + cur.head;
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(to + N * D + (w * ROWS + lane) * 4)), "l"(by),
+                                 "r"(row32 < 0 ? 0 : 4) : "memory");
                 }
-                mbar_wait_warp(&empty[slot], parity, gave_up);
-#pragma unroll
-                for (int i = 0; i < ROWS / RPI; ++i) {
-                    const int r = i * RPI + lane / LPR;
-                    const float scale = __shfl_sync(kFullMask, scale32, r);
-#pragma unroll
-                    for (int j = 0; j < CPR / LPR; ++j) {
-                        const int ch = 2 * (lane % LPR + j * LPR);
-                        uint4 lo, hi;
-                        e4m3x4_scaled(code[i][j].x, scale, lo.x, lo.y);
-                        e4m3x4_scaled(code[i][j].y, scale, lo.z, lo.w);
-                        e4m3x4_scaled(code[i][j].z, scale, hi.x, hi.y);
-                        e4m3x4_scaled(code[i][j].w, scale, hi.z, hi.w);
-                        *reinterpret_cast<uint4*>(tile + tile_offset(w * ROWS + r, ch, N)) = lo;
-                        *reinterpret_cast<uint4*>(tile + tile_offset(w * ROWS + r, ch + 1, N)) = hi;
-                    }
-                }
-                async_proxy_fence();
-                mbar_arrive(&full[slot]);
             }
+            const CacheT* src = static_cast<const CacheT*>(which == 0 ? a.k : a.v);
+#pragma unroll
+            for (int i = 0; i < ROWS / RPI; ++i) {
+                const int r = i * RPI + lane / LPR;
+                const int row = __shfl_sync(kFullMask, row32, r);
+                const uint8_t* p = reinterpret_cast<const uint8_t*>(src + ((size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head) * D);
+#pragma unroll
+                for (int j = 0; j < CPR / LPR; ++j) {
+                    const int ch = lane % LPR + j * LPR;
+                    const uint32_t dst = smem_addr(to + (FP8 ? (((i * (CPR / LPR) + j) * 4 + w) * 32 + lane) * 16 : tile_offset(w * ROWS + r, ch, N)));
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p + 16 * ch), "r"(row < 0 ? 0 : 16) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            pending = pending << 4 | slot;
+            ++in_flight;
+            if (!FP8 && in_flight == DEPTH) hand_over(false);
         };
         for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
             int begin, end, keys, from, to;
@@ -557,7 +578,11 @@ attn_chunk_kernel(AttnArgs a) {
                 rows_of[SBUF] = ahead;
             }
         }
-        if (!FP8) hand_over(0);
+        if (!FP8) {
+            hand_over(true);
+        } else {
+            while (in_flight > 0) widen(true);
+        }
     } else {
         if (Sh::SPLIT) set_registers<Sh::MMA_REGS, false>();
         AttnCursor cur = s_cursor;
