@@ -96,13 +96,12 @@ int launch_rows(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const 
 
 template <typename T, bool FP8, int D>
 int launch_chunk(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const AttnPlan& plan, const char* what) {
-    using Sh = ChunkShape<D>;
+    using Sh = ChunkShape<D, FP8>;
     static std::atomic<unsigned long long> allowed{0};
     auto kernel = attn_chunk_kernel<T, FP8, D>;
-    constexpr size_t smem = FP8 ? Sh::SMEM_FP8 : Sh::SMEM;
-    if (int r = allow_smem(kernel, smem, allowed, what)) return r;
+    if (int r = allow_smem(kernel, Sh::SMEM, allowed, what)) return r;
     const size_t most = dev.sms < kAttnMaxCtas / 2 ? dev.sms : kAttnMaxCtas / 2;
-    return launch_units<T, D, Sh::R, true>(kernel, Sh::THREADS, smem, most, s, a, plan, what);
+    return launch_units<T, D, Sh::R, true>(kernel, Sh::THREADS, Sh::SMEM, most, s, a, plan, what);
 }
 
 template <typename T, bool FP8, int D>

@@ -182,7 +182,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-template <int D>
+template <int D, bool FP8>
 struct ChunkShape {
     static constexpr int TILES = D == 256 ? 1 : 2;        // row blocks of 128
     static constexpr int R = 128 * TILES;                 // rows of a row tile
@@ -190,29 +190,32 @@ struct ChunkShape {
     static constexpr int SBUF = 2;                        // S buffers per row block
     static constexpr int SLOTS = D == 256 ? 2 : 4;        // buffers of K tiles, and as many of V tiles
     static constexpr int OV = 2;                          // a row tile's beginning and end cost about two units
-    static constexpr int THREADS = 128 * TILES + 256;     // softmax, producers, products (one thread of a warpgroup)
-    // Registers: 512 threads start with 128 each; the softmax keeps a row of S in registers.
-    static constexpr bool SPLIT = TILES == 2;
-    static constexpr int SOFTMAX_REGS = 184, PRODUCER_REGS = 80, MMA_REGS = 64;
-    static_assert(!SPLIT || 2 * SOFTMAX_REGS + PRODUCER_REGS + MMA_REGS <= 512, "more than the block was launched with");
+    static constexpr int PRODUCERS = FP8 ? 2 : 1;         // warpgroups: one gathers bf16 rows, widening codes takes two
+    static constexpr int THREADS = 128 * (TILES + PRODUCERS + 1);   // softmax, producers, products (one warp of the last)
+    // Registers: the block starts with START for each thread; the softmax, which keeps a row of S, takes what the others leave.
+    static constexpr bool SPLIT = TILES + PRODUCERS > 2;
+    static constexpr int START = THREADS == 640 ? 96 : (THREADS == 512 ? 128 : 168);
+    static constexpr int SOFTMAX_REGS = THREADS == 640 ? 144 : 184, PRODUCER_REGS = THREADS == 640 ? 64 : (TILES == 2 ? 80 : 96);
+    static constexpr int MMA_REGS = 64;
+    static_assert(!SPLIT || TILES * SOFTMAX_REGS + PRODUCERS * PRODUCER_REGS + MMA_REGS <= START * THREADS / 128, "more than the block started with");
     static constexpr int Q_BYTES = 128 * D * 2;
     static constexpr int KV_BYTES = N * D * 2;
     static constexpr int S_COL = 0;                       // tensor memory columns: S buffers, then O
     static constexpr int O_COL = TILES * SBUF * N;
     static constexpr int STAGES = D == 256 ? 2 : 4;       // FP8: tiles of codes on their way, beside the widened ones
     static constexpr int STAGE_BYTES = N * D + N * 4;     // codes and row scales
-    static constexpr int SMEM = 1024 + TILES * Q_BYTES + 2 * SLOTS * KV_BYTES;
-    static constexpr int SMEM_FP8 = SMEM + STAGES * STAGE_BYTES;
+    static constexpr int SMEM = 1024 + TILES * Q_BYTES + 2 * SLOTS * KV_BYTES + (FP8 ? STAGES * STAGE_BYTES : 0);
 };
 
 // Steps of a segment [begin, end) of key tiles, the same for every role: whole tiles of N keys, none that lies past the
 // last key a row of the tile sees, one at least.
-template <int D>
+template <int D, bool FP8>
 __device__ __forceinline__ void chunk_steps(const AttnArgs& a, const AttnCursor& c, int begin, int end, int& keys, int& from, int& to) {
-    constexpr int PER = kAttnKeys / ChunkShape<D>::N;
-    keys = attn_visible(a, c.span, min((c.tile + 1) * ChunkShape<D>::R, c.span.n * a.group));
+    using Sh = ChunkShape<D, FP8>;
+    constexpr int PER = kAttnKeys / Sh::N;
+    keys = attn_visible(a, c.span, min((c.tile + 1) * Sh::R, c.span.n * a.group));
     from = begin * PER;
-    to = max(from + 1, min(end * PER, (keys + ChunkShape<D>::N - 1) / ChunkShape<D>::N));
+    to = max(from + 1, min(end * PER, (keys + Sh::N - 1) / Sh::N));
 }
 
 // The 128 threads of row block t.
@@ -222,9 +225,9 @@ __device__ __forceinline__ void block_barrier(int t) {
 }
 
 template <typename T, bool FP8, int D>
-__global__ void __launch_bounds__(ChunkShape<D>::THREADS, 1)
+__global__ void __launch_bounds__(ChunkShape<D, FP8>::THREADS, 1)
 attn_chunk_kernel(AttnArgs a) {
-    using Sh = ChunkShape<D>;
+    using Sh = ChunkShape<D, FP8>;
     constexpr int TILES = Sh::TILES, R = Sh::R, N = Sh::N, SBUF = Sh::SBUF, SLOTS = Sh::SLOTS, OV = Sh::OV;
     extern __shared__ uint8_t s_raw[];
     __shared__ uint64_t full[2 * SLOTS], empty[2 * SLOTS], q_ready[TILES], s_ready[TILES * SBUF], p_ready[TILES * SBUF], pv_done[TILES * 2], drained;
@@ -237,9 +240,9 @@ attn_chunk_kernel(AttnArgs a) {
     uint8_t* s_stage = s_kv + 2 * SLOTS * Sh::KV_BYTES;   // FP8 only
     volatile int* gave_up = &s_gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4;
+    constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4 * Sh::PRODUCERS;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2 * SLOTS; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
+        for (int i = 0; i < 2 * SLOTS; ++i) mbar_init(&full[i], 128 * Sh::PRODUCERS), mbar_init(&empty[i], 1);
         for (int i = 0; i < TILES; ++i) mbar_init(&q_ready[i], 128);
         for (int i = 0; i < TILES * SBUF; ++i) mbar_init(&s_ready[i], 1), mbar_init(&p_ready[i], 128);
         for (int i = 0; i < TILES * 2; ++i) mbar_init(&pv_done[i], 1);
@@ -288,7 +291,7 @@ attn_chunk_kernel(AttnArgs a) {
             const int rows = span.n * a.group, row0 = cur.tile * R + t * 128;
             if (begin == end || row0 >= rows) continue;
             int keys, from, to;
-            chunk_steps<D>(a, cur, begin, end, keys, from, to);
+            chunk_steps<D, FP8>(a, cur, begin, end, keys, from, to);
             // q: 16-byte chunks, eight lanes to a 128-byte line, rounded to bf16, into the swizzled tile; eight requests in
             // flight (rows past the last repeat it, and are stored as zeros)
 #pragma unroll 1
@@ -456,8 +459,8 @@ attn_chunk_kernel(AttnArgs a) {
             tc_fence_before();
         }
     } else if (warp < kMmaWarp) {
-        // ---- producers: a warp gathers N / 4 rows of each tile, lane l of it knows row l's place ----------------
-        constexpr int ROWS = N / 4;                       // rows per warp
+        // ---- producers: a warp gathers ROWS rows of each tile, lane l of it knows row l's place -----------------
+        constexpr int WARPS = 4 * Sh::PRODUCERS, ROWS = N / WARPS;
         if (Sh::SPLIT) set_registers<Sh::PRODUCER_REGS, false>();
         AttnCursor cur = s_cursor;
         const int w = warp - kProducerWarp;
@@ -496,7 +499,7 @@ attn_chunk_kernel(AttnArgs a) {
                 const float scale = *reinterpret_cast<const float*>(stage + N * D + r * 4);
 #pragma unroll
                 for (int j = 0; j < CPR / LPR; ++j) {
-                    const uint4 code = *reinterpret_cast<const uint4*>(stage + (((i * (CPR / LPR) + j) * 4 + w) * 32 + lane) * 16);
+                    const uint4 code = *reinterpret_cast<const uint4*>(stage + (((i * (CPR / LPR) + j) * WARPS + w) * 32 + lane) * 16);
                     const int ch = 2 * (lane % LPR + j * LPR);
                     uint4 lo, hi;
                     e4m3x4_scaled(code.x, scale, lo.x, lo.y);
@@ -543,7 +546,7 @@ attn_chunk_kernel(AttnArgs a) {
 #pragma unroll
                 for (int j = 0; j < CPR / LPR; ++j) {
                     const int ch = lane % LPR + j * LPR;
-                    const uint32_t dst = smem_addr(to + (FP8 ? (((i * (CPR / LPR) + j) * 4 + w) * 32 + lane) * 16 : tile_offset(w * ROWS + r, ch, N)));
+                    const uint32_t dst = smem_addr(to + (FP8 ? (((i * (CPR / LPR) + j) * WARPS + w) * 32 + lane) * 16 : tile_offset(w * ROWS + r, ch, N)));
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p + 16 * ch), "r"(row < 0 ? 0 : 16) : "memory");
                 }
             }
@@ -556,7 +559,7 @@ attn_chunk_kernel(AttnArgs a) {
             int begin, end, keys, from, to;
             attn_segment<OV>(a, cur, begin, end);
             if (begin == end) continue;
-            chunk_steps<D>(a, cur, begin, end, keys, from, to);
+            chunk_steps<D, FP8>(a, cur, begin, end, keys, from, to);
             auto lookup = [&](int step) {
                 const int key = step * N + w * ROWS + (lane % ROWS);
                 return step < to && key < keys ? attn_cache_row(a, cur.seq, key) : -1;
@@ -619,7 +622,7 @@ attn_chunk_kernel(AttnArgs a) {
             int begin, end, keys, from, to;
             attn_segment<OV>(a, cur, begin, end);
             if (uniform(begin == end)) continue;
-            chunk_steps<D>(a, cur, begin, end, keys, from, to);
+            chunk_steps<D, FP8>(a, cur, begin, end, keys, from, to);
             const int blocks = uniform(cur.span.n * a.group - cur.tile * R > 128 ? TILES : 1);
             const int count = uniform(to - from);
 #pragma unroll
