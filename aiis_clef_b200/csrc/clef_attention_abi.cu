@@ -64,15 +64,17 @@ void launch_pdl(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t
     (void)cudaLaunchKernelEx(&cfg, kernel, args...);   // errors surface in check_launch
 }
 
-// Launches `kernel` on the list of units, and the joining kernel where a row tile may have been cut.
-template <typename T, int D, int R, bool CHUNK, typename K>
-int launch_units(K kernel, unsigned threads, size_t smem, size_t most, cudaStream_t s, const AttnArgs& a, const AttnPlan& plan,
+// Launches `kernel` on the row tiles, and the joining kernel where one may have been cut. Up to WHOLE key tiles a row tile
+// is left to one CTA: a join costs a launch and some 5 us, about what the key tiles cost one after the other.
+template <typename T, int D, int R, bool CHUNK, int WHOLE, typename K>
+int launch_units(K kernel, unsigned threads, size_t smem, size_t most, cudaStream_t s, AttnArgs a, const AttnPlan& plan,
                  const char* what) {
     const size_t key_tiles = ((size_t)a.table_width * a.page_size + kAttnKeys - 1) / kAttnKeys;
-    const unsigned ctas = clamp_grid(plan.items * key_tiles, most);
+    a.whole = key_tiles <= WHOLE;
+    const unsigned ctas = clamp_grid(a.whole ? plan.items : plan.items * key_tiles, most);
     launch_pdl(kernel, dim3(ctas, 1, 1), threads, smem, s, a);
     if (int r = check_launch(what)) return r;
-    if (key_tiles <= 1 || ctas <= 1) return CLEF_OK;
+    if (a.whole || ctas <= 1) return CLEF_OK;
     // a run of 32 possible beginnings at most, fewer where more row tiles may begin
     const unsigned runs = clamp_grid(plan.items > (ctas + 31) / 32 ? plan.items : (ctas + 31) / 32, ctas);
     if constexpr (CHUNK) launch_pdl(attn_combine_rows_kernel<T, D, R>, dim3(runs, R / 32, 1), 256, 0, s, a, (int)ctas);
@@ -91,7 +93,7 @@ int launch_rows(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const 
     if (int r = allow_smem(kernel, smem, allowed, what)) return r;
     size_t most = (size_t)dev.sms * ctas_per_sm(kernel, smem, occ);
     if (most > kAttnMaxCtas) most = kAttnMaxCtas;
-    return launch_units<T, D, R, false>(kernel, kAttnThreads, smem, most, s, a, plan, what);
+    return launch_units<T, D, R, false, 8>(kernel, kAttnThreads, smem, most, s, a, plan, what);
 }
 
 template <typename T, bool FP8, int D>
@@ -101,7 +103,7 @@ int launch_chunk(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const
     auto kernel = attn_chunk_kernel<T, FP8, D>;
     if (int r = allow_smem(kernel, Sh::SMEM, allowed, what)) return r;
     const size_t most = dev.sms < kAttnMaxCtas / 2 ? dev.sms : kAttnMaxCtas / 2;
-    return launch_units<T, D, Sh::R, true>(kernel, Sh::THREADS, Sh::SMEM, most, s, a, plan, what);
+    return launch_units<T, D, Sh::R, true, 4>(kernel, Sh::THREADS, Sh::SMEM, most, s, a, plan, what);
 }
 
 template <typename T, bool FP8, int D>

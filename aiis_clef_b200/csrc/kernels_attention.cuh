@@ -38,6 +38,7 @@ struct AttnArgs {
     int page_size, table_width, cache_pages;
     FastDiv group_div, page_div;
     float scale_log2;           // scale * log2(e): the softmax runs on exp2
+    int whole;                  // row tiles are not cut: all cost the same, nothing is left to join
     struct AttnDesc* desc;      // workspace: what is in slot 1 of each CTA
     float* part;                // workspace: per slot R maxima, R sums, R x head_dim outputs (attn_chunk_kernel: [head_dim / 4][R][4])
 };
@@ -82,15 +83,18 @@ __device__ __forceinline__ int attn_key_tiles(const AttnArgs& a, const AttnSeq& 
 // Work is shared out by a cost that is linear in the row tile's number, so that sums over row tiles need no loop and no
 // division: a row tile of a sequence with kv - n cached keys before its new ones costs
 //   OV * unit + max(0, (kv - n) * group + (tile + 1) R)      with unit = group * kAttnKeys the cost of a key tile,
-// which is `group` times the keys its last row sees, and OV key tiles' worth for its beginning and end.
+// which is `group` times the keys its last row sees, and OV key tiles' worth for its beginning and end. (Where sequences
+// are short, a.whole: every row tile costs 1 and shares are whole numbers of them.)
 template <int R, int OV>
 __device__ __forceinline__ long long attn_tile_cost(const AttnArgs& a, const AttnSeq& q, int tile) {
+    if (a.whole) return 1;
     return (long long)OV * a.group * kAttnKeys + max(0, (q.kv - q.n) * a.group + (tile + 1) * R);
 }
 // Cost of all row tiles of one (sequence, kv head).
 template <int R, int OV>
 __device__ __forceinline__ long long attn_seq_cost(const AttnArgs& a, const AttnSeq& q) {
     const int tiles = (q.n * a.group + R - 1) / R;
+    if (a.whole) return tiles;
     const int ahead = (q.kv - q.n) * a.group;
     const int none = ahead >= 0 ? 0 : min(tiles, -ahead / R);   // row tiles whose linear part is 0
     const long long some = tiles - none;
@@ -118,7 +122,7 @@ __device__ inline AttnCursor attn_locate(const AttnArgs& a, int cta, int ctas) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(kFullMask, total, off);
     // equal shares, but of a key tile at least: the CTAs that work are the first ones
-    c.share = max((total + ctas - 1) / ctas, (long long)a.group * kAttnKeys);
+    c.share = max((total + ctas - 1) / ctas, a.whole ? 1ll : (long long)a.group * kAttnKeys);
     long long at = cta * c.share;
     c.left = min(c.share, total - at);
     if (c.left <= 0) return c;

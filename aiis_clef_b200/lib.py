@@ -12,6 +12,7 @@ torch is used for device memory and streams only.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -128,11 +129,12 @@ def _check(status: int, what: str):
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current stream of the current device, as the address the C ABI takes."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -185,6 +187,7 @@ def set_scale_layout(layout: int) -> None:
     _check(load().clef_set_scale_layout(int(layout)), "clef_set_scale_layout")
 
 
+@functools.lru_cache(maxsize=1024)
 def paged_attention_workspace(n_seqs: int, total_q: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
     """Bytes of workspace a paged_attention_dev call of these shapes needs."""
     n = _SZ(0)
@@ -203,12 +206,25 @@ class Device:
     def __init__(self, device: int | str | torch.device = 0):
         self.device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
         self.lib = load()
+        self._index = self.device.index or 0
         if not torch.cuda.is_available():
             raise ClefError("no CUDA device: the fused kernels run on a B200 only")
 
     # -- helpers ------------------------------------------------------------------------------
     def _empty(self, shape, dtype):
         return torch.empty(shape, dtype=dtype, device=self.device)
+
+    def _call(self, name: str, *args):
+        """One entry point on this device's current stream; the device is switched to only if it is not the current one."""
+        fn = getattr(self.lib, name)
+        if torch._C._cuda_getDevice() == self._index:
+            return _check(fn(torch._C._cuda_getCurrentRawStream(self._index), *args), name)
+        with torch.cuda.device(self.device):
+            return _check(fn(torch._C._cuda_getCurrentRawStream(self._index), *args), name)
+
+    def _like(self, t, shape, dtype):
+        """An uninitialised output of `shape`: torch makes one in the shape of an input in half the time."""
+        return torch.empty_like(t, dtype=dtype) if t.shape == shape else self._empty(shape, dtype)
 
     def _quant_outputs(self, rows: int, cols: int, tile_m: int):
         blk_mn, chunk = sf_atom_for_tile_m(tile_m)
@@ -502,13 +518,11 @@ class Device:
         elif _dev_tensor(out, "out").dtype != q.dtype or out.numel() != q.numel():
             raise ClefError("out must have the type and the size of q")
         if workspace is None:
-            workspace = self._empty((paged_attention_workspace(n_seqs, total_q, q_heads, kv_heads, head_dim),), torch.uint8)
-        with torch.cuda.device(self.device):
-            _check(self.lib.clef_paged_attention(
-                _stream(), _ptr(out), _ptr(q), _ptr(cache_k), _ptr(cache_v), _ptr(k_scales), _ptr(v_scales),
-                _ptr(page_table), _ptr(q_start), _ptr(kv_len), n_seqs, total_q, q_heads, kv_heads, head_dim, page_size,
-                page_table.shape[1], cache_rows // page_size, scale, _ptr(workspace), workspace.numel(),
-                CLEF_E4M3 if fp8 else CLEF_BF16, _dtype_code(q)), "clef_paged_attention")
+            workspace = q.new_empty((paged_attention_workspace(n_seqs, total_q, q_heads, kv_heads, head_dim),), dtype=torch.uint8)
+        self._call("clef_paged_attention", out.data_ptr(), q.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), _ptr(k_scales),
+                   _ptr(v_scales), page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), n_seqs, total_q, q_heads, kv_heads,
+                   head_dim, page_size, page_table.shape[1], cache_rows // page_size, scale, workspace.data_ptr(),
+                   workspace.numel(), CLEF_E4M3 if fp8 else CLEF_BF16, _dtype_code(q))
         return out
 
     # ==== the FP8 (E4M3) KV cache ================================================================
@@ -532,11 +546,9 @@ class Device:
         """rope_apply_dev on k, then k and v into the FP8 caches and their scales (in place), one launch."""
         _dev_tensor(k, "k"), _dev_tensor(v, "v")
         rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
-        with torch.cuda.device(self.device):
-            _check(self.lib.clef_rope_kv_write_fp8(
-                _stream(), _ptr(cache_k), _ptr(cache_v), _ptr(k_scales), _ptr(v_scales), _ptr(k), _ptr(v), _ptr(cos), _ptr(sin),
-                tokens, kv_heads, head_dim, rotary_dim, _ptr(seq_start), _ptr(pos_base), _ptr(pos_map), _ptr(cache_map),
-                _ptr(cache_len), rows, _dtype_code(k)), "clef_rope_kv_write_fp8")
+        self._call("clef_rope_kv_write_fp8", cache_k.data_ptr(), cache_v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                   k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), tokens, kv_heads, head_dim, rotary_dim,
+                   _ptr(seq_start), _ptr(pos_base), _ptr(pos_map), _ptr(cache_map), _ptr(cache_len), rows, _dtype_code(k))
 
     def rope_qkv_write_fp8_dev(self, q, cache_k, cache_v, k_scales, v_scales, k, v, cos, sin, tokens: int, q_heads: int,
                                kv_heads: int, head_dim: int, rotary_dim: int, seq_start=None, pos_base=None, pos_map=None,
@@ -544,12 +556,11 @@ class Device:
         """rope_apply_dev on q (returned) and rope_kv_write_fp8_dev on k, v (caches written in place), one launch."""
         _dev_tensor(q, "q"), _dev_tensor(k, "k"), _dev_tensor(v, "v")
         rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
-        q_out = self._empty((tokens, q_heads, head_dim), q.dtype)
-        with torch.cuda.device(self.device):
-            _check(self.lib.clef_rope_qkv_write_fp8(
-                _stream(), _ptr(q_out), _ptr(q), q_heads, _ptr(cache_k), _ptr(cache_v), _ptr(k_scales), _ptr(v_scales), _ptr(k),
-                _ptr(v), kv_heads, _ptr(cos), _ptr(sin), tokens, head_dim, rotary_dim, _ptr(seq_start), _ptr(pos_base),
-                _ptr(pos_map), _ptr(cache_map), _ptr(cache_len), rows, _dtype_code(q)), "clef_rope_qkv_write_fp8")
+        q_out = self._like(q, (tokens, q_heads, head_dim), q.dtype)
+        self._call("clef_rope_qkv_write_fp8", q_out.data_ptr(), q.data_ptr(), q_heads, cache_k.data_ptr(), cache_v.data_ptr(),
+                   k_scales.data_ptr(), v_scales.data_ptr(), k.data_ptr(), v.data_ptr(), kv_heads, cos.data_ptr(), sin.data_ptr(),
+                   tokens, head_dim, rotary_dim, _ptr(seq_start), _ptr(pos_base), _ptr(pos_map), _ptr(cache_map),
+                   _ptr(cache_len), rows, _dtype_code(q))
         return q_out
 
     def qk_norm_rope_kv_write_fp8_dev(self, cache_k, cache_v, k_scales, v_scales, k_raw, v, weight, cos, sin, tokens: int,
@@ -558,21 +569,19 @@ class Device:
         """qk_norm_rope_dev on k_raw, then k and v into the FP8 caches and their scales (in place), one launch."""
         _dev_tensor(k_raw, "k_raw"), _dev_tensor(v, "v")
         rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
-        with torch.cuda.device(self.device):
-            _check(self.lib.clef_qk_norm_rope_kv_write_fp8(
-                _stream(), _ptr(cache_k), _ptr(cache_v), _ptr(k_scales), _ptr(v_scales), _ptr(k_raw), _ptr(v), _ptr(weight),
-                _ptr(cos), _ptr(sin), tokens, kv_heads, head_dim, rotary_dim, eps, _ptr(seq_start), _ptr(pos_base),
-                _ptr(pos_map), _ptr(cache_map), _ptr(cache_len), rows, _dtype_code(k_raw)), "clef_qk_norm_rope_kv_write_fp8")
+        self._call("clef_qk_norm_rope_kv_write_fp8", cache_k.data_ptr(), cache_v.data_ptr(), k_scales.data_ptr(),
+                   v_scales.data_ptr(), k_raw.data_ptr(), v.data_ptr(), weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), tokens,
+                   kv_heads, head_dim, rotary_dim, eps, _ptr(seq_start), _ptr(pos_base), _ptr(pos_map), _ptr(cache_map),
+                   _ptr(cache_len), rows, _dtype_code(k_raw))
 
     def kv_read_fp8_dev(self, cache_k, cache_v, k_scales, v_scales, rows: int, kv_heads: int, head_dim: int, row_map=None,
                         dtype=torch.bfloat16):
         """(k, v) [rows, kv_heads, head_dim] of `dtype`: the cache rows row_map (0 .. rows - 1 without a map) read back."""
         cache_rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
-        k, v = self._empty((rows, kv_heads, head_dim), dtype), self._empty((rows, kv_heads, head_dim), dtype)
-        with torch.cuda.device(self.device):
-            _check(self.lib.clef_kv_read_fp8(_stream(), _ptr(k), _ptr(v), _ptr(cache_k), _ptr(cache_v), _ptr(k_scales),
-                                             _ptr(v_scales), _ptr(row_map), rows, cache_rows, kv_heads, head_dim,
-                                             _dtype_code(k)), "clef_kv_read_fp8")
+        k = self._empty((rows, kv_heads, head_dim), dtype)
+        v = torch.empty_like(k)
+        self._call("clef_kv_read_fp8", k.data_ptr(), v.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), k_scales.data_ptr(),
+                   v_scales.data_ptr(), _ptr(row_map), rows, cache_rows, kv_heads, head_dim, _dtype_code(k))
         return k, v
 
     # ==== FP8 (E4M3) activation quantisers ======================================================
@@ -610,14 +619,12 @@ class Device:
         """add_dev followed by rms_norm_fp8_bf16_dev on the stored sum, one pass; returns (sum, codes, row scales, bf16
         copy)."""
         _dev_tensor(a, "a"), _dev_tensor(b, "b")
+        shape = (rows, cols)
         if sum_out is None:
-            sum_out = self._empty((rows, cols), a.dtype)
-        q, qs = self._empty((rows, cols), torch.uint8), self._empty((rows,), torch.int16)
-        bf = self._empty((rows, cols), torch.bfloat16)
-        with torch.cuda.device(self.device):
-            _check(self.lib.clef_add_rms_norm_fp8_bf16(_stream(), _ptr(sum_out), _ptr(a), _ptr(b), _ptr(weight), _ptr(q),
-                                                       _ptr(qs), _ptr(bf), rows, cols, eps, _dtype_code(a)),
-                   "clef_add_rms_norm_fp8_bf16")
+            sum_out = self._like(a, shape, a.dtype)
+        q, qs, bf = self._like(a, shape, torch.uint8), a.new_empty((rows,), dtype=torch.int16), self._like(a, shape, torch.bfloat16)
+        self._call("clef_add_rms_norm_fp8_bf16", sum_out.data_ptr(), a.data_ptr(), b.data_ptr(), weight.data_ptr(), q.data_ptr(),
+                   qs.data_ptr(), bf.data_ptr(), rows, cols, eps, _dtype_code(a))
         return sum_out, q, qs, bf
 
     # -- src/cuda/mod.rs:2304-2328 ------------------------------------------------------------
