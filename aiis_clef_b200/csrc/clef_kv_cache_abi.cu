@@ -14,14 +14,24 @@ using namespace clef::abi;
 
 namespace {
 
+template <typename T, int G, bool NORM, int U>
+void launch_kv_write_u(cudaStream_t s, const DeviceInfo& dev, KvWriteArgs a) {
+    static std::atomic<int> occ{0};
+    auto kernel = kv_write_fp8_kernel<T, G, NORM, U>;
+    const int per_sm = ctas_per_sm(kernel, 0, occ);
+    const int rows = a.q_heads + 2 * a.kv_heads, per_warp = U * (32 / G);
+    a.parts_div = make_fast_div((uint32_t)((rows + per_warp - 1) / per_warp));
+    const size_t units = (size_t)a.tokens * a.parts_div.d;
+    launch_hot(kernel, balanced_grid((units + kCtaThreads / 32 - 1) / (kCtaThreads / 32), (size_t)dev.sms * per_sm), 0, s, a);
+}
+
+// Five groups of head rows per warp (20 head rows of 128, 16 q, 2 k and 2 v, are two warps' work) where that still gives
+// every SM a full set of warps, one where it does not.
 template <typename T, int G, bool NORM>
 void launch_kv_write(cudaStream_t s, const DeviceInfo& dev, const KvWriteArgs& a) {
-    static std::atomic<int> occ{0};
-    auto kernel = kv_write_fp8_kernel<T, G, NORM>;
-    const int per_sm = ctas_per_sm(kernel, 0, occ);
-    const size_t per_cta = (size_t)(kCtaThreads / 32) * (32 / G);
-    const size_t rows = (size_t)a.tokens * a.heads_div.d;
-    launch_hot(kernel, balanced_grid((rows + per_cta - 1) / per_cta, (size_t)dev.sms * per_sm), 0, s, a);
+    const size_t groups = (size_t)a.tokens * (a.q_heads + 2 * a.kv_heads) / (32 / G);
+    if (groups >= (size_t)dev.sms * 16 * 5) launch_kv_write_u<T, G, NORM, 5>(s, dev, a);
+    else launch_kv_write_u<T, G, NORM, 1>(s, dev, a);
 }
 
 template <typename T, bool NORM>
@@ -58,7 +68,6 @@ int kv_write_impl(const char* what, clef_stream_t stream, KvWriteArgs a, bool wi
     if (a.tokens == 0) return CLEF_OK;
     DeviceInfo dev;
     if (int r = device_info(dev)) return r;
-    a.heads_div = make_fast_div((uint32_t)per_token);
     cudaStream_t s = as_stream(stream);
     if (dtype == CLEF_BF16) {
         if (norm) launch_kv_write_for<Bf16, true>(s, dev, a);
@@ -130,16 +139,20 @@ int clef_kv_read_fp8(clef_stream_t stream, void* k_out, void* v_out, const uint8
     DeviceInfo dev;
     if (int r = device_info(dev)) return r;
     cudaStream_t s = as_stream(stream);
-    const size_t pieces = (size_t)head_rows * (head_dim / 8);
-    const FastDiv piece_div = make_fast_div((uint32_t)(head_dim / 8)), heads_div = make_fast_div((uint32_t)kv_heads);
-    auto launch = [&](auto kernel, std::atomic<int>& occ, auto* k, auto* v) {
-        const int per_sm = ctas_per_sm(kernel, 0, occ);
-        launch_hot(kernel, balanced_grid((2 * pieces + kCtaThreads - 1) / kCtaThreads, (size_t)dev.sms * per_sm), 0, s, k, v, cache_k,
-                   cache_v, k_scales, v_scales, (const int*)row_map, pieces, cache_rows, kv_heads, piece_div, heads_div);
+    auto launch = [&](auto kernel, int codes, auto* k, auto* v) {
+        const size_t pieces = (size_t)head_rows * (head_dim / codes);
+        launch_hot(kernel, (unsigned)((pieces + kCtaThreads - 1) / kCtaThreads), 0, s, k, v, cache_k, cache_v, k_scales, v_scales,
+                   (const int*)row_map, (uint32_t)pieces, cache_rows, kv_heads, make_fast_div((uint32_t)(kv_heads * (head_dim / codes))),
+                   make_fast_div((uint32_t)(head_dim / codes)));
     };
-    static std::atomic<int> occ[2];
-    if (dtype == CLEF_BF16) launch(kv_read_fp8_kernel<Bf16>, occ[0], (uint16_t*)k_out, (uint16_t*)v_out);
-    else launch(kv_read_fp8_kernel<F32>, occ[1], (float*)k_out, (float*)v_out);
+    const bool wide = head_dim % 16 == 0 && aligned(cache_k, 16) && aligned(cache_v, 16) && aligned(k_out, 32) && aligned(v_out, 32);
+    if (dtype == CLEF_BF16) {
+        if (wide) launch(kv_read_fp8_kernel<Bf16, 16>, 16, (uint16_t*)k_out, (uint16_t*)v_out);
+        else launch(kv_read_fp8_kernel<Bf16, 8>, 8, (uint16_t*)k_out, (uint16_t*)v_out);
+    } else {
+        if (wide) launch(kv_read_fp8_kernel<F32, 16>, 16, (float*)k_out, (float*)v_out);
+        else launch(kv_read_fp8_kernel<F32, 8>, 8, (float*)k_out, (float*)v_out);
+    }
     return check_launch(what);
 }
 

@@ -305,67 +305,7 @@ attn_rows_kernel(AttnArgs a) {
         if (begin == end) continue;
         const AttnSeq span = cur.span;
         const int row0 = cur.tile * R, rows = span.n * a.group;
-        // q of this lane's row r (and r + 8): the columns that meet its K columns
-        uint32_t qf[NT][D / 16][2];
-        int lim[NT][2];     // keys seen by rows 2c and 2c + 1 of each 8
-        float back[NT][2];  // FP8: score scale of those rows
-        float v_most = 0.0f;   // FP8: a power of two no value scale so far is above; o is that much too small
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int x = row0 + nt * 8 + r;
-            const int token = (int)fast_div((uint32_t)x, a.group_div);
-            const size_t at = ((size_t)(span.q0 + token) * a.q_heads + cur.head * a.group + (x - token * a.group)) * D;
-            const typename T::storage* qr = static_cast<const typename T::storage*>(a.q) + at;
-            float4 f[D / 16];
-            float most = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                // bf16: 8 columns (two steps) at 32 (i / 2) + 8 c; FP8: 16 columns (four steps) at 64 (i / 4) + 16 c
-                const int col = FP8 ? 64 * (i >> 2) + 16 * c + 4 * (i & 3) : 32 * (i >> 1) + 8 * c + 4 * (i & 1);
-                f[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (x < rows) f[i] = load_quad<T>(qr + col, 0);
-                if (FP8) most = fmaxf(fmaxf(fmaxf(most, fabsf(f[i].x)), fmaxf(fabsf(f[i].y), fabsf(f[i].z))), fabsf(f[i].w));
-            }
-            if (FP8) {
-                most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
-                // the power of two below it, kept where it and its reciprocal are normal numbers
-                const int exponent = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100);
-                const float down = __uint_as_float((uint32_t)(127 - exponent) << 23), up = __uint_as_float((uint32_t)(127 + exponent) << 23);
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    qf[nt][i][0] = pack_f16x2(f[i].x * down, f[i].y * down);
-                    qf[nt][i][1] = pack_f16x2(f[i].z * down, f[i].w * down);
-                }
-                // row r's factor to the lanes whose columns of S^T are rows 2c and 2c + 1
-                back[nt][0] = a.scale_log2 * __shfl_sync(kFullMask, up, 8 * c);
-                back[nt][1] = a.scale_log2 * __shfl_sync(kFullMask, up, 8 * c + 4);
-            } else {
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    qf[nt][i][0] = pack_bf16x2(f[i].x, f[i].y);
-                    qf[nt][i][1] = pack_bf16x2(f[i].z, f[i].w);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int y = row0 + nt * 8 + 2 * c + e;
-                lim[nt][e] = y < rows ? attn_visible(a, span, y + 1) : 0;
-            }
-        }
         const int keys = attn_visible(a, span, min(row0 + R, rows));   // seen by any row of the tile
-        float o[NT][VL][VCH / 2][4];
-        float m[NT][2], l[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int b = 0; b < VL; ++b) {
-#pragma unroll
-                for (int i = 0; i < VCH / 2; ++i) o[nt][b][i][0] = o[nt][b][i][1] = o[nt][b][i][2] = o[nt][b][i][3] = 0.0f;
-            }
-            m[nt][0] = m[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.0f;
-        }
         uint4 kr[2][KL];
         uint32_t vr[4][VL][VW];
         float ks[2], vs[2];
@@ -402,10 +342,71 @@ attn_rows_kernel(AttnArgs a) {
                 }
             }
         };
+        // the first keys are asked for before q, whose way is shorter
         int row16 = lookup(begin);
         load_k(row16);
         load_v(row16);
         row16 = lookup(begin + 1);
+        // q of this lane's row r (and r + 8): the columns that meet its K columns
+        uint32_t qf[NT][D / 16][2];
+        int lim[NT][2];     // keys seen by rows 2c and 2c + 1 of each 8
+        float back[NT][2];  // FP8: score scale of those rows
+        float v_most = 0.0f;   // FP8: a power of two no value scale so far is above; o is that much too small
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int x = row0 + nt * 8 + r;
+            const int token = (int)fast_div((uint32_t)x, a.group_div);
+            const size_t at = ((size_t)(span.q0 + token) * a.q_heads + cur.head * a.group + (x - token * a.group)) * D;
+            const typename T::storage* qr = static_cast<const typename T::storage*>(a.q) + at;
+            float4 f[FP8 ? D / 16 : 1];
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < (FP8 ? D / 16 : 0); ++i) {
+                // 16 columns (four steps) at 64 (i / 4) + 16 c
+                f[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (x < rows) f[i] = load_quad<T>(qr + 64 * (i >> 2) + 16 * c + 4 * (i & 3), 0);
+                most = fmaxf(fmaxf(fmaxf(most, fabsf(f[i].x)), fmaxf(fabsf(f[i].y), fabsf(f[i].z))), fabsf(f[i].w));
+            }
+            if (FP8) {
+                most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
+                // the power of two below it, kept where it and its reciprocal are normal numbers
+                const int exponent = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100);
+                const float down = __uint_as_float((uint32_t)(127 - exponent) << 23), up = __uint_as_float((uint32_t)(127 + exponent) << 23);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    qf[nt][i][0] = pack_f16x2(f[i].x * down, f[i].y * down);
+                    qf[nt][i][1] = pack_f16x2(f[i].z * down, f[i].w * down);
+                }
+                // row r's factor to the lanes whose columns of S^T are rows 2c and 2c + 1
+                back[nt][0] = a.scale_log2 * __shfl_sync(kFullMask, up, 8 * c);
+                back[nt][1] = a.scale_log2 * __shfl_sync(kFullMask, up, 8 * c + 4);
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {   // 8 columns (two steps) at 32 (i / 2) + 8 c
+                    const float4 t = x < rows ? load_quad<T>(qr + 32 * (i >> 1) + 8 * c + 4 * (i & 1), 0) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    qf[nt][i][0] = pack_bf16x2(t.x, t.y);
+                    qf[nt][i][1] = pack_bf16x2(t.z, t.w);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int y = row0 + nt * 8 + 2 * c + e;
+                lim[nt][e] = y < rows ? attn_visible(a, span, y + 1) : 0;
+            }
+        }
+        float o[NT][VL][VCH / 2][4];
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int b = 0; b < VL; ++b) {
+#pragma unroll
+                for (int i = 0; i < VCH / 2; ++i) o[nt][b][i][0] = o[nt][b][i][1] = o[nt][b][i][2] = o[nt][b][i][3] = 0.0f;
+            }
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+        }
         for (int tile = begin; tile < end; ++tile) {
             const int t0 = tile * kAttnKeys + warp * 16;
             float s[NT][4];

@@ -6,8 +6,9 @@
 // stored as zero codes with scale NaN, so that whatever reads it sees NaN.
 //
 // Bound by HBM bytes. A head row of head_dim values is a group of G = head_dim / 8 lanes (rounded up to a power of two),
-// 8 values each: 16-byte loads (bf16), and the rotation partner is a second load of a line the group has fetched
-// anyway, which keeps the kernel free of shared memory and of an exchange before the row maximum.
+// 8 values each: 16-byte loads (bf16), the rotation partner and the row maximum by shuffles, no shared memory. A warp
+// takes U groups of head rows of ONE token, requested together: a lane's columns, and with them its cosines and sines,
+// are the same in all of them, and the chain position -> table runs beside the rows' own loads.
 #pragma once
 
 #include "kernels_generic.cuh"
@@ -41,7 +42,7 @@ struct KvWriteArgs {
     const int* cache_len;
     int tokens, kv_heads, head_dim, rotary_dim, cache_rows;
     float eps;
-    FastDiv heads_div;    // q_heads + 2 kv_heads head rows per token
+    FastDiv parts_div;    // warps per token
 };
 
 // Eight scaled values -> eight E4M3 bytes, round to nearest even, saturating.
@@ -72,129 +73,203 @@ __device__ __forceinline__ void store8<F32>(float* p, const float* v) {
     stg_v4(p + 4, make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])));
 }
 
-// G lanes per head row; a warp holds 32 / G head rows. NORM: k rows are normalised first, in the summation order of
-// rms_norm_kernel (kernels/elementwise.cu:4-68: quad i with quad i + 32, then the tree 16, 8, 4, 2, 1 over quads).
-template <typename T, int G, bool NORM>
+// rope_pair's two outputs are one form, a * b + p * q with the product p * q rounded first, of operands that are swapped
+// between a pair's lower and upper element (and q negated for the lower): a lane computes the one that is its own.
+#if CLEF_ROPE_FMA_LO != 1 || CLEF_ROPE_FMA_HI != 2
+#error "kv_write_fp8_kernel spells rope_pair's default contraction"
+#endif
+
+// Eight activations as they are loaded.
+template <typename T>
+struct Raw8 {
+    uint4 w[T::kBytes / 2];
+};
+template <typename T>
+__device__ __forceinline__ void widen8(const Raw8<T>& r, float* v);
+template <>
+__device__ __forceinline__ void widen8<Bf16>(const Raw8<Bf16>& r, float* v) {
+    const uint4 d = r.w[0];
+    v[0] = bf16_lo(d.x), v[1] = bf16_hi(d.x), v[2] = bf16_lo(d.y), v[3] = bf16_hi(d.y);
+    v[4] = bf16_lo(d.z), v[5] = bf16_hi(d.z), v[6] = bf16_lo(d.w), v[7] = bf16_hi(d.w);
+}
+template <>
+__device__ __forceinline__ void widen8<F32>(const Raw8<F32>& r, float* v) {
+    const uint4 a = r.w[0], b = r.w[1];
+    v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
+    v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
+}
+
+// G lanes per head row; a warp holds 32 / G head rows at a time, U of those. NORM: k rows are normalised first, in the
+// summation order of rms_norm_kernel (kernels/elementwise.cu:4-68: quad i with quad i + 32, then the tree 16, 8, 4, 2, 1
+// over quads).
+template <typename T, int G, bool NORM, int U>
 __global__ void __launch_bounds__(kCtaThreads)
 kv_write_fp8_kernel(KvWriteArgs a) {
     constexpr int PER_WARP = 32 / G;
     const int lane = threadIdx.x & 31, sub = lane % G;
     const int col = sub * 8, half = a.rotary_dim >> 1;
-    const bool mine = col < a.head_dim;
-    const uint32_t per_token = a.heads_div.d;
-    const uint32_t rows = (uint32_t)a.tokens * per_token;
-    const uint32_t step = gridDim.x * (kCtaThreads / 32) * PER_WARP;
+    const bool in_row = col < a.head_dim, rotary = col < a.rotary_dim, upper = col >= half;
+    const int partner = rotary ? (upper ? lane - (half >> 3) : lane + (half >> 3)) : lane;
+    const int rows = a.q_heads + 2 * a.kv_heads, parts = (int)a.parts_div.d;
+    const uint32_t units = (uint32_t)a.tokens * parts;
     pdl_launch_dependents();
     pdl_wait_prior_grids();
-    // (the shuffles below need the whole warp: its head rows leave the loop together)
-    for (uint32_t base = (blockIdx.x * (kCtaThreads / 32) + (threadIdx.x >> 5)) * PER_WARP; base < rows; base += step) {
-        const uint32_t row = base + lane / G;
-        const bool live = mine && row < rows;
-        const uint32_t token = fast_div(row < rows ? row : 0u, a.heads_div);
-        const int slot = row < rows ? (int)(row - token * per_token) : 0;
-        const bool is_q = slot < a.q_heads;
-        const int kv_slot = slot - a.q_heads;
-        const bool is_v = kv_slot >= a.kv_heads;
-        const int head = is_q ? slot : (is_v ? kv_slot - a.kv_heads : kv_slot);
-        const typename T::storage* x = static_cast<const typename T::storage*>(is_q ? a.q : (is_v ? a.v : a.k)) +
-                                       ((size_t)token * (is_q ? a.q_heads : a.kv_heads) + head) * a.head_dim;
-        const bool rotates = live && !is_v && col < a.rotary_dim;
-        const bool upper = col >= half;
-        float v[8], other[8];
+    for (uint32_t unit = blockIdx.x * (kCtaThreads / 32) + (threadIdx.x >> 5); unit < units; unit += gridDim.x * (kCtaThreads / 32)) {
+        const int token = (int)fast_div(unit, a.parts_div);
+        const int first = ((int)unit - token * parts) * (U * PER_WARP) + lane / G;
+        Raw8<T> raw[U];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = other[i] = 0.0f;
-        if (live) load8<T>(x + col, v);
-        if (rotates) load8<T>(x + (upper ? col - half : col + half), other);
-        if (NORM) {
-            float s0 = quad_sq(make_float4(v[0], v[1], v[2], v[3])), s1 = quad_sq(make_float4(v[4], v[5], v[6], v[7]));
+        for (int u = 0; u < U; ++u) {
+            const int row = first + u * PER_WARP;
+            const int kv = row - a.q_heads, head = kv < 0 ? row : (kv < a.kv_heads ? kv : kv - a.kv_heads);
+            const typename T::storage* x = static_cast<const typename T::storage*>(kv < 0 ? a.q : (kv < a.kv_heads ? a.k : a.v)) +
+                                           ((size_t)token * (kv < 0 ? a.q_heads : a.kv_heads) + head) * a.head_dim + col;
 #pragma unroll
-            for (int off = G / 2; off > 0; off >>= 1) {
-                s0 = __fadd_rn(s0, __shfl_xor_sync(kFullMask, s0, off));
-                s1 = __fadd_rn(s1, __shfl_xor_sync(kFullMask, s1, off));
-            }
-            if (live && !is_q && !is_v) {
-                const float inv = inv_rms(__fadd_rn(s0, s1), a.head_dim, a.eps);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (1.0f + a.weight[col + i]);
-                if (rotates) {
-                    const float* w = a.weight + (upper ? col - half : col + half);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) other[i] = other[i] * inv * (1.0f + w[i]);
-                }
+            for (int i = 0; i < T::kBytes / 2; ++i) {
+                raw[u].w[i] = in_row && row < rows ? ldg_stream_v4(reinterpret_cast<const uint8_t*>(x) + 16 * i) : make_uint4(0, 0, 0, 0);
             }
         }
-        if (rotates) {
-            const int pos = rope_position((int)token, a.seq_start, a.pos_base, a.pos_map);
+        float b[8], q[8];   // lower: cos, -sin; upper: sin, cos
+        if (rotary) {
+            const int pos = rope_position(token, a.seq_start, a.pos_base, a.pos_map);
             const size_t at = (size_t)pos * a.rotary_dim + (upper ? col - half : col);
-            float c[8], s[8];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                *reinterpret_cast<float4*>(c + 4 * i) = __ldg(reinterpret_cast<const float4*>(a.cos_t + at) + i);
-                *reinterpret_cast<float4*>(s + 4 * i) = __ldg(reinterpret_cast<const float4*>(a.sin_t + at) + i);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float lo, hi;
-                rope_pair(upper ? other[i] : v[i], upper ? v[i] : other[i], c[i], s[i], lo, hi);
-                v[i] = upper ? hi : lo;
+                const float4 c = __ldg(reinterpret_cast<const float4*>(a.cos_t + at) + i), s = __ldg(reinterpret_cast<const float4*>(a.sin_t + at) + i);
+                *reinterpret_cast<float4*>(b + 4 * i) = upper ? s : c;
+                *reinterpret_cast<float4*>(q + 4 * i) = upper ? c : make_float4(-s.x, -s.y, -s.z, -s.w);
             }
         }
-        float amax = 0.0f;
+        const long long place = a.cache_map ? (long long)a.cache_map[token] : (long long)token + (a.cache_len ? a.cache_len[0] : 0);
+        const bool kept = place >= 0 && place < a.cache_rows;   // (a padding token is not)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf_nan(amax, fabsf(v[i]));
+        for (int u = 0; u < U; ++u) {
+            const int row = first + u * PER_WARP;
+            if (row - lane / G >= rows) break;   // (the whole warp)
+            const bool live = in_row && row < rows, is_q = row < a.q_heads, is_v = row >= a.q_heads + a.kv_heads;
+            float v[8];
+            if (NORM) {
+                widen8<T>(raw[u], v);
+                float s0 = quad_sq(make_float4(v[0], v[1], v[2], v[3])), s1 = quad_sq(make_float4(v[4], v[5], v[6], v[7]));
 #pragma unroll
-        for (int off = G / 2; off > 0; off >>= 1) amax = fmaxf_nan(amax, __shfl_xor_sync(kFullMask, amax, off));
-        if (!live) continue;
-        if (is_q) {
-            store8<T>(static_cast<typename T::storage*>(a.q_out) + ((size_t)token * a.q_heads + head) * a.head_dim + col, v);
-            continue;
+                for (int off = G / 2; off > 0; off >>= 1) {
+                    s0 = __fadd_rn(s0, __shfl_xor_sync(kFullMask, s0, off));
+                    s1 = __fadd_rn(s1, __shfl_xor_sync(kFullMask, s1, off));
+                }
+                if (live && !is_q && !is_v) {
+                    const float inv = inv_rms(__fadd_rn(s0, s1), a.head_dim, a.eps);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (1.0f + a.weight[col + i]);
+                }
+            }
+            const bool turns = rotary && !is_v;
+            if (__any_sync(kFullMask, turns)) {
+                float x[8], y[8];   // the element of the lower half and that of the upper, or the other way round
+                if (NORM) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float other = __shfl_sync(kFullMask, v[i], partner);
+                        x[i] = upper ? other : v[i], y[i] = upper ? v[i] : other;
+                    }
+                } else {
+                    Raw8<T> rx, ry;
+#pragma unroll
+                    for (int i = 0; i < T::kBytes / 2; ++i) {
+                        const uint4 o = make_uint4(__shfl_sync(kFullMask, raw[u].w[i].x, partner), __shfl_sync(kFullMask, raw[u].w[i].y, partner),
+                                                   __shfl_sync(kFullMask, raw[u].w[i].z, partner), __shfl_sync(kFullMask, raw[u].w[i].w, partner));
+                        rx.w[i] = upper ? o : raw[u].w[i], ry.w[i] = upper ? raw[u].w[i] : o;
+                    }
+                    widen8<T>(rx, x);
+                    widen8<T>(ry, y);
+                }
+                if (turns) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const f32x2 r = f2_fma(f2_pack(x[i], x[i + 1]), f2_pack(b[i], b[i + 1]), f2_mul(f2_pack(y[i], y[i + 1]), f2_pack(q[i], q[i + 1])));
+                        v[i] = r.x, v[i + 1] = r.y;
+                    }
+                } else if (!NORM) {
+                    widen8<T>(raw[u], v);
+                }
+            } else if (!NORM) {
+                widen8<T>(raw[u], v);
+            }
+            float amax = 0.0f;
+            if (__any_sync(kFullMask, !is_q)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) amax = fmaxf_nan(amax, fabsf(v[i]));
+#pragma unroll
+                for (int off = G / 2; off > 0; off >>= 1) amax = fmaxf_nan(amax, __shfl_xor_sync(kFullMask, amax, off));
+            }
+            if (live && is_q) {
+                store8<T>(static_cast<typename T::storage*>(a.q_out) + ((size_t)token * a.q_heads + row) * a.head_dim + col, v);
+            } else if (live && kept) {
+                const size_t head_row = (size_t)place * a.kv_heads + (row - a.q_heads - (is_v ? a.kv_heads : 0));
+                const bool finite = amax < INFINITY, some = amax >= kKvMinAmax;   // both false for a NaN
+                const float scale = finite ? (some ? __fdiv_rn(amax, 448.0f) : 0.0f) : __int_as_float(0x7fc00000);
+                uint2 code = make_uint2(0u, 0u);
+                if (finite && some) code = e4m3x8_rn(v, __frcp_rn(scale));
+                stg_v2((is_v ? a.cache_v : a.cache_k) + head_row * a.head_dim + col, code);
+                if (sub == 0) (is_v ? a.v_scales : a.k_scales)[head_row] = scale;
+            }
         }
-        const long long at = a.cache_map ? (long long)a.cache_map[token]
-                                         : (long long)token + (a.cache_len ? a.cache_len[0] : 0);
-        if (at < 0 || at >= a.cache_rows) continue;   // a padding token
-        const size_t head_row = (size_t)at * a.kv_heads + head;
-        const bool finite = amax < INFINITY, some = amax >= kKvMinAmax;   // both false for a NaN
-        const float scale = finite ? (some ? __fdiv_rn(amax, 448.0f) : 0.0f) : __int_as_float(0x7fc00000);
-        uint2 code = make_uint2(0u, 0u);
-        if (finite && some) code = e4m3x8_rn(v, __frcp_rn(scale));
-        stg_v2((is_v ? a.cache_v : a.cache_k) + head_row * a.head_dim + col, code);
-        if (sub == 0) (is_v ? a.v_scales : a.k_scales)[head_row] = scale;
     }
 }
 
-// Reading back: out[i] = code * scale of cache row row_map[i] (i without a map), k and v in one launch; rows the map puts
-// outside the cache come back as zeros. One lane per 8 values.
-template <typename T>
+// Reading back: out[i] = code * scale of cache row row_map[i] (i without a map); rows the map puts outside the cache come
+// back as zeros. A lane takes CODES of a row's k and the same of its v (16 where head_dim allows: 16-byte loads, 32 bytes
+// out), so that the way from the row number to the codes is walked once for both, and each thread has one piece: with
+// full occupancy that streamed better than several pieces a thread (130,712 rows of 2 x 128: 43 us against 47 to 51).
+template <typename T, int CODES>
 __global__ void __launch_bounds__(kCtaThreads)
-kv_read_fp8_kernel(typename T::storage* k_out, typename T::storage* v_out, const uint8_t* __restrict__ cache_k,
-                   const uint8_t* __restrict__ cache_v, const float* __restrict__ k_scales,
-                   const float* __restrict__ v_scales, const int* __restrict__ row_map, size_t pieces, int cache_rows,
-                   int kv_heads, FastDiv piece_div, FastDiv heads_div) {
+kv_read_fp8_kernel(typename T::storage* __restrict__ k_out, typename T::storage* __restrict__ v_out,
+                   const uint8_t* __restrict__ cache_k, const uint8_t* __restrict__ cache_v, const float* __restrict__ k_scales,
+                   const float* __restrict__ v_scales, const int* __restrict__ row_map, uint32_t pieces, int cache_rows,
+                   int kv_heads, FastDiv row_div, FastDiv head_div) {
     pdl_launch_dependents();
     pdl_wait_prior_grids();
-    const size_t step = (size_t)gridDim.x * kCtaThreads;
-    for (size_t i = (size_t)blockIdx.x * kCtaThreads + threadIdx.x; i < 2 * pieces; i += step) {
-        const bool is_v = i >= pieces;
-        const uint32_t piece = (uint32_t)(is_v ? i - pieces : i);
-        const uint32_t head_row = fast_div(piece, piece_div), part = piece - head_row * piece_div.d;
-        const uint32_t row = fast_div(head_row, heads_div);
-        const int at = row_map ? row_map[row] : (int)row;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if ((unsigned)at < (unsigned)cache_rows) {
-            const size_t src = (size_t)at * kv_heads + (head_row - row * heads_div.d);
-            const uint2 code = ldg_stream_v2((is_v ? cache_v : cache_k) + (src * piece_div.d + part) * 8);
-            const float scale = (is_v ? v_scales : k_scales)[src];
+    const uint32_t piece = blockIdx.x * kCtaThreads + threadIdx.x;
+    if (piece >= pieces) return;
+    const uint32_t row = fast_div(piece, row_div), part = piece - row * row_div.d;
+    const int at = row_map ? row_map[row] : (int)row;
+    const bool there = (unsigned)at < (unsigned)cache_rows;
+    const size_t src = ((size_t)(there ? at : 0) * row_div.d + part) * CODES;
+    const size_t head_row = (size_t)(there ? at : 0) * kv_heads + fast_div(part, head_div);
+    uint32_t code[2][CODES / 4];
+    float scale[2];
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                const uint16_t pair = (uint16_t)((h < 2 ? code.x : code.y) >> (16 * (h & 1)));
-                uint32_t f16;
-                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f16) : "h"(pair));
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&f16));
-                v[2 * h] = f.x * scale;
-                v[2 * h + 1] = f.y * scale;
-            }
+    for (int h = 0; h < 2; ++h) {
+        const uint8_t* p = (h == 0 ? cache_k : cache_v) + src;
+        if (CODES == 16) {
+            const uint4 t = there ? ldg_stream_v4(p) : make_uint4(0, 0, 0, 0);
+            code[h][0] = t.x, code[h][1] = t.y, code[h][CODES / 4 - 2] = t.z, code[h][CODES / 4 - 1] = t.w;
+        } else {
+            const uint2 t = there ? ldg_stream_v2(p) : make_uint2(0, 0);
+            code[h][0] = t.x, code[h][1] = t.y;
         }
-        store8<T>((is_v ? v_out : k_out) + (size_t)piece * 8, v);
+        scale[h] = there ? (h == 0 ? k_scales : v_scales)[head_row] : 0.0f;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float v[CODES];
+#pragma unroll
+        for (int w = 0; w < CODES / 2; ++w) {
+            const uint16_t pair = (uint16_t)(code[h][w / 2] >> (16 * (w & 1)));
+            uint32_t f16;
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f16) : "h"(pair));
+            const f32x2 f = f2_mul(__half22float2(*reinterpret_cast<const __half2*>(&f16)), f2_splat(scale[h]));
+            v[2 * w] = f.x, v[2 * w + 1] = f.y;
+        }
+        typename T::storage* dst = (h == 0 ? k_out : v_out) + (size_t)piece * CODES;
+        if (T::kBytes == 2 && CODES == 16) {
+            U8x32 o;   // (the outputs are 32-byte aligned then)
+#pragma unroll
+            for (int w = 0; w < 8; ++w) o.w[w] = pack_bf16x2(v[2 * w], v[2 * w + 1 < CODES ? 2 * w + 1 : 0]);
+            stg_v8(dst, o);
+        } else {
+#pragma unroll
+            for (int w = 0; w < CODES; w += 8) store8<T>(dst + w, v + w);
+        }
     }
 }
 
