@@ -14,31 +14,45 @@ using namespace clef::abi;
 
 namespace {
 
-template <typename T, int G, bool NORM, int U>
-void launch_kv_write_u(cudaStream_t s, const DeviceInfo& dev, KvWriteArgs a) {
-    static std::atomic<int> occ{0};
-    auto kernel = kv_write_fp8_kernel<T, G, NORM, U>;
+// Warps of `per_warp` head rows of a token.
+template <typename K>
+void launch_units(K kernel, std::atomic<int>& occ, int rows, int per_warp, cudaStream_t s, const DeviceInfo& dev, KvWriteArgs a) {
     const int per_sm = ctas_per_sm(kernel, 0, occ);
-    const int rows = a.q_heads + 2 * a.kv_heads, per_warp = U * (32 / G);
     a.parts_div = make_fast_div((uint32_t)((rows + per_warp - 1) / per_warp));
     const size_t units = (size_t)a.tokens * a.parts_div.d;
     launch_hot(kernel, balanced_grid((units + kCtaThreads / 32 - 1) / (kCtaThreads / 32), (size_t)dev.sms * per_sm), 0, s, a);
 }
 
-// Five groups of head rows per warp (20 head rows of 128, 16 q, 2 k and 2 v, are two warps' work) where that still gives
-// every SM a full set of warps, one where it does not.
-template <typename T, int G, bool NORM>
+// U groups of head rows per warp where that still gives every SM 16 warps, one where it does not (8,192 tokens of 16 + 2
+// heads of 128: 17.0 us with two or three groups, 18.1 with one or five).
+template <typename T, int G>
 void launch_kv_write(cudaStream_t s, const DeviceInfo& dev, const KvWriteArgs& a) {
-    const size_t groups = (size_t)a.tokens * (a.q_heads + 2 * a.kv_heads) / (32 / G);
-    if (groups >= (size_t)dev.sms * 16 * 5) launch_kv_write_u<T, G, NORM, 5>(s, dev, a);
-    else launch_kv_write_u<T, G, NORM, 1>(s, dev, a);
+    constexpr int U = 2;
+    static std::atomic<int> occ[2];
+    const int rows = a.q_heads + 2 * a.kv_heads;
+    if ((size_t)a.tokens * rows / (32 / G) >= (size_t)dev.sms * 16 * U) {
+        launch_units(kv_write_fp8_kernel<T, G, U>, occ[0], rows, U * (32 / G), s, dev, a);
+    } else {
+        launch_units(kv_write_fp8_kernel<T, G, 1>, occ[1], rows, 32 / G, s, dev, a);
+    }
+}
+template <typename T, int G>
+void launch_kv_norm_write(cudaStream_t s, const DeviceInfo& dev, const KvWriteArgs& a) {
+    static std::atomic<int> occ{0};
+    launch_units(kv_norm_write_fp8_kernel<T, G>, occ, 2 * a.kv_heads, 32 / G, s, dev, a);
 }
 
-template <typename T, bool NORM>
-void launch_kv_write_for(cudaStream_t s, const DeviceInfo& dev, const KvWriteArgs& a) {
-    if (a.head_dim <= 64) launch_kv_write<T, 8, NORM>(s, dev, a);
-    else if (a.head_dim <= 128) launch_kv_write<T, 16, NORM>(s, dev, a);
-    else launch_kv_write<T, 32, NORM>(s, dev, a);
+template <typename T>
+void launch_kv_write_for(cudaStream_t s, const DeviceInfo& dev, const KvWriteArgs& a, bool norm) {
+    if (norm) {
+        if (a.head_dim <= 64) launch_kv_norm_write<T, 8>(s, dev, a);
+        else if (a.head_dim <= 128) launch_kv_norm_write<T, 16>(s, dev, a);
+        else launch_kv_norm_write<T, 32>(s, dev, a);
+    } else {
+        if (a.head_dim <= 64) launch_kv_write<T, 4>(s, dev, a);
+        else if (a.head_dim <= 128) launch_kv_write<T, 8>(s, dev, a);
+        else launch_kv_write<T, 16>(s, dev, a);
+    }
 }
 
 int kv_write_impl(const char* what, clef_stream_t stream, KvWriteArgs a, bool with_q, bool norm, int dtype) {
@@ -69,13 +83,8 @@ int kv_write_impl(const char* what, clef_stream_t stream, KvWriteArgs a, bool wi
     DeviceInfo dev;
     if (int r = device_info(dev)) return r;
     cudaStream_t s = as_stream(stream);
-    if (dtype == CLEF_BF16) {
-        if (norm) launch_kv_write_for<Bf16, true>(s, dev, a);
-        else launch_kv_write_for<Bf16, false>(s, dev, a);
-    } else {
-        if (norm) launch_kv_write_for<F32, true>(s, dev, a);
-        else launch_kv_write_for<F32, false>(s, dev, a);
-    }
+    if (dtype == CLEF_BF16) launch_kv_write_for<Bf16>(s, dev, a, norm);
+    else launch_kv_write_for<F32>(s, dev, a, norm);
     return check_launch(what);
 }
 

@@ -5,10 +5,12 @@
 // A head row whose maximum is below 2^-100 is stored as zeros with scale 0; one that holds an infinity or a NaN is
 // stored as zero codes with scale NaN, so that whatever reads it sees NaN.
 //
-// Bound by HBM bytes. A head row of head_dim values is a group of G = head_dim / 8 lanes (rounded up to a power of two),
-// 8 values each: 16-byte loads (bf16), the rotation partner and the row maximum by shuffles, no shared memory. A warp
-// takes U groups of head rows of ONE token, requested together: a lane's columns, and with them its cosines and sines,
-// are the same in all of them, and the chain position -> table runs beside the rows' own loads.
+// Bound by HBM bytes, if the instructions per row are few. A lane takes 16 values of a head row: 8 of the rotated half
+// and their partners half a rotary span up, or 16 that pass through (G = head_dim / 16 lanes for a head row, rounded up
+// to a power of two); nothing is exchanged but the row maximum. A warp takes U groups of 32 / G head rows of ONE token,
+// requested together: a lane's columns, and with them its cosines and sines, are the same in all of them, and the chain
+// position -> table runs beside the rows' own loads. With the per-head norm (k rows only) a lane takes 8 consecutive
+// values instead, the order of the sum.
 #pragma once
 
 #include "kernels_generic.cuh"
@@ -73,12 +75,6 @@ __device__ __forceinline__ void store8<F32>(float* p, const float* v) {
     stg_v4(p + 4, make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])));
 }
 
-// rope_pair's two outputs are one form, a * b + p * q with the product p * q rounded first, of operands that are swapped
-// between a pair's lower and upper element (and q negated for the lower): a lane computes the one that is its own.
-#if CLEF_ROPE_FMA_LO != 1 || CLEF_ROPE_FMA_HI != 2
-#error "kv_write_fp8_kernel spells rope_pair's default contraction"
-#endif
-
 // Eight activations as they are loaded.
 template <typename T>
 struct Raw8 {
@@ -99,17 +95,41 @@ __device__ __forceinline__ void widen8<F32>(const Raw8<F32>& r, float* v) {
     v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
 }
 
-// G lanes per head row; a warp holds 32 / G head rows at a time, U of those. NORM: k rows are normalised first, in the
-// summation order of rms_norm_kernel (kernels/elementwise.cu:4-68: quad i with quad i + 32, then the tree 16, 8, 4, 2, 1
-// over quads).
-template <typename T, int G, bool NORM, int U>
+template <typename T>
+__device__ __forceinline__ Raw8<T> narrow8(const float* v);
+template <>
+__device__ __forceinline__ Raw8<Bf16> narrow8<Bf16>(const float* v) {
+    return Raw8<Bf16>{{make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]))}};
+}
+template <>
+__device__ __forceinline__ Raw8<F32> narrow8<F32>(const float* v) {
+    return Raw8<F32>{{make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])),
+                      make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]))}};
+}
+
+// Where a token's rows go; false for a padding token.
+__device__ __forceinline__ bool kv_place(const KvWriteArgs& a, int token, size_t& row) {
+    const long long at = a.cache_map ? (long long)a.cache_map[token] : (long long)token + (a.cache_len ? a.cache_len[0] : 0);
+    row = (size_t)at;
+    return at >= 0 && at < a.cache_rows;
+}
+// The scale of a head row with maximum `amax` (NaN if it holds one), and the factor its values are multiplied by (0: codes 0).
+__device__ __forceinline__ float kv_scale(float amax, float& by) {
+    const bool finite = amax < INFINITY, some = amax >= kKvMinAmax;   // both false for a NaN
+    const float scale = finite ? (some ? __fdiv_rn(amax, 448.0f) : 0.0f) : __int_as_float(0x7fc00000);
+    by = finite && some ? __frcp_rn(scale) : 0.0f;
+    return scale;
+}
+
+template <typename T, int G, int U>
 __global__ void __launch_bounds__(kCtaThreads)
 kv_write_fp8_kernel(KvWriteArgs a) {
     constexpr int PER_WARP = 32 / G;
     const int lane = threadIdx.x & 31, sub = lane % G;
-    const int col = sub * 8, half = a.rotary_dim >> 1;
-    const bool in_row = col < a.head_dim, rotary = col < a.rotary_dim, upper = col >= half;
-    const int partner = rotary ? (upper ? lane - (half >> 3) : lane + (half >> 3)) : lane;
+    const int half = a.rotary_dim >> 1, turning = half >> 3;   // lanes of a row that rotate
+    const bool turns_at = sub < turning;
+    const int col = turns_at ? sub * 8 : a.rotary_dim + (sub - turning) * 16, col2 = turns_at ? col + half : col + 8;
+    const bool in_row = col < a.head_dim, in_row2 = col2 < a.head_dim;
     const int rows = a.q_heads + 2 * a.kv_heads, parts = (int)a.parts_div.d;
     const uint32_t units = (uint32_t)a.tokens * parts;
     pdl_launch_dependents();
@@ -117,101 +137,151 @@ kv_write_fp8_kernel(KvWriteArgs a) {
     for (uint32_t unit = blockIdx.x * (kCtaThreads / 32) + (threadIdx.x >> 5); unit < units; unit += gridDim.x * (kCtaThreads / 32)) {
         const int token = (int)fast_div(unit, a.parts_div);
         const int first = ((int)unit - token * parts) * (U * PER_WARP) + lane / G;
-        Raw8<T> raw[U];
+        Raw8<T> raw[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int row = first + u * PER_WARP, kv = row - a.q_heads;
+            const int head = kv < 0 ? row : (kv < a.kv_heads ? kv : kv - a.kv_heads);
+            const typename T::storage* x = static_cast<const typename T::storage*>(kv < 0 ? a.q : (kv < a.kv_heads ? a.k : a.v)) +
+                                           ((size_t)token * (kv < 0 ? a.q_heads : a.kv_heads) + head) * a.head_dim;
+#pragma unroll
+            for (int i = 0; i < T::kBytes / 2; ++i) {
+                raw[u][0].w[i] = in_row && row < rows ? ldg_stream_v4(reinterpret_cast<const uint8_t*>(x + col) + 16 * i) : make_uint4(0, 0, 0, 0);
+                raw[u][1].w[i] = in_row2 && row < rows ? ldg_stream_v4(reinterpret_cast<const uint8_t*>(x + col2) + 16 * i) : make_uint4(0, 0, 0, 0);
+            }
+        }
+        float c[8], s[8];
+        if (turns_at) {
+            const int pos = rope_position(token, a.seq_start, a.pos_base, a.pos_map);
+            const size_t at = (size_t)pos * a.rotary_dim + col;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                *reinterpret_cast<float4*>(c + 4 * i) = __ldg(reinterpret_cast<const float4*>(a.cos_t + at) + i);
+                *reinterpret_cast<float4*>(s + 4 * i) = __ldg(reinterpret_cast<const float4*>(a.sin_t + at) + i);
+            }
+        }
+        size_t place;
+        const bool kept = kv_place(a, token, place);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int row = first + u * PER_WARP;
-            const int kv = row - a.q_heads, head = kv < 0 ? row : (kv < a.kv_heads ? kv : kv - a.kv_heads);
-            const typename T::storage* x = static_cast<const typename T::storage*>(kv < 0 ? a.q : (kv < a.kv_heads ? a.k : a.v)) +
-                                           ((size_t)token * (kv < 0 ? a.q_heads : a.kv_heads) + head) * a.head_dim + col;
+            if (row - lane / G >= rows) break;   // (the whole warp)
+            const bool is_q = row < a.q_heads, is_v = row >= a.q_heads + a.kv_heads, live = in_row && row < rows;
+            if (__all_sync(kFullMask, is_q)) {   // rotated or passed through, in the activation type
+                if (turns_at) {
+                    float v[8], w[8];
+                    widen8<T>(raw[u][0], v);
+                    widen8<T>(raw[u][1], w);
 #pragma unroll
-            for (int i = 0; i < T::kBytes / 2; ++i) {
-                raw[u].w[i] = in_row && row < rows ? ldg_stream_v4(reinterpret_cast<const uint8_t*>(x) + 16 * i) : make_uint4(0, 0, 0, 0);
+                    for (int i = 0; i < 8; ++i) rope_pair(v[i], w[i], c[i], s[i], v[i], w[i]);
+                    raw[u][0] = narrow8<T>(v);
+                    raw[u][1] = narrow8<T>(w);
+                }
+                uint8_t* dst = reinterpret_cast<uint8_t*>(static_cast<typename T::storage*>(a.q_out) + ((size_t)token * a.q_heads + row) * a.head_dim);
+#pragma unroll
+                for (int i = 0; i < T::kBytes / 2; ++i) {
+                    if (in_row) stg_v4(dst + (size_t)col * T::kBytes + 16 * i, raw[u][0].w[i]);
+                    if (in_row2) stg_v4(dst + (size_t)col2 * T::kBytes + 16 * i, raw[u][1].w[i]);
+                }
+                continue;
+            }
+            float v[8], w[8];
+            widen8<T>(raw[u][0], v);
+            widen8<T>(raw[u][1], w);
+            if (turns_at && !is_v) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) rope_pair(v[i], w[i], c[i], s[i], v[i], w[i]);
+            }
+            float amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) amax = max3_abs_nan(amax, v[i], w[i]);
+#pragma unroll
+            for (int off = G / 2; off > 0; off >>= 1) amax = fmaxf_nan(amax, __shfl_xor_sync(kFullMask, amax, off));
+            if (!live) continue;
+            if (is_q) {   // a group with rows of both kinds
+                typename T::storage* dst = static_cast<typename T::storage*>(a.q_out) + ((size_t)token * a.q_heads + row) * a.head_dim;
+                store8<T>(dst + col, v);
+                if (in_row2) store8<T>(dst + col2, w);
+            } else if (kept) {
+                const size_t head_row = place * a.kv_heads + (row - a.q_heads - (is_v ? a.kv_heads : 0));
+                float by;
+                const float scale = kv_scale(amax, by);
+                uint8_t* dst = (is_v ? a.cache_v : a.cache_k) + head_row * a.head_dim;
+                stg_v2(dst + col, by > 0.0f ? e4m3x8_rn(v, by) : make_uint2(0u, 0u));
+                if (in_row2) stg_v2(dst + col2, by > 0.0f ? e4m3x8_rn(w, by) : make_uint2(0u, 0u));
+                if (sub == 0) (is_v ? a.v_scales : a.k_scales)[head_row] = scale;
             }
         }
-        float b[8], q[8];   // lower: cos, -sin; upper: sin, cos
+    }
+}
+
+// k rows normalised first, in the summation order of rms_norm_kernel (kernels/elementwise.cu:4-68: quad i with quad i + 32,
+// then the tree 16, 8, 4, 2, 1 over quads); G = head_dim / 8 lanes per head row, k and v rows of a token.
+template <typename T, int G>
+__global__ void __launch_bounds__(kCtaThreads)
+kv_norm_write_fp8_kernel(KvWriteArgs a) {
+    constexpr int PER_WARP = 32 / G;
+    const int lane = threadIdx.x & 31, sub = lane % G;
+    const int col = sub * 8, half = a.rotary_dim >> 1;
+    const bool in_row = col < a.head_dim, rotary = col < a.rotary_dim, upper = col >= half;
+    const int partner = rotary ? (upper ? lane - (half >> 3) : lane + (half >> 3)) : lane;
+    const int rows = 2 * a.kv_heads, parts = (int)a.parts_div.d;
+    const uint32_t units = (uint32_t)a.tokens * parts;
+    pdl_launch_dependents();
+    pdl_wait_prior_grids();
+    for (uint32_t unit = blockIdx.x * (kCtaThreads / 32) + (threadIdx.x >> 5); unit < units; unit += gridDim.x * (kCtaThreads / 32)) {
+        const int token = (int)fast_div(unit, a.parts_div);
+        const int row = ((int)unit - token * parts) * PER_WARP + lane / G;
+        const bool is_v = row >= a.kv_heads, live = in_row && row < rows;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        if (live) {
+            load8<T>(static_cast<const typename T::storage*>(is_v ? a.v : a.k) +
+                     ((size_t)token * a.kv_heads + (is_v ? row - a.kv_heads : row)) * a.head_dim + col, v);
+        }
+        float c[8], s[8];
         if (rotary) {
             const int pos = rope_position(token, a.seq_start, a.pos_base, a.pos_map);
             const size_t at = (size_t)pos * a.rotary_dim + (upper ? col - half : col);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float4 c = __ldg(reinterpret_cast<const float4*>(a.cos_t + at) + i), s = __ldg(reinterpret_cast<const float4*>(a.sin_t + at) + i);
-                *reinterpret_cast<float4*>(b + 4 * i) = upper ? s : c;
-                *reinterpret_cast<float4*>(q + 4 * i) = upper ? c : make_float4(-s.x, -s.y, -s.z, -s.w);
+                *reinterpret_cast<float4*>(c + 4 * i) = __ldg(reinterpret_cast<const float4*>(a.cos_t + at) + i);
+                *reinterpret_cast<float4*>(s + 4 * i) = __ldg(reinterpret_cast<const float4*>(a.sin_t + at) + i);
             }
         }
-        const long long place = a.cache_map ? (long long)a.cache_map[token] : (long long)token + (a.cache_len ? a.cache_len[0] : 0);
-        const bool kept = place >= 0 && place < a.cache_rows;   // (a padding token is not)
+        float s0 = quad_sq(make_float4(v[0], v[1], v[2], v[3])), s1 = quad_sq(make_float4(v[4], v[5], v[6], v[7]));
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int row = first + u * PER_WARP;
-            if (row - lane / G >= rows) break;   // (the whole warp)
-            const bool live = in_row && row < rows, is_q = row < a.q_heads, is_v = row >= a.q_heads + a.kv_heads;
-            float v[8];
-            if (NORM) {
-                widen8<T>(raw[u], v);
-                float s0 = quad_sq(make_float4(v[0], v[1], v[2], v[3])), s1 = quad_sq(make_float4(v[4], v[5], v[6], v[7]));
+        for (int off = G / 2; off > 0; off >>= 1) {
+            s0 = __fadd_rn(s0, __shfl_xor_sync(kFullMask, s0, off));
+            s1 = __fadd_rn(s1, __shfl_xor_sync(kFullMask, s1, off));
+        }
+        if (live && !is_v) {
+            const float inv = inv_rms(__fadd_rn(s0, s1), a.head_dim, a.eps);
 #pragma unroll
-                for (int off = G / 2; off > 0; off >>= 1) {
-                    s0 = __fadd_rn(s0, __shfl_xor_sync(kFullMask, s0, off));
-                    s1 = __fadd_rn(s1, __shfl_xor_sync(kFullMask, s1, off));
-                }
-                if (live && !is_q && !is_v) {
-                    const float inv = inv_rms(__fadd_rn(s0, s1), a.head_dim, a.eps);
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (1.0f + a.weight[col + i]);
+        }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (1.0f + a.weight[col + i]);
-                }
+        for (int i = 0; i < 8; ++i) {
+            const float other = __shfl_sync(kFullMask, v[i], partner);
+            float lo, hi;
+            if (rotary && !is_v) {
+                rope_pair(upper ? other : v[i], upper ? v[i] : other, c[i], s[i], lo, hi);
+                v[i] = upper ? hi : lo;
             }
-            const bool turns = rotary && !is_v;
-            if (__any_sync(kFullMask, turns)) {
-                float x[8], y[8];   // the element of the lower half and that of the upper, or the other way round
-                if (NORM) {
+        }
+        float amax = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float other = __shfl_sync(kFullMask, v[i], partner);
-                        x[i] = upper ? other : v[i], y[i] = upper ? v[i] : other;
-                    }
-                } else {
-                    Raw8<T> rx, ry;
+        for (int i = 0; i < 8; i += 2) amax = max3_abs_nan(amax, v[i], v[i + 1]);
 #pragma unroll
-                    for (int i = 0; i < T::kBytes / 2; ++i) {
-                        const uint4 o = make_uint4(__shfl_sync(kFullMask, raw[u].w[i].x, partner), __shfl_sync(kFullMask, raw[u].w[i].y, partner),
-                                                   __shfl_sync(kFullMask, raw[u].w[i].z, partner), __shfl_sync(kFullMask, raw[u].w[i].w, partner));
-                        rx.w[i] = upper ? o : raw[u].w[i], ry.w[i] = upper ? raw[u].w[i] : o;
-                    }
-                    widen8<T>(rx, x);
-                    widen8<T>(ry, y);
-                }
-                if (turns) {
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const f32x2 r = f2_fma(f2_pack(x[i], x[i + 1]), f2_pack(b[i], b[i + 1]), f2_mul(f2_pack(y[i], y[i + 1]), f2_pack(q[i], q[i + 1])));
-                        v[i] = r.x, v[i + 1] = r.y;
-                    }
-                } else if (!NORM) {
-                    widen8<T>(raw[u], v);
-                }
-            } else if (!NORM) {
-                widen8<T>(raw[u], v);
-            }
-            float amax = 0.0f;
-            if (__any_sync(kFullMask, !is_q)) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) amax = fmaxf_nan(amax, fabsf(v[i]));
-#pragma unroll
-                for (int off = G / 2; off > 0; off >>= 1) amax = fmaxf_nan(amax, __shfl_xor_sync(kFullMask, amax, off));
-            }
-            if (live && is_q) {
-                store8<T>(static_cast<typename T::storage*>(a.q_out) + ((size_t)token * a.q_heads + row) * a.head_dim + col, v);
-            } else if (live && kept) {
-                const size_t head_row = (size_t)place * a.kv_heads + (row - a.q_heads - (is_v ? a.kv_heads : 0));
-                const bool finite = amax < INFINITY, some = amax >= kKvMinAmax;   // both false for a NaN
-                const float scale = finite ? (some ? __fdiv_rn(amax, 448.0f) : 0.0f) : __int_as_float(0x7fc00000);
-                uint2 code = make_uint2(0u, 0u);
-                if (finite && some) code = e4m3x8_rn(v, __frcp_rn(scale));
-                stg_v2((is_v ? a.cache_v : a.cache_k) + head_row * a.head_dim + col, code);
-                if (sub == 0) (is_v ? a.v_scales : a.k_scales)[head_row] = scale;
-            }
+        for (int off = G / 2; off > 0; off >>= 1) amax = fmaxf_nan(amax, __shfl_xor_sync(kFullMask, amax, off));
+        size_t place;
+        if (kv_place(a, token, place) && live) {
+            const size_t head_row = place * a.kv_heads + (is_v ? row - a.kv_heads : row);
+            float by;
+            const float scale = kv_scale(amax, by);
+            stg_v2((is_v ? a.cache_v : a.cache_k) + head_row * a.head_dim + col, by > 0.0f ? e4m3x8_rn(v, by) : make_uint2(0u, 0u));
+            if (sub == 0) (is_v ? a.v_scales : a.k_scales)[head_row] = scale;
         }
     }
 }
