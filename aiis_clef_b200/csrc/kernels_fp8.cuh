@@ -151,88 +151,6 @@ fp8_rows_kernel(const typename T::storage* __restrict__ a, const typename T::sto
     }
 }
 
-// add_rms_norm_fp8_bf16 for any cols % 8 == 0: sum = a + b, rounded to T and stored (sum_out may be a or b), then
-// rms_norm_fp8_bf16 of the stored sum. One CTA of the reference's team of threads (kernels/elementwise.cu:8) owns a row;
-// thread t holds quads t, t + team, ... (QMAX of them at most) in registers from the one read on, in the order
-// team_sum_squares adds them.
-template <typename T, int QMAX>
-__global__ void __launch_bounds__(kCtaThreads)
-add_rms_norm_fp8_kernel(const typename T::storage* a, const typename T::storage* b, typename T::storage* sum_out,
-                        const float* __restrict__ weight, uint8_t* __restrict__ out, uint16_t* __restrict__ scales,
-                        uint16_t* __restrict__ bf_out, int rows, int cols, float eps) {
-    __shared__ float s_part[2][kCtaThreads / 32];
-    const int team = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = team >> 5, c4 = cols >> 2;
-    pdl_launch_dependents();
-    pdl_wait_prior_grids();
-    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-        const size_t at = (size_t)row * cols;
-        float4 v[QMAX];
-#pragma unroll
-        for (int k = 0; k < QMAX; ++k) {
-            const int i = threadIdx.x + k * team;
-            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (i < c4) {
-                const float4 p = load_quad<T>(a + at, i), q = load_quad<T>(b + at, i);
-                v[k] = make_float4(__fadd_rn(p.x, q.x), __fadd_rn(p.y, q.y), __fadd_rn(p.z, q.z), __fadd_rn(p.w, q.w));
-            }
-        }
-        float acc = 0.0f;
-#pragma unroll
-        for (int k = 0; k < QMAX; ++k) {
-            const int i = threadIdx.x + k * team;
-            if (i < c4) {
-                store_quad<T>(sum_out + at, i, v[k]);
-                if (T::kBytes == 2) {   // the norm sees the stored sum
-                    const uint32_t lo = pack_bf16x2(v[k].x, v[k].y), hi = pack_bf16x2(v[k].z, v[k].w);
-                    v[k] = make_float4(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi));
-                }
-                acc = __fadd_rn(acc, quad_sq(v[k]));
-            }
-        }
-        float total = warp_tree_sum(acc);
-        if (warps > 1) {
-            if (lane == 0) s_part[0][warp] = total;
-            __syncthreads();
-            total = lane < warps ? s_part[0][lane] : 0.0f;
-#pragma unroll
-            for (int off = 4; off > 0; off >>= 1) total = __fadd_rn(total, __shfl_xor_sync(kFullMask, total, off));
-            total = __shfl_sync(kFullMask, total, 0);
-        }
-        const float inv_norm = inv_rms(total, cols, eps);
-        float amax = 0.0f;
-#pragma unroll
-        for (int k = 0; k < QMAX; ++k) {
-            const int i = threadIdx.x + k * team;
-            if (i < c4) {
-                const float4 w = *reinterpret_cast<const float4*>(weight + 4 * i);
-                v[k] = make_float4(v[k].x * inv_norm * (1.0f + w.x), v[k].y * inv_norm * (1.0f + w.y),
-                                   v[k].z * inv_norm * (1.0f + w.z), v[k].w * inv_norm * (1.0f + w.w));
-                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
-            }
-        }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kFullMask, amax, off));
-        if (warps > 1) {
-            if (lane == 0) s_part[1][warp] = amax;
-            __syncthreads();
-            for (int w = 0; w < warps; ++w) amax = fmaxf(amax, s_part[1][w]);
-        }
-        const float scale = __fdiv_rn(amax, 448.0f);
-        if (threadIdx.x == 0) scales[row] = (uint16_t)(__float_as_uint(scale) >> 16);
-        const float inv = (scale > 0.0f) ? __fdiv_rn(1.0f, scale) : 0.0f;
-#pragma unroll
-        for (int k = 0; k < QMAX; ++k) {
-            const int i = threadIdx.x + k * team;
-            if (i < c4) {
-                const uint32_t code = fp8_code(v[k].x, inv) | (fp8_code(v[k].y, inv) << 8) | (fp8_code(v[k].z, inv) << 16) |
-                                      (fp8_code(v[k].w, inv) << 24);
-                *reinterpret_cast<uint32_t*>(out + at + 4 * i) = code;
-                if (bf_out) store_quad<Bf16>(bf_out + at, i, v[k]);
-            }
-        }
-    }
-}
-
 // rms_norm_gated_quantise_fp8 (kernels/quantise.cu:123-191): one CTA per token; warp w normalises the
 // head rows w, w + 8, ... (< vh) of the token, a lane the quads lane, lane + 32 (cols <= 256) of a head
 // row in the reference's order; v = x * inv * weight * __fdividef(g, 1 + __expf(-g)); the token's amax
@@ -454,6 +372,108 @@ __device__ __forceinline__ uint4 fp8_encode16_qp(const f32x2* v, f32x2 inv2) {
         }
     }
     return make_uint4(word[0], word[1], word[2], word[3]);
+}
+
+// add_rms_norm_fp8_bf16 for any cols % 8 == 0: sum = a + b, rounded to T and stored (sum_out may be a or b), then
+// rms_norm_fp8_bf16 of the stored sum. One CTA of the reference's team of threads (kernels/elementwise.cu:8) owns a row;
+// thread t holds quads t, t + team, ... (QMAX of them at most) in registers from the one read on, in the order
+// team_sum_squares adds them.
+template <typename T, int QMAX>
+__global__ void __launch_bounds__(kCtaThreads)
+add_rms_norm_fp8_kernel(const typename T::storage* a, const typename T::storage* b, typename T::storage* sum_out,
+                        const float* __restrict__ weight, uint8_t* __restrict__ out, uint16_t* __restrict__ scales,
+                        uint16_t* __restrict__ bf_out, int rows, int cols, float eps) {
+    __shared__ float s_part[3][kCtaThreads / 32];
+    const int team = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = team >> 5, c4 = cols >> 2;
+    pdl_launch_dependents();
+    pdl_wait_prior_grids();
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        const size_t at = (size_t)row * cols;
+        float4 v[QMAX];
+#pragma unroll
+        for (int k = 0; k < QMAX; ++k) {
+            const int i = threadIdx.x + k * team;
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i < c4) {
+                const float4 p = load_quad<T>(a + at, i), q = load_quad<T>(b + at, i);
+                v[k] = make_float4(__fadd_rn(p.x, q.x), __fadd_rn(p.y, q.y), __fadd_rn(p.z, q.z), __fadd_rn(p.w, q.w));
+            }
+        }
+        float acc = 0.0f;
+#pragma unroll
+        for (int k = 0; k < QMAX; ++k) {
+            const int i = threadIdx.x + k * team;
+            if (i < c4) {
+                store_quad<T>(sum_out + at, i, v[k]);
+                if (T::kBytes == 2) {   // the norm sees the stored sum
+                    const uint32_t lo = pack_bf16x2(v[k].x, v[k].y), hi = pack_bf16x2(v[k].z, v[k].w);
+                    v[k] = make_float4(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi));
+                }
+                acc = __fadd_rn(acc, quad_sq(v[k]));
+            }
+        }
+        float total = warp_tree_sum(acc);
+        if (warps > 1) {
+            if (lane == 0) s_part[0][warp] = total;
+            __syncthreads();
+            total = lane < warps ? s_part[0][lane] : 0.0f;
+#pragma unroll
+            for (int off = 4; off > 0; off >>= 1) total = __fadd_rn(total, __shfl_xor_sync(kFullMask, total, off));
+            total = __shfl_sync(kFullMask, total, 0);
+        }
+        const float inv_norm = inv_rms(total, cols, eps);
+        float amax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < QMAX; ++k) {
+            const int i = threadIdx.x + k * team;
+            if (i < c4) {
+                const float4 w = *reinterpret_cast<const float4*>(weight + 4 * i);
+                v[k] = make_float4(v[k].x * inv_norm * (1.0f + w.x), v[k].y * inv_norm * (1.0f + w.y),
+                                   v[k].z * inv_norm * (1.0f + w.z), v[k].w * inv_norm * (1.0f + w.w));
+                amax = max3_abs_nan(max3_abs_nan(amax, v[k].x, v[k].y), v[k].z, v[k].w);
+            }
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) amax = fmaxf_nan(amax, __shfl_xor_sync(kFullMask, amax, off));
+        if (warps > 1) {
+            if (lane == 0) s_part[1][warp] = amax;
+            __syncthreads();
+            for (int w = 0; w < warps; ++w) amax = fmaxf_nan(amax, s_part[1][w]);
+        }
+        const bool fast = amax == 0.0f || (amax >= kFp8FastMinAmax && amax <= kFp8FastMaxAmax);   // false for NaN; the same for the row
+        if (!fast) {   // the recipe's maximum leaves NaN out
+            amax = 0.0f;
+#pragma unroll
+            for (int k = 0; k < QMAX; ++k) {
+                if (threadIdx.x + k * team < c4) amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
+            }
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kFullMask, amax, off));
+            if (warps > 1) {
+                if (lane == 0) s_part[2][warp] = amax;
+                __syncthreads();
+                for (int w = 0; w < warps; ++w) amax = fmaxf(amax, s_part[2][w]);
+            }
+        }
+        const float scale = __fdiv_rn(amax, 448.0f);
+        if (threadIdx.x == 0) scales[row] = (uint16_t)(__float_as_uint(scale) >> 16);
+        const float inv = (scale > 0.0f) ? __fdiv_rn(1.0f, scale) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < QMAX; ++k) {
+            const int i = threadIdx.x + k * team;
+            if (i < c4) {
+                uint32_t code;
+                if (fast) {   // the converter, and the integer form where it may differ; see fp8_encode16_qp
+                    code = e4m3x4_hw(__fmul_rn(v[k].x, inv), __fmul_rn(v[k].y, inv), __fmul_rn(v[k].z, inv), __fmul_rn(v[k].w, inv));
+                    if (e4m3x4_suspect(code)) code = fp8_encode4_int(v[k].x, v[k].y, v[k].z, v[k].w, inv);
+                } else {
+                    code = fp8_code(v[k].x, inv) | (fp8_code(v[k].y, inv) << 8) | (fp8_code(v[k].z, inv) << 16) | (fp8_code(v[k].w, inv) << 24);
+                }
+                *reinterpret_cast<uint32_t*>(out + at + 4 * i) = code;
+                if (bf_out) store_quad<Bf16>(bf_out + at, i, v[k]);
+            }
+        }
+    }
 }
 
 // Literal encoder for one block of a row that left the short encoder's domain: values recomputed from global

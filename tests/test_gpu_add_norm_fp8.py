@@ -33,7 +33,7 @@ def same(x, y):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
 @pytest.mark.parametrize("rows,cols", [(1, 2048), (778, 2048), (1, 4096), (301, 4096), (3, 8), (65, 1000), (9, 512), (40, 1792), (17, 2056),
-                                       (6, 6144), (5, 8200), (2, 16384), (2500, 2048)])
+                                       (6, 6144), (5, 8200), (2, 16384), (2500, 2048), (1300, 4096)])
 def test_equals_the_chain(cuda_dev, rows, cols, dtype):
     a, b, w = inputs(rows, cols, dtype, rows + cols)
     if rows > 8:
@@ -65,11 +65,11 @@ def test_equals_the_chain(cuda_dev, rows, cols, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
 def test_general_kernel_equals_the_tuned_one(cuda_dev, dtype):
-    a, b, w = inputs(130, 2048, dtype, 1)
-    tuned = cuda_dev.add_rms_norm_fp8_bf16_dev(a, b, w, 130, 2048, EPS)
+    a, b, w = inputs(1300, 2048, dtype, 1)
+    tuned = cuda_dev.add_rms_norm_fp8_bf16_dev(a, b, w, 1300, 2048, EPS)
     clef.set_kernel_choice(1)
     try:
-        general = cuda_dev.add_rms_norm_fp8_bf16_dev(a, b, w, 130, 2048, EPS)
+        general = cuda_dev.add_rms_norm_fp8_bf16_dev(a, b, w, 1300, 2048, EPS)
     finally:
         clef.set_kernel_choice(0)
     assert all(same(x.view(-1), y.view(-1)) for x, y in zip(tuned, general))
