@@ -5,9 +5,11 @@
 //   P = exp2(...) bf16, written over S in tensor memory, one thread per row,
 //   O += P V      [128 x D] f32, P read from tensor memory, V [keys][dims] as it lies in the cache (MN-major).
 // Warps are specialised: one warpgroup of softmax per 128 rows, one warpgroup that gathers K and V rows from the pages
-// into a ring of four buffers (K, V, K, V ...), one thread that issues the products. For head_dim 64 and 128 the two
-// row blocks alternate, the products of one run under the softmax of the other; head_dim 256 has tensor memory for one
-// row block only and alternates two S buffers instead, with key tiles of 64 so that the ring fits.
+// into rings of K and of V tiles, one warp that issues the products. For head_dim 64 and 128 the two row blocks
+// alternate, the products of one run under the softmax of the other; head_dim 256 has tensor memory for one row block
+// only. An FP8 cache is multiplied in f16, as in attn_rows_kernel: codes are widened exactly in shared memory, the scale of
+// a key multiplies its column of S, that of its value its column of P. Key tiles are 64 keys and S has two buffers per row block, so that the scores of the next step are
+// there when the softmax comes to them.
 // The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (weights then stay
 // below 2^8, exact enough in f32 sums and bf16 weights alike), so the softmax rarely touches O.
 //
@@ -84,16 +86,6 @@ __device__ __forceinline__ uint32_t elect_lane() {
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(kFullMask, x, 0); }
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Four E4M3 codes times their row's scale, rounded to bf16 (what a bf16 cache would hold: half a step of 2^-8 per value,
-// next to the codes' own 2^-4; it frees the softmax of two products per key).
-__device__ __forceinline__ void e4m3x4_scaled(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
-    uint32_t a, b;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
-    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
-    lo = pack_bf16x2(x.x * scale, x.y * scale);
-    hi = pack_bf16x2(y.x * scale, y.y * scale);
-}
-
 // D[128 x N] (tensor memory) (+)= A B^T; A from shared memory or from tensor memory.
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, uint32_t leader) {
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
@@ -143,9 +135,9 @@ __device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t leading) {
 __device__ __forceinline__ uint64_t smem_desc(uint32_t low, uint32_t bytes_on) {
     return ((uint64_t)((1024 >> 4) | (1u << 14) | (2u << 29)) << 32) | (low + (bytes_on >> 4));
 }
-// Instruction descriptor: f32 accumulators, bf16 operands, A K-major; B K-major or MN-major.
-__host__ __device__ constexpr uint32_t mma_idesc(int n, bool b_mn_major) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+// Instruction descriptor: f32 accumulators, f16 or bf16 operands, A K-major; B K-major or MN-major.
+__host__ __device__ constexpr uint32_t mma_idesc(int n, bool b_mn_major, bool f16) {
+    return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 
 // Byte offset of 16-byte chunk `chunk` of row `row` in a tile of `rows` rows: 64 columns (128 bytes) side by side, the
@@ -154,7 +146,7 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int chunk, int rows) {
     return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
-// Eight q values as they are loaded, and as bf16.
+// Eight q values as they are loaded, as f32, and as operands: bf16, or f16 of the values times `by`.
 template <typename T>
 struct RawQ {
     uint4 w[T::kBytes / 2];
@@ -162,11 +154,27 @@ struct RawQ {
 #pragma unroll
         for (int i = 0; i < T::kBytes / 2; ++i) w[i] = ldg_stream_v4(reinterpret_cast<const uint8_t*>(p) + 16 * i);
     }
+    __device__ __forceinline__ void floats(float* f) const {
+        const uint4 a = w[0], b = w[T::kBytes / 2 - 1];
+        if (T::kBytes == 2) {
+            f[0] = bf16_lo(a.x), f[1] = bf16_hi(a.x), f[2] = bf16_lo(a.y), f[3] = bf16_hi(a.y);
+            f[4] = bf16_lo(a.z), f[5] = bf16_hi(a.z), f[6] = bf16_lo(a.w), f[7] = bf16_hi(a.w);
+        } else {
+            f[0] = __uint_as_float(a.x), f[1] = __uint_as_float(a.y), f[2] = __uint_as_float(a.z), f[3] = __uint_as_float(a.w);
+            f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y), f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
+        }
+    }
     __device__ __forceinline__ uint4 bf16() const {
         if (T::kBytes == 2) return w[0];
-        const uint4 b = w[T::kBytes / 2 - 1];
-        return make_uint4(pack_bf16x2(__uint_as_float(w[0].x), __uint_as_float(w[0].y)), pack_bf16x2(__uint_as_float(w[0].z), __uint_as_float(w[0].w)),
-                          pack_bf16x2(__uint_as_float(b.x), __uint_as_float(b.y)), pack_bf16x2(__uint_as_float(b.z), __uint_as_float(b.w)));
+        float f[8];
+        floats(f);
+        return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+    }
+    __device__ __forceinline__ uint4 f16(float by) const {
+        float f[8];
+        floats(f);
+        return make_uint4(pack_f16x2(f[0] * by, f[1] * by), pack_f16x2(f[2] * by, f[3] * by), pack_f16x2(f[4] * by, f[5] * by),
+                          pack_f16x2(f[6] * by, f[7] * by));
     }
 };
 
@@ -190,21 +198,19 @@ struct ChunkShape {
     static constexpr int SBUF = 2;                        // S buffers per row block
     static constexpr int SLOTS = D == 256 ? 2 : 4;        // buffers of K tiles, and as many of V tiles
     static constexpr int OV = 2;                          // a row tile's beginning and end cost about two units
-    static constexpr int PRODUCERS = FP8 ? 2 : 1;         // warpgroups: one gathers bf16 rows, widening codes takes two
-    static constexpr int THREADS = 128 * (TILES + PRODUCERS + 1);   // softmax, producers, products (one warp of the last)
-    // Registers: the block starts with START for each thread; the softmax, which keeps a row of S, takes what the others leave.
-    static constexpr bool SPLIT = TILES + PRODUCERS > 2;
-    static constexpr int START = THREADS == 640 ? 96 : (THREADS == 512 ? 128 : 168);
-    static constexpr int SOFTMAX_REGS = THREADS == 640 ? 144 : 184, PRODUCER_REGS = THREADS == 640 ? 64 : (TILES == 2 ? 80 : 96);
-    static constexpr int MMA_REGS = 64;
-    static_assert(!SPLIT || TILES * SOFTMAX_REGS + PRODUCERS * PRODUCER_REGS + MMA_REGS <= START * THREADS / 128, "more than the block started with");
+    static constexpr int THREADS = 128 * (TILES + 2);     // softmax, producers, products (one warp of the last)
+    // Registers: 512 threads start with 128 each; the softmax, which keeps a row of S, takes what the others leave.
+    static constexpr bool SPLIT = TILES == 2;
+    static constexpr int SOFTMAX_REGS = 184, PRODUCER_REGS = 80, MMA_REGS = 64;
+    static_assert(!SPLIT || TILES * SOFTMAX_REGS + PRODUCER_REGS + MMA_REGS <= 512, "more than the block started with");
     static constexpr int Q_BYTES = 128 * D * 2;
     static constexpr int KV_BYTES = N * D * 2;
     static constexpr int S_COL = 0;                       // tensor memory columns: S buffers, then O
     static constexpr int O_COL = TILES * SBUF * N;
-    static constexpr int STAGES = D == 256 ? 2 : 4;       // FP8: tiles of codes on their way, beside the widened ones
-    static constexpr int STAGE_BYTES = N * D + N * 4;     // codes and row scales
-    static constexpr int SMEM = 1024 + TILES * Q_BYTES + 2 * SLOTS * KV_BYTES + (FP8 ? STAGES * STAGE_BYTES : 0);
+    // FP8: steps whose scales are kept. Those of step n are asked for when its K tile has a slot, so when the scores of step
+    // n - SLOTS are done, which come SBUF steps after weights: no softmax is behind step n - SLOTS - 1 then.
+    static constexpr int SCALE_STEPS = 2 * SLOTS;
+    static constexpr int SMEM = 1024 + TILES * Q_BYTES + 2 * SLOTS * KV_BYTES + (FP8 ? SCALE_STEPS * 2 * N * 4 + TILES * 512 : 0);
 };
 
 // Steps of a segment [begin, end) of key tiles, the same for every role: whole tiles of N keys, none that lies past the
@@ -237,12 +243,13 @@ attn_chunk_kernel(AttnArgs a) {
     uint8_t* s_base = s_raw + ((1024 - (smem_addr(s_raw) & 1023)) & 1023);
     uint8_t* s_q = s_base;
     uint8_t* s_kv = s_q + TILES * Sh::Q_BYTES;
-    uint8_t* s_stage = s_kv + 2 * SLOTS * Sh::KV_BYTES;   // FP8 only
+    float* s_scales = reinterpret_cast<float*>(s_kv + 2 * SLOTS * Sh::KV_BYTES);   // FP8: [SCALE_STEPS][k, v][N]
+    float* s_q_scale = s_scales + Sh::SCALE_STEPS * 2 * N;                         // FP8: [TILES][128]
     volatile int* gave_up = &s_gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4 * Sh::PRODUCERS;
+    constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2 * SLOTS; ++i) mbar_init(&full[i], 128 * Sh::PRODUCERS), mbar_init(&empty[i], 1);
+        for (int i = 0; i < 2 * SLOTS; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
         for (int i = 0; i < TILES; ++i) mbar_init(&q_ready[i], 128);
         for (int i = 0; i < TILES * SBUF; ++i) mbar_init(&s_ready[i], 1), mbar_init(&p_ready[i], 128);
         for (int i = 0; i < TILES * 2; ++i) mbar_init(&pv_done[i], 1);
@@ -275,8 +282,8 @@ attn_chunk_kernel(AttnArgs a) {
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;          // (32 (warp % 4)) << 16
         const uint32_t o_addr = tmem + lanes + Sh::O_COL + t * D;
         uint8_t* q_tile = s_q + t * Sh::Q_BYTES;
-        const float scale = fabsf(a.scale_log2);
         const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale negates q instead
+        uint32_t kv_steps = 0;                                      // of the CTA, over all segments
         int steps_done = 0;                                         // of this row block, over all segments
         // The product with P of the nth step. Even and odd steps have a barrier each: a wait may be left out, as that for
         // the step after the next one on the same barrier cannot end before this block's softmax has come that far.
@@ -289,9 +296,12 @@ attn_chunk_kernel(AttnArgs a) {
             attn_segment<OV>(a, cur, begin, end);
             const AttnSeq span = cur.span;
             const int rows = span.n * a.group, row0 = cur.tile * R + t * 128;
-            if (begin == end || row0 >= rows) continue;
+            if (begin == end) continue;
             int keys, from, to;
             chunk_steps<D, FP8>(a, cur, begin, end, keys, from, to);
+            const uint32_t kv_first = kv_steps;
+            kv_steps += to - from;
+            if (row0 >= rows) continue;
             // q: 16-byte chunks, eight lanes to a 128-byte line, rounded to bf16, into the swizzled tile; eight requests in
             // flight (rows past the last repeat it, and are stored as zeros)
 #pragma unroll 1
@@ -307,13 +317,32 @@ attn_chunk_kernel(AttnArgs a) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int i = (i0 + j) * 128 + x, r = i / (D / 8);
-                    uint4 w = raw[j].bf16();
+                    uint4 w;
+                    if (FP8) {   // f16, of the row divided by the power of two that its largest element has
+                        float f[8], most = 0.0f;
+                        raw[j].floats(f);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]));
+#pragma unroll
+                        for (int off = 1; off < D / 8; off <<= 1) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, off));
+                        const int exponent = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100);
+                        w = raw[j].f16(__uint_as_float((uint32_t)(127 - exponent) << 23));
+                        if (i % (D / 8) == 0) s_q_scale[t * 128 + r] = __uint_as_float((uint32_t)(127 + exponent) << 23);
+                    } else {
+                        w = raw[j].bf16();
+                    }
                     w = row0 + r < rows ? make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip) : make_uint4(0, 0, 0, 0);
                     *reinterpret_cast<uint4*>(q_tile + tile_offset(r, i % (D / 8), 128)) = w;
                 }
             }
             async_proxy_fence();
             mbar_arrive(&q_ready[t]);
+            float scale = fabsf(a.scale_log2);
+            int v_exponent = -100;   // FP8: the value scales seen so far are not above 2^v_exponent
+            if (FP8) {
+                block_barrier(t);
+                scale *= s_q_scale[t * 128 + x];
+            }
             const int lim = row0 + x < rows ? attn_visible(a, span, row0 + x + 1) : 0;
             float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
@@ -321,12 +350,29 @@ attn_chunk_kernel(AttnArgs a) {
                 const int buf = SBUF == 1 ? 0 : (steps_done & 1);
                 const uint32_t s_addr = tmem + lanes + Sh::S_COL + (t * SBUF + buf) * N;
                 const uint32_t s_parity = (SBUF == 1 ? steps_done : steps_done >> 1) & 1;
+                // FP8: the scales of the step's keys came with its V tile, whose slot is not used again before this step's weights
+                const uint32_t nth_kv = kv_first + (step - from);
+                const float* sc = s_scales + nth_kv % Sh::SCALE_STEPS * 2 * N;
+                if (FP8) mbar_wait_warp(&full[SLOTS + nth_kv % SLOTS], (nth_kv / SLOTS) & 1, gave_up);
                 mbar_wait_warp(&s_ready[t * SBUF + buf], s_parity, gave_up);
                 tc_fence_after();
                 f32x2 s[N / 2];
 #pragma unroll
                 for (int c = 0; c < N; c += 32) tc_ld32(s_addr + c, reinterpret_cast<float*>(s + c / 2));
                 tc_wait_ld();
+                if (FP8) {
+#pragma unroll
+                    for (int i = 0; i < N / 2; i += 2) {
+                        const float4 k4 = *reinterpret_cast<const float4*>(sc + 2 * i);
+                        s[i] = f2_mul(s[i], f2_pack(k4.x, k4.y));
+                        s[i + 1] = f2_mul(s[i + 1], f2_pack(k4.z, k4.w));
+                    }
+                    // weight times value scale is to stay within f16: the reference that the weights are taken against is
+                    // raised by the exponent of the largest value scale (O and the sum are divided by the same)
+                    const float vs = fmaxf(sc[N + (x & 31)], sc[N + 32 + (x & 31)]);   // (NaN, of a head row that held one, counts as 0)
+                    const int e = vs < INFINITY ? max((int)(__float_as_uint(vs) >> 23) - 126, -100) : -100;
+                    if (__any_sync(kFullMask, e > v_exponent)) v_exponent = max(v_exponent, __reduce_max_sync(kFullMask, e));
+                }
                 const int base = step * N;
                 const bool edge = __any_sync(kFullMask, base + N > lim);   // some keys of the step are hidden from some row
                 if (edge) {
@@ -343,7 +389,7 @@ attn_chunk_kernel(AttnArgs a) {
                     top1 = max3(top1, s[i + 1].x, s[i + 1].y);
                 }
                 float top = fmaxf(max3(top0, top1, s[N / 2 - 1].x), s[N / 2 - 1].y);
-                top = top == -INFINITY ? top : top * scale;
+                top = top == -INFINITY ? top : top * scale + (FP8 ? (float)v_exponent : 0.0f);
                 const bool grown = top > m + 8.0f;   // (m = -inf: any key at all)
                 if (__any_sync(kFullMask, grown)) {
                     const float now = grown ? top : m;
@@ -383,7 +429,17 @@ attn_chunk_kernel(AttnArgs a) {
                             }
                             if (i % 2 == 0) sum0 = f2_add(sum0, e);
                             else sum1 = f2_add(sum1, e);
-                            p[i] = pack_bf16x2(e.x, e.y);
+                            if (FP8) {
+                                const float4 v4 = *reinterpret_cast<const float4*>(sc + N + 2 * (c + (i & ~1)));
+                                e = f2_mul(e, i % 2 == 0 ? f2_pack(v4.x, v4.y) : f2_pack(v4.z, v4.w));
+                                if (EDGE) {   // whatever scale a hidden key has, its weight is 0
+                                    e.x = base + 2 * (c + i) < lim ? e.x : 0.0f;
+                                    e.y = base + 2 * (c + i) + 1 < lim ? e.y : 0.0f;
+                                }
+                                p[i] = pack_f16x2(e.x, e.y);
+                            } else {
+                                p[i] = pack_bf16x2(e.x, e.y);
+                            }
                         }
                         tc_st16(s_addr + c, p);   // over columns of S that are in registers
                     }
@@ -460,7 +516,7 @@ attn_chunk_kernel(AttnArgs a) {
         }
     } else if (warp < kMmaWarp) {
         // ---- producers: a warp gathers ROWS rows of each tile, lane l of it knows row l's place -----------------
-        constexpr int WARPS = 4 * Sh::PRODUCERS, ROWS = N / WARPS;
+        constexpr int WARPS = 4, ROWS = N / WARPS;
         if (Sh::SPLIT) set_registers<Sh::PRODUCER_REGS, false>();
         AttnCursor cur = s_cursor;
         const int w = warp - kProducerWarp;
@@ -468,74 +524,63 @@ attn_chunk_kernel(AttnArgs a) {
         constexpr int CPR = D * (FP8 ? 1 : 2) / 16;       // 16-byte pieces of a cache row
         constexpr int RPI = 32 / (CPR < 8 ? CPR : 8);     // rows a warp touches at once
         constexpr int LPR = 32 / RPI;                     // lanes per row
-        constexpr int DEPTH = FP8 ? Sh::STAGES : 3;   // tiles on their way
+        constexpr int DEPTH = 3;              // tiles on their way
         uint32_t asked[2] = {0, 0};           // K and V tiles so far
         uint32_t pending = 0, in_flight = 0;  // the slots not handed over yet, four bits each, the oldest on top
-        uint32_t used_slots[2] = {0, 0}, taken = 0;
-        auto arrived = [&](bool all) {        // the oldest tile on its way (with `all`, every one)
-            if (all) asm volatile("cp.async.wait_group 0;" ::: "memory");
-            else asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
-        };
-        auto oldest = [&]() { return pending >> (4 * (in_flight - 1)) & 15; };
-        // bf16: rows go straight into their slot, and are handed over once there
+        // place of this thread's nth piece of codes: the upper half of the slot that they are widened into
+        auto code_at = [&](uint8_t* tile, int n) { return tile + Sh::KV_BYTES / 2 + ((n * WARPS + w) * 32 + lane) * 16; };
+        // Hands over the oldest tile on its way, or all of them, once they have arrived. bf16 rows are where they belong. E4M3
+        // codes are widened to f16, exactly: each thread takes up the codes that it copied, and when all have, the f16
+        // rows are written over them.
         auto hand_over = [&](bool all) {
             if (in_flight == 0) return;
-            arrived(all);
-            async_proxy_fence();
-            for (; in_flight > (all ? 0u : DEPTH - 1u); --in_flight) mbar_arrive(&full[oldest()]);
-        };
-        // FP8: the oldest staged tile is widened into its slot. A thread reads the codes that it copied itself; the row scales
-        // are the warp's.
-        auto widen = [&](bool all) {
-            arrived(all);
-            __syncwarp();
-            const uint32_t slot = oldest(), which = slot / SLOTS, parity = ((used_slots[which]++ / SLOTS) & 1) ^ 1;
-            const uint8_t* stage = s_stage + taken % Sh::STAGES * Sh::STAGE_BYTES;
-            uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
-            mbar_wait_warp(&empty[slot], parity, gave_up);
+            if (all) asm volatile("cp.async.wait_group 0;" ::: "memory");
+            else asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+            if (!FP8) async_proxy_fence();
+            for (; in_flight > (all ? 0u : DEPTH - 1u); --in_flight) {
+                const uint32_t slot = pending >> (4 * (in_flight - 1)) & 15;
+                if (FP8) {
+                    uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
+                    uint4 code[ROWS / RPI * (CPR / LPR)];
 #pragma unroll
-            for (int i = 0; i < ROWS / RPI; ++i) {
-                const int r = w * ROWS + i * RPI + lane / LPR;
-                const float scale = *reinterpret_cast<const float*>(stage + N * D + r * 4);
+                    for (int n = 0; n < ROWS / RPI * (CPR / LPR); ++n) code[n] = *reinterpret_cast<const uint4*>(code_at(tile, n));
+                    asm volatile("bar.sync 3, 128;" ::: "memory");
 #pragma unroll
-                for (int j = 0; j < CPR / LPR; ++j) {
-                    const uint4 code = *reinterpret_cast<const uint4*>(stage + (((i * (CPR / LPR) + j) * WARPS + w) * 32 + lane) * 16);
-                    const int ch = 2 * (lane % LPR + j * LPR);
-                    uint4 lo, hi;
-                    e4m3x4_scaled(code.x, scale, lo.x, lo.y);
-                    e4m3x4_scaled(code.y, scale, lo.z, lo.w);
-                    e4m3x4_scaled(code.z, scale, hi.x, hi.y);
-                    e4m3x4_scaled(code.w, scale, hi.z, hi.w);
-                    *reinterpret_cast<uint4*>(tile + tile_offset(r, ch, N)) = lo;
-                    *reinterpret_cast<uint4*>(tile + tile_offset(r, ch + 1, N)) = hi;
+                    for (int n = 0; n < ROWS / RPI * (CPR / LPR); ++n) {
+                        const int r = w * ROWS + n / (CPR / LPR) * RPI + lane / LPR, ch = 2 * (lane % LPR + n % (CPR / LPR) * LPR);
+                        uint4 lo, hi;
+                        e4m3x4_to_f16(code[n].x, lo.x, lo.y);
+                        e4m3x4_to_f16(code[n].y, lo.z, lo.w);
+                        e4m3x4_to_f16(code[n].z, hi.x, hi.y);
+                        e4m3x4_to_f16(code[n].w, hi.z, hi.w);
+                        *reinterpret_cast<uint4*>(tile + tile_offset(r, ch, N)) = lo;
+                        *reinterpret_cast<uint4*>(tile + tile_offset(r, ch + 1, N)) = hi;
+                    }
+                    async_proxy_fence();
                 }
+                mbar_arrive(&full[slot]);
             }
-            async_proxy_fence();
-            mbar_arrive(&full[slot]);
-            --in_flight, ++taken;
-            __syncwarp();
         };
         // tile `which` (0: K, 1: V) of the step whose cache rows are row32
         auto fetch = [&](int which, int row32) {
-            const uint32_t nth = asked[which]++, slot = which * SLOTS + nth % SLOTS;
-            uint8_t* to;
-            if (!FP8) {
-                // While its slot is still being read, the warp lets the rows it has asked for arrive, and hands them over.
-                const uint32_t parity = ((nth / SLOTS) & 1) ^ 1;
-                if (!mbar_try(&empty[slot], parity)) {
-                    hand_over(true);
-                    mbar_wait(&empty[slot], parity, gave_up);
-                }
-                __syncwarp();
-                to = s_kv + slot * Sh::KV_BYTES;
-            } else {
-                if (in_flight == DEPTH) widen(false);
-                to = s_stage + (taken + in_flight) % Sh::STAGES * Sh::STAGE_BYTES;
-                if (lane < ROWS) {
-                    const float* by = (which == 0 ? a.k_scales : a.v_scales) + (size_t)(row32 < 0 ? 0 : row32) * a.kv_heads + cur.head;
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(to + N * D + (w * ROWS + lane) * 4)), "l"(by),
-                                 "r"(row32 < 0 ? 0 : 4) : "memory");
-                }
+            const uint32_t nth = asked[which]++, slot = which * SLOTS + nth % SLOTS, parity = ((nth / SLOTS) & 1) ^ 1;
+            uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
+            // While the slot is still being read, what has been asked for is handed over as it arrives. (FP8: the four warps
+            // decide alike, they widen together.)
+            uint32_t busy = !mbar_try(&empty[slot], parity);
+            if (FP8) {
+                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %0, 0;\n\tbarrier.cta.red.or.pred q, 3, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                             : "+r"(busy)::"memory");
+            }
+            if (busy) {
+                hand_over(true);
+                mbar_wait(&empty[slot], parity, gave_up);
+            }
+            __syncwarp();
+            if (FP8 && lane < ROWS) {
+                const float* from = (which == 0 ? a.k_scales : a.v_scales) + (size_t)(row32 < 0 ? 0 : row32) * a.kv_heads + cur.head;
+                const uint32_t to = smem_addr(s_scales + (nth % Sh::SCALE_STEPS * 2 + which) * N + w * ROWS + lane);
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(row32 < 0 ? 0 : 4) : "memory");
             }
             const CacheT* src = static_cast<const CacheT*>(which == 0 ? a.k : a.v);
 #pragma unroll
@@ -546,14 +591,13 @@ attn_chunk_kernel(AttnArgs a) {
 #pragma unroll
                 for (int j = 0; j < CPR / LPR; ++j) {
                     const int ch = lane % LPR + j * LPR;
-                    const uint32_t dst = smem_addr(to + (FP8 ? (((i * (CPR / LPR) + j) * WARPS + w) * 32 + lane) * 16 : tile_offset(w * ROWS + r, ch, N)));
+                    const uint32_t dst = smem_addr(FP8 ? code_at(tile, i * (CPR / LPR) + j) : tile + tile_offset(w * ROWS + r, ch, N));
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p + 16 * ch), "r"(row < 0 ? 0 : 16) : "memory");
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             pending = pending << 4 | slot;
-            ++in_flight;
-            if (!FP8 && in_flight == DEPTH) hand_over(false);
+            if (++in_flight == DEPTH) hand_over(false);
         };
         for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
             int begin, end, keys, from, to;
@@ -581,11 +625,7 @@ attn_chunk_kernel(AttnArgs a) {
                 rows_of[SBUF] = ahead;
             }
         }
-        if (!FP8) {
-            hand_over(true);
-        } else {
-            while (in_flight > 0) widen(true);
-        }
+        hand_over(true);
     } else {
         if (Sh::SPLIT) set_registers<Sh::MMA_REGS, false>();
         AttnCursor cur = s_cursor;
@@ -593,7 +633,7 @@ attn_chunk_kernel(AttnArgs a) {
         // ---- products: one warp, one lane of which issues ----------------------------------------------------------
         const uint32_t leader = elect_lane();
         const uint32_t q_base = uniform((int)smem_addr(s_q)), kv_base = uniform((int)smem_addr(s_kv)), acc = uniform((int)tmem);
-        constexpr uint32_t s_idesc = mma_idesc(N, false), o_idesc = mma_idesc(D, true);
+        constexpr uint32_t s_idesc = mma_idesc(N, false, FP8), o_idesc = mma_idesc(D, true, FP8);
         uint32_t used = 0;                // K tiles, and V tiles, consumed so far
         int segments[TILES] = {}, steps_done[TILES] = {};
         auto scores = [&](int t, int nth, uint32_t k_slot) {   // S of the nth step of row block t
