@@ -7,8 +7,9 @@
 // Warps are specialised: one warpgroup of softmax per 128 rows, one warpgroup that gathers K and V rows from the pages
 // into rings of K and of V tiles, one warp that issues the products. For head_dim 64 and 128 the two row blocks
 // alternate, the products of one run under the softmax of the other; head_dim 256 has tensor memory for one row block
-// only. An FP8 cache is multiplied in f16, as in attn_rows_kernel: codes are widened exactly in shared memory, the scale of
-// a key multiplies its column of S, that of its value its column of P. Key tiles are 64 keys and S has two buffers per row block, so that the scores of the next step are
+// only. An FP8 cache is multiplied in f16: the 16 rows that a producer warp widens are brought under one power of two,
+// code * (scale / 2^e) in f16 (2^-11 per value, next to the codes' own 2^-4), which the softmax multiplies back: 2^e of K
+// with the score scale of those 16 keys, 2^e of V with the reference of their weights. Key tiles are 64 keys and S has two buffers per row block, so that the scores of the next step are
 // there when the softmax comes to them.
 // The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (weights then stay
 // below 2^8, exact enough in f32 sums and bf16 weights alike), so the softmax rarely touches O.
@@ -85,6 +86,12 @@ __device__ __forceinline__ uint32_t elect_lane() {
 }
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(kFullMask, x, 0); }
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 
 // D[128 x N] (tensor memory) (+)= A B^T; A from shared memory or from tensor memory.
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, uint32_t leader) {
@@ -207,10 +214,10 @@ struct ChunkShape {
     static constexpr int KV_BYTES = N * D * 2;
     static constexpr int S_COL = 0;                       // tensor memory columns: S buffers, then O
     static constexpr int O_COL = TILES * SBUF * N;
-    // FP8: steps whose scales are kept. Those of step n are asked for when its K tile has a slot, so when the scores of step
-    // n - SLOTS are done, which come SBUF steps after weights: no softmax is behind step n - SLOTS - 1 then.
+    // FP8: steps whose scales and exponents are kept. Those of step n are asked for when its K tile has a slot, so when the
+    // scores of step n - SLOTS are done, which come SBUF steps after weights: no softmax is behind step n - SLOTS - 1 then.
     static constexpr int SCALE_STEPS = 2 * SLOTS;
-    static constexpr int SMEM = 1024 + TILES * Q_BYTES + 2 * SLOTS * KV_BYTES + (FP8 ? SCALE_STEPS * 2 * N * 4 + TILES * 512 : 0);
+    static constexpr int SMEM = 1024 + TILES * Q_BYTES + 2 * SLOTS * KV_BYTES + (FP8 ? SCALE_STEPS * (2 * N + 8) * 4 + TILES * 512 : 0);
 };
 
 // Steps of a segment [begin, end) of key tiles, the same for every role: whole tiles of N keys, none that lies past the
@@ -237,6 +244,7 @@ attn_chunk_kernel(AttnArgs a) {
     constexpr int TILES = Sh::TILES, R = Sh::R, N = Sh::N, SBUF = Sh::SBUF, SLOTS = Sh::SLOTS, OV = Sh::OV;
     extern __shared__ uint8_t s_raw[];
     __shared__ uint64_t full[2 * SLOTS], empty[2 * SLOTS], q_ready[TILES], s_ready[TILES * SBUF], p_ready[TILES * SBUF], pv_done[TILES * 2], drained;
+    __shared__ uint64_t exponents_ready[Sh::SCALE_STEPS];   // FP8
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ AttnCursor s_cursor;
@@ -244,7 +252,8 @@ attn_chunk_kernel(AttnArgs a) {
     uint8_t* s_q = s_base;
     uint8_t* s_kv = s_q + TILES * Sh::Q_BYTES;
     float* s_scales = reinterpret_cast<float*>(s_kv + 2 * SLOTS * Sh::KV_BYTES);   // FP8: [SCALE_STEPS][k, v][N]
-    float* s_q_scale = s_scales + Sh::SCALE_STEPS * 2 * N;                         // FP8: [TILES][128]
+    int* s_exponents = reinterpret_cast<int*>(s_scales + Sh::SCALE_STEPS * 2 * N); // FP8: [SCALE_STEPS][k, v][4]
+    float* s_q_scale = reinterpret_cast<float*>(s_exponents + Sh::SCALE_STEPS * 8);   // FP8: [TILES][128]
     volatile int* gave_up = &s_gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4;
@@ -253,6 +262,7 @@ attn_chunk_kernel(AttnArgs a) {
         for (int i = 0; i < TILES; ++i) mbar_init(&q_ready[i], 128);
         for (int i = 0; i < TILES * SBUF; ++i) mbar_init(&s_ready[i], 1), mbar_init(&p_ready[i], 128);
         for (int i = 0; i < TILES * 2; ++i) mbar_init(&pv_done[i], 1);
+        for (int i = 0; i < Sh::SCALE_STEPS; ++i) mbar_init(&exponents_ready[i], 4);
         mbar_init(&drained, 1);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -350,29 +360,32 @@ attn_chunk_kernel(AttnArgs a) {
                 const int buf = SBUF == 1 ? 0 : (steps_done & 1);
                 const uint32_t s_addr = tmem + lanes + Sh::S_COL + (t * SBUF + buf) * N;
                 const uint32_t s_parity = (SBUF == 1 ? steps_done : steps_done >> 1) & 1;
-                // FP8: the scales of the step's keys came with its V tile, whose slot is not used again before this step's weights
                 const uint32_t nth_kv = kv_first + (step - from);
-                const float* sc = s_scales + nth_kv % Sh::SCALE_STEPS * 2 * N;
-                if (FP8) mbar_wait_warp(&full[SLOTS + nth_kv % SLOTS], (nth_kv / SLOTS) & 1, gave_up);
+                if (FP8) mbar_wait_warp(&exponents_ready[nth_kv % Sh::SCALE_STEPS], (nth_kv / Sh::SCALE_STEPS) & 1, gave_up);
+                // score scale and weight exponent of each 16 keys
+                constexpr int GROUPS = FP8 ? N / 16 : 1;
+                float by[GROUPS];
+                int e_v[GROUPS];
+                by[0] = scale, e_v[0] = 0;
+                if (FP8) {
+                    const int4 ek = *reinterpret_cast<const int4*>(s_exponents + nth_kv % Sh::SCALE_STEPS * 8);
+                    const int4 ev = *reinterpret_cast<const int4*>(s_exponents + nth_kv % Sh::SCALE_STEPS * 8 + 4);
+                    const int k[4] = {ek.x, ek.y, ek.z, ek.w}, v[4] = {ev.x, ev.y, ev.z, ev.w};
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g) {
+                        by[g] = scale * __int_as_float((127 + k[g]) << 23);
+                        e_v[g] = v[g];
+                        // the reference that weights are taken against is raised by the largest exponent of V so far, so that
+                        // weight times 2^e stays within f16 (O and the sum are divided by the same)
+                        v_exponent = max(v_exponent, v[g]);
+                    }
+                }
                 mbar_wait_warp(&s_ready[t * SBUF + buf], s_parity, gave_up);
                 tc_fence_after();
                 f32x2 s[N / 2];
 #pragma unroll
                 for (int c = 0; c < N; c += 32) tc_ld32(s_addr + c, reinterpret_cast<float*>(s + c / 2));
                 tc_wait_ld();
-                if (FP8) {
-#pragma unroll
-                    for (int i = 0; i < N / 2; i += 2) {
-                        const float4 k4 = *reinterpret_cast<const float4*>(sc + 2 * i);
-                        s[i] = f2_mul(s[i], f2_pack(k4.x, k4.y));
-                        s[i + 1] = f2_mul(s[i + 1], f2_pack(k4.z, k4.w));
-                    }
-                    // weight times value scale is to stay within f16: the reference that the weights are taken against is
-                    // raised by the exponent of the largest value scale (O and the sum are divided by the same)
-                    const float vs = fmaxf(sc[N + (x & 31)], sc[N + 32 + (x & 31)]);   // (NaN, of a head row that held one, counts as 0)
-                    const int e = vs < INFINITY ? max((int)(__float_as_uint(vs) >> 23) - 126, -100) : -100;
-                    if (__any_sync(kFullMask, e > v_exponent)) v_exponent = max(v_exponent, __reduce_max_sync(kFullMask, e));
-                }
                 const int base = step * N;
                 const bool edge = __any_sync(kFullMask, base + N > lim);   // some keys of the step are hidden from some row
                 if (edge) {
@@ -382,14 +395,20 @@ attn_chunk_kernel(AttnArgs a) {
                         s[i].y = base + 2 * i + 1 < lim ? s[i].y : -INFINITY;
                     }
                 }
-                float top0 = s[0].x, top1 = s[0].y;
+                float top = -INFINITY;
 #pragma unroll
-                for (int i = 1; i < N / 2 - 1; i += 2) {
-                    top0 = max3(top0, s[i].x, s[i].y);
-                    top1 = max3(top1, s[i + 1].x, s[i + 1].y);
+                for (int g = 0; g < GROUPS; ++g) {
+                    constexpr int PAIRS = N / 2 / GROUPS;
+                    float top0 = s[g * PAIRS].x, top1 = s[g * PAIRS].y;
+#pragma unroll
+                    for (int i = 1; i < PAIRS - 1; i += 2) {
+                        top0 = max3(top0, s[g * PAIRS + i].x, s[g * PAIRS + i].y);
+                        top1 = max3(top1, s[g * PAIRS + i + 1].x, s[g * PAIRS + i + 1].y);
+                    }
+                    top0 = fmaxf(max3(top0, top1, s[g * PAIRS + PAIRS - 1].x), s[g * PAIRS + PAIRS - 1].y);
+                    top = fmaxf(top, top0 == -INFINITY ? top0 : top0 * by[g]);
                 }
-                float top = fmaxf(max3(top0, top1, s[N / 2 - 1].x), s[N / 2 - 1].y);
-                top = top == -INFINITY ? top : top * scale + (FP8 ? (float)v_exponent : 0.0f);
+                if (FP8) top += (float)v_exponent;
                 const bool grown = top > m + 8.0f;   // (m = -inf: any key at all)
                 if (__any_sync(kFullMask, grown)) {
                     const float now = grown ? top : m;
@@ -410,9 +429,8 @@ attn_chunk_kernel(AttnArgs a) {
                         }
                     }
                 }
-                const f32x2 ref = f2_splat(m == -INFINITY ? 0.0f : -m);
-                const f32x2 by = f2_splat(scale);
-                f32x2 sum0 = f2_splat(0.0f), sum1 = f2_splat(0.0f);
+                const float ref = m == -INFINITY ? 0.0f : -m;
+                f32x2 sums[GROUPS][2];
                 auto weights = [&](auto with_edge) {   // (compiled twice: a test per pair would cost more than the pair)
                     constexpr bool EDGE = decltype(with_edge)::value;
 #pragma unroll
@@ -420,34 +438,28 @@ attn_chunk_kernel(AttnArgs a) {
                         uint32_t p[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            f32x2 e = f2_fma(s[c + i], by, ref);
+                            const int g = FP8 ? (c + i) / 8 : 0;
+                            f32x2 e = f2_fma(s[c + i], f2_splat(by[g]), f2_splat(FP8 ? ref + (float)e_v[g] : ref));
                             if (EDGE) {   // hidden keys: a weight of exactly 0 (and scale 0 would make NaN of their -inf)
                                 e.x = base + 2 * (c + i) < lim ? fast_exp2(e.x) : 0.0f;
                                 e.y = base + 2 * (c + i) + 1 < lim ? fast_exp2(e.y) : 0.0f;
                             } else {
                                 e = f2_pack(fast_exp2(e.x), fast_exp2(e.y));
                             }
-                            if (i % 2 == 0) sum0 = f2_add(sum0, e);
-                            else sum1 = f2_add(sum1, e);
-                            if (FP8) {
-                                const float4 v4 = *reinterpret_cast<const float4*>(sc + N + 2 * (c + (i & ~1)));
-                                e = f2_mul(e, i % 2 == 0 ? f2_pack(v4.x, v4.y) : f2_pack(v4.z, v4.w));
-                                if (EDGE) {   // whatever scale a hidden key has, its weight is 0
-                                    e.x = base + 2 * (c + i) < lim ? e.x : 0.0f;
-                                    e.y = base + 2 * (c + i) + 1 < lim ? e.y : 0.0f;
-                                }
-                                p[i] = pack_f16x2(e.x, e.y);
-                            } else {
-                                p[i] = pack_bf16x2(e.x, e.y);
-                            }
+                            const bool opens = FP8 ? (c + i) % 8 < 2 : c + i < 2;
+                            sums[g][i % 2] = opens ? e : f2_add(sums[g][i % 2], e);
+                            p[i] = FP8 ? pack_f16x2(e.x, e.y) : pack_bf16x2(e.x, e.y);
                         }
                         tc_st16(s_addr + c, p);   // over columns of S that are in registers
                     }
                 };
                 if (edge) weights(std::true_type{});
                 else weights(std::false_type{});
-                sum0 = f2_add(sum0, sum1);
-                l += sum0.x + sum0.y;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    const f32x2 sum = f2_add(sums[g][0], sums[g][1]);
+                    l = FP8 ? fmaf(sum.x + sum.y, __int_as_float((127 - e_v[g]) << 23), l) : l + (sum.x + sum.y);
+                }
                 tc_wait_st();
                 tc_fence_before();
                 mbar_arrive(&p_ready[t * SBUF + buf]);
@@ -530,8 +542,10 @@ attn_chunk_kernel(AttnArgs a) {
         // place of this thread's nth piece of codes: the upper half of the slot that they are widened into
         auto code_at = [&](uint8_t* tile, int n) { return tile + Sh::KV_BYTES / 2 + ((n * WARPS + w) * 32 + lane) * 16; };
         // Hands over the oldest tile on its way, or all of them, once they have arrived. bf16 rows are where they belong. E4M3
-        // codes are widened to f16, exactly: each thread takes up the codes that it copied, and when all have, the f16
-        // rows are written over them.
+        // codes are widened: each thread takes up the codes that it copied, and when all have, the f16 rows are written over
+        // them. A head row that held no number (its scale is NaN) makes its score NaN, whichever of the two it is, and
+        // counts as zeros in V: a row that does not see the key is spared.
+        uint32_t widened[2] = {0, 0};
         auto hand_over = [&](bool all) {
             if (in_flight == 0) return;
             if (all) asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -544,6 +558,22 @@ attn_chunk_kernel(AttnArgs a) {
                     uint4 code[ROWS / RPI * (CPR / LPR)];
 #pragma unroll
                     for (int n = 0; n < ROWS / RPI * (CPR / LPR); ++n) code[n] = *reinterpret_cast<const uint4*>(code_at(tile, n));
+                    const uint32_t which = slot / SLOTS, nth = widened[which]++ % Sh::SCALE_STEPS;
+                    const float* sc = s_scales + nth * 2 * N + w * ROWS + lane % ROWS;   // (as this lane or lane % ROWS copied them)
+                    __syncwarp();
+                    const float k = sc[0], v = sc[N];
+                    // the powers of two that no scale of the warp's rows reaches
+                    auto exponent = [&](float scale) {
+                        return __reduce_max_sync(kFullMask, scale < INFINITY ? max((int)(__float_as_uint(scale) >> 23) - 126, -100) : -100);
+                    };
+                    const int ek = exponent(k), ev = exponent(v);
+                    if (which == 0 && lane == 0) {
+                        s_exponents[nth * 8 + w] = ek, s_exponents[nth * 8 + 4 + w] = ev;
+                        mbar_arrive(&exponents_ready[nth]);
+                    }
+                    float unit = which == 0 ? k * __int_as_float((127 - ek) << 23) : v * __int_as_float((127 - ev) << 23);
+                    if (!(v < INFINITY)) unit = which == 0 ? __int_as_float(0x7fc00000) : 0.0f;
+                    const uint32_t by = pack_f16x2(unit, unit);
                     asm volatile("bar.sync 3, 128;" ::: "memory");
 #pragma unroll
                     for (int n = 0; n < ROWS / RPI * (CPR / LPR); ++n) {
@@ -553,6 +583,9 @@ attn_chunk_kernel(AttnArgs a) {
                         e4m3x4_to_f16(code[n].y, lo.z, lo.w);
                         e4m3x4_to_f16(code[n].z, hi.x, hi.y);
                         e4m3x4_to_f16(code[n].w, hi.z, hi.w);
+                        const uint32_t f = __shfl_sync(kFullMask, by, n / (CPR / LPR) * RPI + lane / LPR);
+                        lo = make_uint4(mul_f16x2(lo.x, f), mul_f16x2(lo.y, f), mul_f16x2(lo.z, f), mul_f16x2(lo.w, f));
+                        hi = make_uint4(mul_f16x2(hi.x, f), mul_f16x2(hi.y, f), mul_f16x2(hi.z, f), mul_f16x2(hi.w, f));
                         *reinterpret_cast<uint4*>(tile + tile_offset(r, ch, N)) = lo;
                         *reinterpret_cast<uint4*>(tile + tile_offset(r, ch + 1, N)) = hi;
                     }
@@ -577,10 +610,11 @@ attn_chunk_kernel(AttnArgs a) {
                 mbar_wait(&empty[slot], parity, gave_up);
             }
             __syncwarp();
-            if (FP8 && lane < ROWS) {
-                const float* from = (which == 0 ? a.k_scales : a.v_scales) + (size_t)(row32 < 0 ? 0 : row32) * a.kv_heads + cur.head;
-                const uint32_t to = smem_addr(s_scales + (nth % Sh::SCALE_STEPS * 2 + which) * N + w * ROWS + lane);
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(row32 < 0 ? 0 : 4) : "memory");
+            if (FP8 && which == 0 && lane < ROWS) {   // both scales come with K
+                const size_t at = (size_t)(row32 < 0 ? 0 : row32) * a.kv_heads + cur.head;
+                const uint32_t to = smem_addr(s_scales + nth % Sh::SCALE_STEPS * 2 * N + w * ROWS + lane);
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(a.k_scales + at), "r"(row32 < 0 ? 0 : 4) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + N * 4), "l"(a.v_scales + at), "r"(row32 < 0 ? 0 : 4) : "memory");
             }
             const CacheT* src = static_cast<const CacheT*>(which == 0 ? a.k : a.v);
 #pragma unroll
