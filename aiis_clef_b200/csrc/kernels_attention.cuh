@@ -609,7 +609,7 @@ attn_rows_kernel(AttnArgs a) {
 // and outputs of several partials requested together: the time is a chain of memory latencies.
 // attn_combine_kernel (partials of attn_rows_kernel): WARPS = 8, few row tiles with many partials: a block per row and 64
 // columns, warp w takes every eighth partial, joined in shared memory in a fixed order; WARPS = 1: a warp per row.
-// attn_combine_rows_kernel (of attn_chunk_kernel): many rows with few partials, four rows per warp.
+// attn_combine_rows_kernel (of attn_chunk_kernel): four rows at a time, of a warp (WARPS = 1) or a block (8), likewise.
 // ---------------------------------------------------------------------------------------------
 // The next CTA from `from` on, before `to`, that begins a row tile others go on with; `to` if there is none.
 __device__ __forceinline__ int attn_next_first(const AttnArgs& a, int from, int to) {
@@ -720,30 +720,25 @@ attn_combine_kernel(AttnArgs a, int ctas) {
     }
 }
 
-template <typename T, int D, int R>
+template <typename T, int D, int R, int WARPS>
 __global__ void __launch_bounds__(256)
 attn_combine_rows_kernel(AttnArgs a, int ctas) {
-    constexpr int Q = D / 32;   // column quads of a lane: lane / 4, lane / 4 + 8, ... of row lane % 4 of the warp's four
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int Q = D / 32;   // column quads of a lane: lane / 4, lane / 4 + 8, ... of row lane % 4 of the four
+    __shared__ float4 s_acc[WARPS == 1 ? 1 : 8][Q][32];
+    __shared__ float s_top[WARPS == 1 ? 1 : 8][4], s_sum[WARPS == 1 ? 1 : 8][4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = WARPS == 1 ? 0 : warp;
+    const int x0 = WARPS == 1 ? (blockIdx.y * 8 + warp) * 4 : blockIdx.y * 4, x = x0 + (lane & 3);
     pdl_launch_dependents();
     pdl_wait_prior_grids();
     const int from = (int)((long long)blockIdx.x * ctas / gridDim.x), to = (int)((long long)(blockIdx.x + 1) * ctas / gridDim.x);
     for (int first = attn_next_first(a, from, to); first < to; first = attn_next_first(a, first + 1, to)) {
         const AttnDesc d = a.desc[first];
-        const int x0 = (blockIdx.y * 8 + warp) * 4, x = x0 + (lane & 3);
-        if (d.tile * R + x0 >= d.rows) continue;
+        if (d.tile * R + x0 >= d.rows) continue;   // (the same for the whole block, or a warp of its own)
         float top = -INFINITY, sum = 0.0f;
         float4 acc[Q];
 #pragma unroll
         for (int e = 0; e < Q; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-        for (int i = 0; i < d.parts; ++i) {
-            const float* p = attn_slot(a, first + i, i == 0 ? 1 : 0, R, D);
-            const float4* src = reinterpret_cast<const float4*>(p + 2 * R) + (lane >> 2) * R + x;
-            float4 o[Q];
-            const float m = p[x], l = p[R + x];
-#pragma unroll
-            for (int e = 0; e < Q; ++e) o[e] = src[8 * e * R];
+        auto add = [&](float m, float l, const float4* o) {
             const float now = fmaxf(top, m), ref = now == -INFINITY ? 0.0f : now;
             const float f = fast_exp2(m - ref), g = fast_exp2(top - ref);
             top = now;
@@ -752,6 +747,31 @@ attn_combine_rows_kernel(AttnArgs a, int ctas) {
             for (int e = 0; e < Q; ++e) {
                 acc[e].x = fmaf(f, o[e].x, acc[e].x * g), acc[e].y = fmaf(f, o[e].y, acc[e].y * g);
                 acc[e].z = fmaf(f, o[e].z, acc[e].z * g), acc[e].w = fmaf(f, o[e].w, acc[e].w * g);
+            }
+        };
+#pragma unroll 2
+        for (int i = sub; i < d.parts; i += WARPS) {
+            const float* p = attn_slot(a, first + i, i == 0 ? 1 : 0, R, D);
+            const float4* src = reinterpret_cast<const float4*>(p + 2 * R) + (lane >> 2) * R + x;
+            float4 o[Q];
+            const float m = p[x], l = p[R + x];
+#pragma unroll
+            for (int e = 0; e < Q; ++e) o[e] = src[8 * e * R];
+            add(m, l, o);
+        }
+        if (WARPS > 1) {
+            __syncthreads();   // the last row tile's join is over
+#pragma unroll
+            for (int e = 0; e < Q; ++e) s_acc[warp][e][lane] = acc[e];
+            if (lane < 4) s_top[warp][lane] = top, s_sum[warp][lane] = sum;
+            __syncthreads();
+            if (warp > 0) continue;
+#pragma unroll 1
+            for (int w = 1; w < WARPS; ++w) {
+                float4 o[Q];
+#pragma unroll
+                for (int e = 0; e < Q; ++e) o[e] = s_acc[w][e][lane];
+                add(s_top[w][lane & 3], s_sum[w][lane & 3], o);
             }
         }
         if (d.tile * R + x < d.rows) {

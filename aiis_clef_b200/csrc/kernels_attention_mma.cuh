@@ -353,13 +353,21 @@ attn_chunk_kernel(AttnArgs a) {
                 block_barrier(t);
                 scale *= s_q_scale[t * 128 + x];
             }
-            const int lim = row0 + x < rows ? attn_visible(a, span, row0 + x + 1) : 0;
+            // rows past the last one are computed along where their warp has a live row (of zeros, nothing hidden), and what
+            // comes of them is not stored; a warp without one only keeps step
+            const int lim = row0 + x < rows ? attn_visible(a, span, row0 + x + 1) : 0x7fffffff;
+            const bool warp_live = row0 + (x & ~31) < rows;
             float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
             for (int step = from; step < to; ++step, ++steps_done) {
                 const int buf = SBUF == 1 ? 0 : (steps_done & 1);
                 const uint32_t s_addr = tmem + lanes + Sh::S_COL + (t * SBUF + buf) * N;
                 const uint32_t s_parity = (SBUF == 1 ? steps_done : steps_done >> 1) & 1;
+                if (!warp_live) {
+                    mbar_wait_warp(&s_ready[t * SBUF + buf], s_parity, gave_up);
+                    mbar_arrive(&p_ready[t * SBUF + buf]);
+                    continue;
+                }
                 const uint32_t nth_kv = kv_first + (step - from);
                 if (FP8) mbar_wait_warp(&exponents_ready[nth_kv % Sh::SCALE_STEPS], (nth_kv / Sh::SCALE_STEPS) & 1, gave_up);
                 // score scale and weight exponent of each 16 keys
