@@ -85,9 +85,7 @@ int launch_units(K kernel, unsigned threads, size_t smem, size_t most, cudaStrea
     if constexpr (CHUNK) {
         if (ctas > 8 * plan.items) launch_pdl(attn_combine_rows_kernel<T, D, R, 8>, dim3(runs, R / 4, 1), 256, 0, s, a, (int)ctas);
         else launch_pdl(attn_combine_rows_kernel<T, D, R, 1>, dim3(runs, R / 32, 1), 256, 0, s, a, (int)ctas);
-        return check_launch(what);
-    }
-    if constexpr (!CHUNK) {
+    } else {
         if (ctas > 8 * plan.items) launch_pdl(attn_combine_kernel<T, D, R, 8>, dim3(runs, R, D / 64), 256, 0, s, a, (int)ctas);
         else launch_pdl(attn_combine_kernel<T, D, R, 1>, dim3(runs, R / 8, 1), 256, 0, s, a, (int)ctas);
     }
@@ -120,7 +118,10 @@ int launch_chunk(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const
 template <typename T, bool FP8, int D>
 int launch_for(cudaStream_t s, const DeviceInfo& dev, const AttnArgs& a, const AttnPlan& plan, const char* what) {
     if (plan.chunk) return launch_chunk<T, FP8, D>(s, dev, a, plan, what);
-    return plan.rows == 8 ? launch_rows<T, FP8, D, 1>(s, dev, a, plan, what) : launch_rows<T, FP8, D, 2>(s, dev, a, plan, what);
+    if constexpr (FP8 || D != 256) {   // (a plan of 16 rows)
+        if (plan.rows == 16) return launch_rows<T, FP8, D, 2>(s, dev, a, plan, what);
+    }
+    return launch_rows<T, FP8, D, 1>(s, dev, a, plan, what);
 }
 
 template <typename T, bool FP8>

@@ -187,16 +187,16 @@ int clef_add_rms_norm_fp8_bf16(clef_stream_t stream, void* sum_out, const void* 
                                int dtype) {
     const char* what = "clef_add_rms_norm_fp8_bf16";
     if (int r = check_dtype(dtype, what)) return r;
-    if (!sum_out || !a || !b || !weight || !q_out || !q_scales) return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
     if (rows < 0 || cols <= 0 || cols % 8 != 0) {
         return fail(CLEF_ERR_INVALID, "%s: rows %d, cols %d (cols must be a positive multiple of 8)", what, rows, cols);
     }
     if (cols > kFp8MaxCols) return fail(CLEF_ERR_TOO_LARGE, "%s: cols %d above %d", what, cols, kFp8MaxCols);
+    if (rows == 0) return CLEF_OK;
+    if (!sum_out || !a || !b || !weight || !q_out || !q_scales) return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
     if (!aligned(sum_out, 16) || !aligned(a, 16) || !aligned(b, 16) || !aligned(weight, 16) || !aligned(q_out, 8) ||
         !aligned(q_scales, 2) || (bf_out && !aligned(bf_out, 16))) {
         return fail(CLEF_ERR_INVALID, "%s: activations, weight and the bf16 output must be 16-byte aligned, codes 8-byte", what);
     }
-    if (rows == 0) return CLEF_OK;
     DeviceInfo dev;
     if (int r = device_info(dev)) return r;
     cudaStream_t s = as_stream(stream);

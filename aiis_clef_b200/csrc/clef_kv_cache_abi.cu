@@ -57,10 +57,6 @@ void launch_kv_write_for(cudaStream_t s, const DeviceInfo& dev, const KvWriteArg
 
 int kv_write_impl(const char* what, clef_stream_t stream, KvWriteArgs a, bool with_q, bool norm, int dtype) {
     if (int r = check_dtype(dtype, what)) return r;
-    if (!a.cache_k || !a.cache_v || !a.k_scales || !a.v_scales || !a.k || !a.v || !a.cos_t || !a.sin_t ||
-        (with_q && (!a.q || !a.q_out)) || (norm && !a.weight)) {
-        return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
-    }
     if (a.tokens < 0 || a.kv_heads <= 0 || (with_q && a.q_heads <= 0) || a.head_dim <= 0 || a.rotary_dim < 0 || a.cache_rows < 0) {
         return fail(CLEF_ERR_INVALID, "%s: tokens %d q_heads %d kv_heads %d head_dim %d rotary_dim %d cache_rows %d", what, a.tokens,
                     a.q_heads, a.kv_heads, a.head_dim, a.rotary_dim, a.cache_rows);
@@ -70,6 +66,11 @@ int kv_write_impl(const char* what, clef_stream_t stream, KvWriteArgs a, bool wi
                     a.head_dim, a.rotary_dim);
     }
     if (a.head_dim > kKvMaxHeadDim) return fail(CLEF_ERR_TOO_LARGE, "%s: head_dim %d above %d", what, a.head_dim, kKvMaxHeadDim);
+    if (a.tokens == 0) return CLEF_OK;
+    if (!a.cache_k || !a.cache_v || !a.k_scales || !a.v_scales || !a.k || !a.v || !a.cos_t || !a.sin_t ||
+        (with_q && (!a.q || !a.q_out)) || (norm && !a.weight)) {
+        return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
+    }
     if (with_q && a.q_out == a.q) return fail(CLEF_ERR_INVALID, "%s: q_out must not alias q", what);
     if ((with_q && (!aligned(a.q, 16) || !aligned(a.q_out, 16))) || !aligned(a.k, 16) || !aligned(a.v, 16) ||
         !aligned(a.cos_t, 16) || !aligned(a.sin_t, 16) || !aligned(a.cache_k, 8) || !aligned(a.cache_v, 8) ||
@@ -79,7 +80,6 @@ int kv_write_impl(const char* what, clef_stream_t stream, KvWriteArgs a, bool wi
     const long long per_token = (long long)a.q_heads + 2LL * a.kv_heads;
     // the grid-stride counter advances past the last head row by up to one grid of them
     if (per_token * a.tokens >= 0x40000000LL) return fail(CLEF_ERR_TOO_LARGE, "%s: %d tokens x %lld head rows", what, a.tokens, per_token);
-    if (a.tokens == 0) return CLEF_OK;
     DeviceInfo dev;
     if (int r = device_info(dev)) return r;
     cudaStream_t s = as_stream(stream);
@@ -131,11 +131,12 @@ int clef_kv_read_fp8(clef_stream_t stream, void* k_out, void* v_out, const uint8
                      int kv_heads, int head_dim, int dtype) {
     const char* what = "clef_kv_read_fp8";
     if (int r = check_dtype(dtype, what)) return r;
-    if (!k_out || !v_out || !cache_k || !cache_v || !k_scales || !v_scales) return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
     if (rows < 0 || cache_rows < 0 || kv_heads <= 0 || head_dim <= 0 || head_dim % 8 != 0) {
         return fail(CLEF_ERR_INVALID, "%s: rows %d cache_rows %d kv_heads %d head_dim %d (a multiple of 8)", what, rows, cache_rows,
                     kv_heads, head_dim);
     }
+    if (rows == 0) return CLEF_OK;
+    if (!k_out || !v_out || !cache_k || !cache_v || !k_scales || !v_scales) return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
     if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(cache_k, 8) || !aligned(cache_v, 8) || !aligned(k_scales, 4) ||
         !aligned(v_scales, 4)) {
         return fail(CLEF_ERR_INVALID, "%s: outputs must be 16-byte aligned, codes 8-byte", what);
@@ -144,7 +145,6 @@ int clef_kv_read_fp8(clef_stream_t stream, void* k_out, void* v_out, const uint8
     if (head_rows >= 0x7fffffffull || head_rows * (head_dim / 8) >= 0x7fffffffull) {
         return fail(CLEF_ERR_TOO_LARGE, "%s: %d rows of %d x %d", what, rows, kv_heads, head_dim);
     }
-    if (rows == 0) return CLEF_OK;
     DeviceInfo dev;
     if (int r = device_info(dev)) return r;
     cudaStream_t s = as_stream(stream);

@@ -2,13 +2,13 @@
 // the two. For query row i of a sequence with n new tokens and kv cached ones (the new ones included, they are the
 // last n), the keys it sees are 0 .. kv - n + i:
 //   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp2(scale log2(e) q_i . k_j - m_i),   m_i = running maximum
-// Scores, maxima, sums and outputs are f32; q, p and the cached values enter the products as bf16.
+// Scores, maxima, sums and outputs are f32; q and p enter the products as bf16 over a bf16 cache, as f16 over an FP8 one.
 //
 // The q heads that share a kv head are rows of ONE product: row x of a (sequence, kv head) is new token x / group,
 // head x % group. Rows are cut into row tiles of R, keys into tiles of kAttnKeys, and the (row tile, key tile) units
 // of the whole batch are one flat list that every CTA takes an equal, contiguous share of: a lone long sequence
 // fills the machine as well as an uneven batch does, and the grid depends on shapes alone. A row tile whose keys
-// were cut over several CTAs leaves (m, l, o) partials in the workspace, and attn_combine_kernel joins them in CTA
+// were cut over several CTAs leaves (m, l, o) partials in the workspace, and a second kernel joins them in a fixed
 // order, so results do not depend on timing.
 #pragma once
 
@@ -501,12 +501,13 @@ attn_rows_kernel(AttnArgs a) {
                     p[2 + e] = fast_exp2(s[nt][2 + e] - ref);
                     l[nt][e] += p[e] + p[2 + e];
                 }
-                // weights rounded to bf16 or f16 for the product (the sum above keeps them in f32); masked keys stay exactly 0
+                // weights rounded to bf16 or f16 for the product (the sum above keeps them in f32); hidden keys stay exactly 0,
+                // whatever their scale
                 if (FP8) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        p[e] = p[e] == 0.0f ? 0.0f : p[e] * vs0;
-                        p[2 + e] = p[2 + e] == 0.0f ? 0.0f : p[2 + e] * vs1;
+                        p[e] = t0 + r < lim[nt][e] ? p[e] * vs0 : 0.0f;
+                        p[2 + e] = t0 + r + 8 < lim[nt][e] ? p[2 + e] * vs1 : 0.0f;
                     }
                 }
                 pf[nt][0] = transpose8x8(FP8 ? pack_f16x2(p[0], p[1]) : pack_bf16x2(p[0], p[1]));

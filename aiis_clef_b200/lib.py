@@ -206,7 +206,7 @@ class Device:
     def __init__(self, device: int | str | torch.device = 0):
         self.device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
         self.lib = load()
-        self._index = self.device.index or 0
+        self._index = self.device.index   # None: whichever is current at the call
         if not torch.cuda.is_available():
             raise ClefError("no CUDA device: the fused kernels run on a B200 only")
 
@@ -217,10 +217,17 @@ class Device:
     def _call(self, name: str, *args):
         """One entry point on this device's current stream; the device is switched to only if it is not the current one."""
         fn = getattr(self.lib, name)
-        if torch._C._cuda_getDevice() == self._index:
-            return _check(fn(torch._C._cuda_getCurrentRawStream(self._index), *args), name)
+        if self._index is None or torch._C._cuda_getDevice() == self._index:
+            return _check(fn(_stream(), *args), name)
         with torch.cuda.device(self.device):
             return _check(fn(torch._C._cuda_getCurrentRawStream(self._index), *args), name)
+
+    def _operand(self, t, what: str, dtype, least: int):
+        """Refuses a tensor that a kernel could not read as `least` or more contiguous values of `dtype` on this device."""
+        if t is None or t.dtype != dtype or t.numel() < least or not t.is_contiguous() or not t.is_cuda or (
+                self._index is not None and t.get_device() != self._index):
+            got = "None" if t is None else f"{t.numel()} values of {t.dtype} on {t.device}" + ("" if t.is_contiguous() else ", not contiguous")
+            raise ClefError(f"{what} must be a contiguous CUDA tensor of {dtype} on {self.device} with {least} or more values, got {got}")
 
     def _like(self, t, shape, dtype):
         """An uninitialised output of `shape`: torch makes one in the shape of an input in half the time."""
@@ -494,30 +501,27 @@ class Device:
         and v_scales) cache; page_table [n_seqs, width], q_start [n_seqs + 1] and kv_len [n_seqs] are int32. `out` rows
         outside every sequence are left as they are; without `out` a new tensor is returned. `workspace` defaults to a
         fresh one of paged_attention_workspace bytes."""
-        for t, name in ((q, "q"), (cache_k, "cache_k"), (cache_v, "cache_v"), (page_table, "page_table"),
-                        (q_start, "q_start"), (kv_len, "kv_len")):
-            _dev_tensor(t, name)
         for t, name in ((page_table, "page_table"), (q_start, "q_start"), (kv_len, "kv_len")):
-            if t.dtype != torch.int32:
-                raise ClefError(f"{name} must be int32, got {t.dtype}")
+            self._operand(t, name, torch.int32, 0)
+        self._operand(q, "q", q.dtype, 0)
         n_seqs, total_q = kv_len.numel(), q.numel() // (q_heads * head_dim)
         if page_table.dim() != 2 or page_table.shape[0] != n_seqs or q_start.numel() != n_seqs + 1:
             raise ClefError(f"page_table {tuple(page_table.shape)} and q_start {tuple(q_start.shape)} must be [n_seqs, width] "
                             f"and [n_seqs + 1] for n_seqs = {n_seqs}")
         fp8 = cache_k.dtype in (torch.uint8, torch.float8_e4m3fn)
-        if cache_v.dtype != cache_k.dtype or not (fp8 or cache_k.dtype == torch.bfloat16):
-            raise ClefError(f"the caches must both be bfloat16 or E4M3 codes, got {cache_k.dtype} and {cache_v.dtype}")
         if fp8:
             cache_rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
         else:
             cache_rows = cache_k.numel() // (kv_heads * head_dim)
-            if cache_v.numel() != cache_k.numel():
-                raise ClefError("cache_k and cache_v must have the same size")
+            self._operand(cache_k, "cache_k", torch.bfloat16, 0)
+            self._operand(cache_v, "cache_v", torch.bfloat16, cache_k.numel())
         if out is None:
             out = torch.empty_like(q)
-        elif _dev_tensor(out, "out").dtype != q.dtype or out.numel() != q.numel():
-            raise ClefError("out must have the type and the size of q")
-        if workspace is None:
+        else:
+            self._operand(out, "out", q.dtype, q.numel())
+        if workspace is not None:
+            self._operand(workspace, "workspace", torch.uint8, 0)
+        else:
             workspace = q.new_empty((paged_attention_workspace(n_seqs, total_q, q_heads, kv_heads, head_dim),), dtype=torch.uint8)
         self._call("clef_paged_attention", out.data_ptr(), q.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), _ptr(k_scales),
                    _ptr(v_scales), page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), n_seqs, total_q, q_heads, kv_heads,
@@ -529,22 +533,32 @@ class Device:
 
     def _fp8_cache(self, cache_k, cache_v, k_scales, v_scales, kv_heads: int, head_dim: int) -> int:
         """Checks the four buffers of an FP8 cache against each other; returns its rows."""
-        for t, name in ((cache_k, "cache_k"), (cache_v, "cache_v")):
-            if _dev_tensor(t, name).dtype not in (torch.uint8, torch.float8_e4m3fn):
-                raise ClefError(f"{name} must hold E4M3 codes (uint8 or float8_e4m3fn), got {t.dtype}")
+        if cache_k.dtype not in (torch.uint8, torch.float8_e4m3fn):
+            raise ClefError(f"cache_k must hold E4M3 codes (uint8 or float8_e4m3fn), got {cache_k.dtype}")
         rows = cache_k.numel() // (kv_heads * head_dim)
-        if cache_v.numel() != cache_k.numel():
-            raise ClefError("cache_k and cache_v must have the same size")
-        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
-            if _dev_tensor(t, name).dtype != torch.float32 or t.numel() != rows * kv_heads:
-                raise ClefError(f"{name} must be float32 with one value per cache row and kv head")
+        self._operand(cache_k, "cache_k", cache_k.dtype, 0)
+        self._operand(cache_v, "cache_v", cache_k.dtype, cache_k.numel())
+        self._operand(k_scales, "k_scales", torch.float32, rows * kv_heads)
+        self._operand(v_scales, "v_scales", torch.float32, rows * kv_heads)
         return rows
+
+    def _kv_write_inputs(self, k, v, cos, sin, tokens: int, kv_heads: int, head_dim: int, seq_start, pos_base, pos_map, cache_map,
+                         cache_len):
+        """Checks what the three writers of an FP8 cache read beside it."""
+        self._operand(k, "k", k.dtype, tokens * kv_heads * head_dim)
+        self._operand(v, "v", k.dtype, tokens * kv_heads * head_dim)
+        self._operand(cos, "cos", torch.float32, 0)
+        self._operand(sin, "sin", torch.float32, cos.numel())
+        for t, name, least in ((seq_start, "seq_start", 1), (pos_base, "pos_base", 1), (pos_map, "pos_map", tokens),
+                               (cache_map, "cache_map", tokens), (cache_len, "cache_len", 1)):
+            if t is not None:
+                self._operand(t, name, torch.int32, least)
 
     def rope_kv_write_fp8_dev(self, cache_k, cache_v, k_scales, v_scales, k, v, cos, sin, tokens: int, kv_heads: int,
                               head_dim: int, rotary_dim: int, seq_start=None, pos_base=None, pos_map=None, cache_map=None,
                               cache_len=None):
         """rope_apply_dev on k, then k and v into the FP8 caches and their scales (in place), one launch."""
-        _dev_tensor(k, "k"), _dev_tensor(v, "v")
+        self._kv_write_inputs(k, v, cos, sin, tokens, kv_heads, head_dim, seq_start, pos_base, pos_map, cache_map, cache_len)
         rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
         self._call("clef_rope_kv_write_fp8", cache_k.data_ptr(), cache_v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                    k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), tokens, kv_heads, head_dim, rotary_dim,
@@ -554,7 +568,8 @@ class Device:
                                kv_heads: int, head_dim: int, rotary_dim: int, seq_start=None, pos_base=None, pos_map=None,
                                cache_map=None, cache_len=None):
         """rope_apply_dev on q (returned) and rope_kv_write_fp8_dev on k, v (caches written in place), one launch."""
-        _dev_tensor(q, "q"), _dev_tensor(k, "k"), _dev_tensor(v, "v")
+        self._kv_write_inputs(k, v, cos, sin, tokens, kv_heads, head_dim, seq_start, pos_base, pos_map, cache_map, cache_len)
+        self._operand(q, "q", k.dtype, tokens * q_heads * head_dim)
         rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
         q_out = self._like(q, (tokens, q_heads, head_dim), q.dtype)
         self._call("clef_rope_qkv_write_fp8", q_out.data_ptr(), q.data_ptr(), q_heads, cache_k.data_ptr(), cache_v.data_ptr(),
@@ -567,7 +582,8 @@ class Device:
                                       kv_heads: int, head_dim: int, rotary_dim: int, eps: float, seq_start=None,
                                       pos_base=None, pos_map=None, cache_map=None, cache_len=None):
         """qk_norm_rope_dev on k_raw, then k and v into the FP8 caches and their scales (in place), one launch."""
-        _dev_tensor(k_raw, "k_raw"), _dev_tensor(v, "v")
+        self._kv_write_inputs(k_raw, v, cos, sin, tokens, kv_heads, head_dim, seq_start, pos_base, pos_map, cache_map, cache_len)
+        self._operand(weight, "weight", torch.float32, head_dim)
         rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
         self._call("clef_qk_norm_rope_kv_write_fp8", cache_k.data_ptr(), cache_v.data_ptr(), k_scales.data_ptr(),
                    v_scales.data_ptr(), k_raw.data_ptr(), v.data_ptr(), weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), tokens,
@@ -578,6 +594,8 @@ class Device:
                         dtype=torch.bfloat16):
         """(k, v) [rows, kv_heads, head_dim] of `dtype`: the cache rows row_map (0 .. rows - 1 without a map) read back."""
         cache_rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
+        if row_map is not None:
+            self._operand(row_map, "row_map", torch.int32, rows)
         k = self._empty((rows, kv_heads, head_dim), dtype)
         v = torch.empty_like(k)
         self._call("clef_kv_read_fp8", k.data_ptr(), v.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), k_scales.data_ptr(),
@@ -618,10 +636,14 @@ class Device:
     def add_rms_norm_fp8_bf16_dev(self, a, b, weight, rows: int, cols: int, eps: float, sum_out=None):
         """add_dev followed by rms_norm_fp8_bf16_dev on the stored sum, one pass; returns (sum, codes, row scales, bf16
         copy)."""
-        _dev_tensor(a, "a"), _dev_tensor(b, "b")
+        self._operand(a, "a", a.dtype, rows * cols)
+        self._operand(b, "b", a.dtype, rows * cols)
+        self._operand(weight, "weight", torch.float32, cols)
         shape = (rows, cols)
         if sum_out is None:
             sum_out = self._like(a, shape, a.dtype)
+        else:
+            self._operand(sum_out, "sum_out", a.dtype, rows * cols)
         q, qs, bf = self._like(a, shape, torch.uint8), a.new_empty((rows,), dtype=torch.int16), self._like(a, shape, torch.bfloat16)
         self._call("clef_add_rms_norm_fp8_bf16", sum_out.data_ptr(), a.data_ptr(), b.data_ptr(), weight.data_ptr(), q.data_ptr(),
                    qs.data_ptr(), bf.data_ptr(), rows, cols, eps, _dtype_code(a))

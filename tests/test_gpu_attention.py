@@ -252,3 +252,134 @@ def test_rows_past_32_bit_offsets(cuda_dev):
         out = cuda_dev.paged_attention_dev(q, k, v, table, torch.tensor([0, n], dtype=torch.int32, device="cuda"),
                                            torch.tensor([16], dtype=torch.int32, device="cuda"), kvh, kvh, d, page, 0.1)
         assert (out == 3.0).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16_cache", "fp8_cache"])
+def test_more_sequences_than_a_warp_scans_at_once(cuda_dev, fp8):
+    g = np.random.default_rng(8)
+    decode = [(1, int(n)) for n in g.integers(1, 400, 150)]
+    mixed = [(int(n), int(n + m)) for n, m in zip(g.integers(0, 60, 70), g.integers(0, 300, 70))]
+    for lens in (decode, mixed):
+        p = Problem(lens, (8, 2), 128, 16, fp8, seed=len(lens))
+        p.check(p.run(cuda_dev))
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_batches(cuda_dev, seed):
+    g = np.random.default_rng(seed)
+    lens = []
+    for _ in range(int(g.integers(1, 7))):
+        n = int(g.choice([1, 1, g.integers(1, 9), g.integers(1, 200)]))
+        lens.append((n, int(n + g.choice([0, g.integers(0, 40), g.integers(0, 3000)]))))
+    kvh = int(g.choice([1, 2, 3, 8]))
+    p = Problem(lens, (kvh * int(g.choice([1, 2, 5, 8, 16])), kvh), int(g.choice([64, 128, 256])), int(g.choice([1, 7, 16, 64, 512])),
+                bool(g.integers(2)), DTYPES[int(g.integers(2))], seed=seed)
+    p.check(p.run(cuda_dev))
+
+
+@pytest.mark.parametrize("lens", [[(1, 700)], [(90, 700)]], ids=["token", "chunk"])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_fp8_scales_far_apart(cuda_dev, lens, head_dim):
+    """Head rows from 2^-40 to 2^12 in one tile, some of them zero. q is scaled down so that scores stay moderate."""
+    p = Problem(lens, (8, 2), head_dim, 16, True)
+    g = torch.Generator().manual_seed(3)
+    for scales, values in ((p.ks, p.k64), (p.vs, p.v64)):
+        fine = torch.isfinite(scales)
+        factor = torch.exp2(torch.randint(-40, 13, scales.shape, generator=g).float()) * (torch.rand(scales.shape, generator=g) > 0.1)
+        scales[fine] = (scales * factor)[fine]
+        values *= factor[..., None].double()
+    p.q = (p.q.float() * 2.0 ** -10).to(p.q.dtype)
+    # as above, and 2^-10 more: a value's scale under the tile's power of two is rounded to f16 (2^-11) and so is the product
+    p.check(p.run(cuda_dev), bound=2 ** -7 + 2 ** -10 + 2 ** -13)
+
+
+@pytest.mark.parametrize("head_dim", [128, 256])
+@pytest.mark.parametrize("lens", [[(1, 300)], [(40, 300)]], ids=["token", "chunk"])
+def test_fp8_rows_that_held_no_number(cuda_dev, lens, head_dim):
+    """A NaN scale, of K or of V, makes NaN of the rows that see the key and leaves those that do not."""
+    n = lens[0][0]
+    for which in ("ks", "vs"):
+        p = Problem(lens, (4, 2), head_dim, 16, True, behind=0)
+        key = 300 - (n + 1) // 2 if n > 1 else 250      # the second half of a chunk sees it
+        getattr(p, which)[p.rows[0][key], 0] = math.nan
+        out = p.run(cuda_dev).cpu().double()
+        want, most = p.want()
+        sees = torch.arange(n) + 300 - n >= key
+        assert torch.isnan(out[sees][:, :2]).all()
+        err = (out - want).abs()
+        assert (err[~sees] <= 2 ** -6 * most[~sees]).all() and (err[:, 2:] <= 2 ** -6 * most[:, 2:]).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16_cache", "fp8_cache"])
+@pytest.mark.parametrize("lens", [[(1, 300), (2, 900)], [(60, 300), (1, 900)]], ids=["tokens", "chunk"])
+@pytest.mark.parametrize("scale", [0.0, -0.05])
+def test_scales_that_are_not_positive(cuda_dev, lens, fp8, scale):
+    p = Problem(lens, (8, 2), 128, 16, fp8)
+    p.scale = scale
+    p.check(p.run(cuda_dev))
+
+
+def test_infinite_scores_give_nan_in_their_rows_alone(cuda_dev):
+    for lens in ([(1, 300), (1, 300)], [(40, 300), (40, 300)]):
+        p = Problem(lens, (4, 2), 128, 16, behind=0)
+        p.q[0] = math.inf
+        out = p.run(cuda_dev).cpu().double()
+        want, most = p.want()
+        assert torch.isnan(out[0]).all()
+        assert ((out - want).abs()[1:] <= (2 ** -7 + 2 ** -13) * most[1:]).all()
+
+
+def test_two_calls_at_once(cuda_dev):
+    """Two streams, each with a workspace of its own, many times over."""
+    a, b = Problem([(1, 6000), (1, 50)], (16, 2), 128, 64), Problem([(200, 2000)], (16, 2), 128, 64, True)
+    want = [p.run(cuda_dev) for p in (a, b)]
+    torch.cuda.synchronize()
+    args = [([t.cuda() for t in (p.q, p.k, p.v, p.table, p.q_start, p.kv_len)], {k: t.cuda() for k, t in (("k_scales", p.ks), ("v_scales", p.vs)) if t is not None}) for p in (a, b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [torch.full_like(w, 77.0) for w in want]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for p, (x, y), s, o in zip((a, b), args, streams, outs):
+            with torch.cuda.stream(s):
+                cuda_dev.paged_attention_dev(*x, p.qh, p.kvh, p.d, p.page, p.scale, out=o, **y)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+@pytest.mark.parametrize("choice", ["rows", "chunk"])
+def test_sequences_longer_than_the_average_rows(cuda_dev, choice):
+    """A long chunk among many single tokens stays with the kernel for few rows; a lone token in a batch of chunks with the
+    other. Both have to hold whatever the average says."""
+    lens = [(1, 40)] * 60 + [(50, 333)] if choice == "rows" else [(150, 150)] * 4 + [(1, 2000), (2, 3)]
+    for fp8 in (False, True):
+        p = Problem(lens, (16, 2), 128, 16, fp8, seed=9)
+        p.check(p.run(cuda_dev))
+
+
+def test_float8_tensors_and_views_as_caches(cuda_dev):
+    p = Problem([(1, 100)], (4, 2), 128, 16, True, behind=0)
+    plain = p.run(cuda_dev)
+    p.k, p.v = p.k.view(torch.float8_e4m3fn), p.v.view(torch.float8_e4m3fn)
+    assert torch.equal(p.run(cuda_dev), plain)
+
+
+def test_the_binding_refuses_what_does_not_fit(cuda_dev):
+    p = Problem([(1, 100)], (4, 2), 128, 16, True)
+    good = dict(q=p.q, cache_k=p.k, cache_v=p.v, page_table=p.table, q_start=p.q_start, kv_len=p.kv_len)
+    good = {k: t.cuda() for k, t in good.items()}
+    rest = dict(q_heads=4, kv_heads=2, head_dim=128, page_size=16, scale=0.1, k_scales=p.ks.cuda(), v_scales=p.vs.cuda())
+
+    def refused(match, **other):
+        with pytest.raises(clef.ClefError, match=match):
+            cuda_dev.paged_attention_dev(**{**good, **rest, **other})
+
+    refused("kv_len must be .*int32", kv_len=good["kv_len"].long())
+    refused("n_seqs", q_start=good["q_start"][:1])
+    refused("k_scales", k_scales=None)
+    refused("v_scales must be .*float32", v_scales=rest["v_scales"].half())
+    refused("cache_v", cache_v=good["cache_v"][:16])
+    refused("cache_v must be .*uint8", cache_v=good["cache_v"].view(torch.int8))
+    refused("contiguous", cache_k=good["cache_k"].transpose(0, 1))
+    refused("CUDA", page_table=p.table)
+    refused("out must", out=good["q"].float())
+    refused("workspace", workspace=torch.empty(256, dtype=torch.uint8, device="cuda"))

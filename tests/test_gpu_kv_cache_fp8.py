@@ -243,3 +243,92 @@ def test_rows_past_32_bit_offsets(cuda_dev):
     code, scale = recipe(x.float())
     assert torch.equal(got, code.view(torch.float8_e4m3fn).float() * scale[..., None])
     assert not cache[0][1:rows - 1].any()
+
+
+def fp8_cache(rows, kvh, dim):
+    c = torch.zeros(rows, kvh, dim, dtype=torch.uint8, device="cuda")
+    return [c, torch.zeros_like(c), torch.zeros(rows, kvh, device="cuda"), torch.zeros(rows, kvh, device="cuda")]
+
+
+def test_calls_without_a_token(cuda_dev):
+    cache = fp8_cache(8, 2, 64)
+    x, q = torch.empty(0, 2, 64, device="cuda"), torch.empty(0, 4, 64, device="cuda")
+    cos, sin = tables(4, 32)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    cuda_dev.rope_kv_write_fp8_dev(*cache, x, x, cos, sin, 0, 2, 64, 32, cache_map=none)
+    assert cuda_dev.rope_qkv_write_fp8_dev(q, *cache, x, x, cos, sin, 0, 4, 2, 64, 32).shape == q.shape
+    cuda_dev.qk_norm_rope_kv_write_fp8_dev(*cache, x, x, torch.zeros(64, device="cuda"), cos, sin, 0, 2, 64, 32, EPS)
+    k, v = cuda_dev.kv_read_fp8_dev(*cache, 0, 2, 64, row_map=none)
+    assert k.shape == v.shape == (0, 2, 64)
+    torch.cuda.synchronize()
+    assert not any(t.any() for t in cache)
+
+
+def test_reading_past_the_cache_without_a_map(cuda_dev):
+    cache = fp8_cache(5, 2, 64)
+    cache[0].fill_(0x38), cache[1].fill_(0x40), cache[2].fill_(1.0), cache[3].fill_(0.5)
+    k, v = cuda_dev.kv_read_fp8_dev(*cache, 9, 2, 64)
+    assert (k[:5] == 1).all() and (v[:5] == 1).all() and not k[5:].any() and not v[5:].any()
+
+
+def test_a_row_read_many_times(cuda_dev):
+    cache = fp8_cache(70, 3, 96)
+    x, y = (torch.randn(70, 3, 96, generator=gen(11), device="cuda") for _ in range(2))
+    cos, sin = tables(80, 32)
+    cuda_dev.rope_kv_write_fp8_dev(*cache, x, y, cos, sin, 70, 3, 96, 0)
+    at = torch.full((501,), 69, dtype=torch.int32, device="cuda")
+    k, v = cuda_dev.kv_read_fp8_dev(*cache, 501, 3, 96, row_map=at, dtype=torch.float32)
+    for got, want in ((k, x), (v, y)):
+        code, scale = recipe(want[69])
+        assert torch.equal(got, (code.view(torch.float8_e4m3fn).float() * scale[:, None]).expand(501, 3, 96))
+
+
+def test_on_another_stream_behind_its_work(cuda_dev):
+    """Written on a stream that has first to finish filling the inputs, read on the same one."""
+    tokens, kvh, dim = 4000, 2, 128
+    cache = fp8_cache(tokens, kvh, dim)
+    cos, sin = tables(tokens, 64)
+    x = torch.randn(tokens, kvh, dim, generator=gen(12), device="cuda").bfloat16()
+    k = torch.zeros_like(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            k.copy_(-x)
+        k.copy_(x)
+        cuda_dev.rope_kv_write_fp8_dev(*cache, k, k, cos, sin, tokens, kvh, dim, 0)
+        got, _ = cuda_dev.kv_read_fp8_dev(*cache, tokens, kvh, dim, dtype=torch.float32)
+    side.synchronize()
+    code, scale = recipe(x.float())
+    assert torch.equal(got, code.view(torch.float8_e4m3fn).float() * scale[..., None])
+
+
+def test_the_binding_refuses_what_does_not_fit(cuda_dev):
+    cache = fp8_cache(16, 2, 64)
+    k, q = torch.zeros(4, 2, 64, device="cuda"), torch.zeros(4, 8, 64, device="cuda")
+    cos, sin = tables(8, 32)
+    at = torch.arange(4, dtype=torch.int32, device="cuda")
+    w = torch.zeros(64, device="cuda")
+
+    def refused(match, call, *args, **kw):
+        with pytest.raises(clef.ClefError, match=match):
+            call(*args, **kw)
+
+    write, read = cuda_dev.rope_kv_write_fp8_dev, cuda_dev.kv_read_fp8_dev
+    refused("k must", write, *cache, k[:3], k, cos, sin, 4, 2, 64, 32)
+    refused("v must be .*float32", write, *cache, k, k.bfloat16(), cos, sin, 4, 2, 64, 32)
+    refused("cos must", write, *cache, k, k, cos.bfloat16(), sin, 4, 2, 64, 32)
+    refused("sin must", write, *cache, k, k, cos, sin.cpu(), 4, 2, 64, 32)
+    refused("cache_map must be .*int32", write, *cache, k, k, cos, sin, 4, 2, 64, 32, cache_map=at.long())
+    refused("pos_map must", write, *cache, k, k, cos, sin, 4, 2, 64, 32, pos_map=at[:3])
+    refused("E4M3", write, cache[0].float(), *cache[1:], k, k, cos, sin, 4, 2, 64, 32)
+    refused("k_scales must", write, cache[0], cache[1], cache[2][:8], cache[3], k, k, cos, sin, 4, 2, 64, 32)
+    refused("q must be .*float32", cuda_dev.rope_qkv_write_fp8_dev, q.bfloat16(), *cache, k, k, cos, sin, 4, 8, 2, 64, 32)
+    refused("weight must", cuda_dev.qk_norm_rope_kv_write_fp8_dev, *cache, k, k, w[:32], cos, sin, 4, 2, 64, 32, EPS)
+    refused("row_map must", read, *cache, 4, 2, 64, row_map=at.cpu())
+    refused("float32", read, *cache, 4, 2, 64, dtype=torch.float16)
+    a = torch.zeros(4, 64, device="cuda")
+    refused("b must be .*float32", cuda_dev.add_rms_norm_fp8_bf16_dev, a, a.bfloat16(), w, 4, 64, EPS)
+    refused("weight must", cuda_dev.add_rms_norm_fp8_bf16_dev, a, a, w.bfloat16(), 4, 64, EPS)
+    refused("sum_out must", cuda_dev.add_rms_norm_fp8_bf16_dev, a, a, w, 4, 64, EPS, sum_out=a[:2])
+    assert [t.shape for t in cuda_dev.add_rms_norm_fp8_bf16_dev(a[:0], a[:0], w, 0, 64, EPS)] == [(0, 64), (0, 64), (0,), (0, 64)]
