@@ -547,10 +547,12 @@ attn_chunk_kernel(AttnArgs a) {
         constexpr int DEPTH = 3;              // tiles on their way
         uint32_t asked[2] = {0, 0};           // K and V tiles so far
         uint32_t pending = 0, in_flight = 0;  // the slots not handed over yet, four bits each, the oldest on top
-        // place of this thread's nth piece of codes: the upper half of the slot that they are widened into
-        auto code_at = [&](uint8_t* tile, int n) { return tile + Sh::KV_BYTES / 2 + ((n * WARPS + w) * 32 + lane) * 16; };
+        // place of this thread's nth piece of codes: the upper half of what the warp's own rows are widened into
+        auto code_at = [&](uint8_t* tile, int n) {
+            return tile + (D == 64 ? ROWS * 64 : (D / 128 + n / 4) * N * 128) + w * ROWS * 128 + (n % 4 * 32 + lane) * 16;
+        };
         // Hands over the oldest tile on its way, or all of them, once they have arrived. bf16 rows are where they belong. E4M3
-        // codes are widened: each thread takes up the codes that it copied, and when all have, the f16 rows are written over
+        // codes are widened: each lane takes up the codes that it copied, and when its warp has, the f16 rows are written over
         // them. A head row that held no number (its scale is NaN) makes its score NaN, whichever of the two it is, and
         // counts as zeros in V: a row that does not see the key is spared.
         uint32_t widened[2] = {0, 0};
@@ -571,18 +573,22 @@ attn_chunk_kernel(AttnArgs a) {
                     __syncwarp();
                     const float k = sc[0], v = sc[N];
                     // the powers of two that no scale of the warp's rows reaches
-                    auto exponent = [&](float scale) {
+                    auto exponent = [](float scale) {
                         return __reduce_max_sync(kFullMask, scale < INFINITY ? max((int)(__float_as_uint(scale) >> 23) - 126, -100) : -100);
                     };
-                    const int ek = exponent(k), ev = exponent(v);
-                    if (which == 0 && lane == 0) {
-                        s_exponents[nth * 8 + w] = ek, s_exponents[nth * 8 + 4 + w] = ev;
-                        mbar_arrive(&exponents_ready[nth]);
+                    const int ev = exponent(v);
+                    float unit = v * __int_as_float((127 - ev) << 23);
+                    if (which == 0) {
+                        const int ek = exponent(k);
+                        unit = k * __int_as_float((127 - ek) << 23);
+                        if (lane == 0) {
+                            s_exponents[nth * 8 + w] = ek, s_exponents[nth * 8 + 4 + w] = ev;
+                            mbar_arrive(&exponents_ready[nth]);
+                        }
                     }
-                    float unit = which == 0 ? k * __int_as_float((127 - ek) << 23) : v * __int_as_float((127 - ev) << 23);
                     if (!(v < INFINITY)) unit = which == 0 ? __int_as_float(0x7fc00000) : 0.0f;
                     const uint32_t by = pack_f16x2(unit, unit);
-                    asm volatile("bar.sync 3, 128;" ::: "memory");
+                    __syncwarp();   // (every lane has its codes)
 #pragma unroll
                     for (int n = 0; n < ROWS / RPI * (CPR / LPR); ++n) {
                         const int r = w * ROWS + n / (CPR / LPR) * RPI + lane / LPR, ch = 2 * (lane % LPR + n % (CPR / LPR) * LPR);
@@ -606,14 +612,8 @@ attn_chunk_kernel(AttnArgs a) {
         auto fetch = [&](int which, int row32) {
             const uint32_t nth = asked[which]++, slot = which * SLOTS + nth % SLOTS, parity = ((nth / SLOTS) & 1) ^ 1;
             uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
-            // While the slot is still being read, what has been asked for is handed over as it arrives. (FP8: the four warps
-            // decide alike, they widen together.)
-            uint32_t busy = !mbar_try(&empty[slot], parity);
-            if (FP8) {
-                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %0, 0;\n\tbarrier.cta.red.or.pred q, 3, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                             : "+r"(busy)::"memory");
-            }
-            if (busy) {
+            // While the slot is still being read, what has been asked for is handed over as it arrives.
+            if (__any_sync(kFullMask, !mbar_try(&empty[slot], parity))) {
                 hand_over(true);
                 mbar_wait(&empty[slot], parity, gave_up);
             }

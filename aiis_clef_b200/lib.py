@@ -224,8 +224,8 @@ class Device:
 
     def _operand(self, t, what: str, dtype, least: int):
         """Refuses a tensor that a kernel could not read as `least` or more contiguous values of `dtype` on this device."""
-        if t is None or t.dtype != dtype or t.numel() < least or not t.is_contiguous() or not t.is_cuda or (
-                self._index is not None and t.get_device() != self._index):
+        index = torch._C._cuda_getDevice() if self._index is None else self._index
+        if t is None or t.dtype is not dtype or t.numel() < least or not t.is_contiguous() or t.get_device() != index:
             got = "None" if t is None else f"{t.numel()} values of {t.dtype} on {t.device}" + ("" if t.is_contiguous() else ", not contiguous")
             raise ClefError(f"{what} must be a contiguous CUDA tensor of {dtype} on {self.device} with {least} or more values, got {got}")
 
