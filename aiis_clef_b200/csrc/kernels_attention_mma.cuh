@@ -205,11 +205,12 @@ struct ChunkShape {
     static constexpr int SBUF = 2;                        // S buffers per row block
     static constexpr int SLOTS = D == 256 ? 2 : 4;        // buffers of K tiles, and as many of V tiles
     static constexpr int OV = 2;                          // a row tile's beginning and end cost about two units
-    static constexpr int THREADS = 128 * (TILES + 2);     // softmax, producers, products (one warp of the last)
+    static constexpr int PRODUCERS = D == 256 && FP8 ? 2 : 1;   // warpgroups of them; two share the columns
+    static constexpr int THREADS = 128 * (TILES + PRODUCERS + 1);   // softmax, producers, products (one warp of the last)
     // Registers: 512 threads start with 128 each; the softmax, which keeps a row of S, takes what the others leave.
-    static constexpr bool SPLIT = TILES == 2;
-    static constexpr int SOFTMAX_REGS = 184, PRODUCER_REGS = 80, MMA_REGS = 64;
-    static_assert(!SPLIT || TILES * SOFTMAX_REGS + PRODUCER_REGS + MMA_REGS <= 512, "more than the block started with");
+    static constexpr bool SPLIT = THREADS == 512;
+    static constexpr int SOFTMAX_REGS = 184, PRODUCER_REGS = PRODUCERS == 2 ? 104 : 80, MMA_REGS = 64;
+    static_assert(!SPLIT || TILES * SOFTMAX_REGS + PRODUCERS * PRODUCER_REGS + MMA_REGS <= 512, "more than the block started with");
     static constexpr int Q_BYTES = 128 * D * 2;
     static constexpr int KV_BYTES = N * D * 2;
     static constexpr int S_COL = 0;                       // tensor memory columns: S buffers, then O
@@ -217,7 +218,7 @@ struct ChunkShape {
     // FP8: steps whose scales and exponents are kept. Those of step n are asked for when its K tile has a slot, so when the
     // scores of step n - SLOTS are done, which come SBUF steps after weights: no softmax is behind step n - SLOTS - 1 then.
     static constexpr int SCALE_STEPS = 2 * SLOTS;
-    static constexpr int SMEM = 1024 + TILES * Q_BYTES + 2 * SLOTS * KV_BYTES + (FP8 ? SCALE_STEPS * (2 * N + 8) * 4 + TILES * 512 : 0);
+    static constexpr int SMEM = 1024 + TILES * Q_BYTES + 2 * SLOTS * KV_BYTES + (FP8 ? SCALE_STEPS * (2 * N * PRODUCERS + 8) * 4 + TILES * 512 : 0);
 };
 
 // Steps of a segment [begin, end) of key tiles, the same for every role: whole tiles of N keys, none that lies past the
@@ -251,14 +252,14 @@ attn_chunk_kernel(AttnArgs a) {
     uint8_t* s_base = s_raw + ((1024 - (smem_addr(s_raw) & 1023)) & 1023);
     uint8_t* s_q = s_base;
     uint8_t* s_kv = s_q + TILES * Sh::Q_BYTES;
-    float* s_scales = reinterpret_cast<float*>(s_kv + 2 * SLOTS * Sh::KV_BYTES);   // FP8: [SCALE_STEPS][k, v][N]
-    int* s_exponents = reinterpret_cast<int*>(s_scales + Sh::SCALE_STEPS * 2 * N); // FP8: [SCALE_STEPS][k, v][4]
+    float* s_scales = reinterpret_cast<float*>(s_kv + 2 * SLOTS * Sh::KV_BYTES);   // FP8: [PRODUCERS][SCALE_STEPS][k, v][N]
+    int* s_exponents = reinterpret_cast<int*>(s_scales + Sh::PRODUCERS * Sh::SCALE_STEPS * 2 * N);   // FP8: [SCALE_STEPS][k, v][4]
     float* s_q_scale = reinterpret_cast<float*>(s_exponents + Sh::SCALE_STEPS * 8);   // FP8: [TILES][128]
     volatile int* gave_up = &s_gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4;
+    constexpr int kProducerWarp = 4 * TILES, kMmaWarp = kProducerWarp + 4 * Sh::PRODUCERS;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2 * SLOTS; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
+        for (int i = 0; i < 2 * SLOTS; ++i) mbar_init(&full[i], 128 * Sh::PRODUCERS), mbar_init(&empty[i], 1);
         for (int i = 0; i < TILES; ++i) mbar_init(&q_ready[i], 128);
         for (int i = 0; i < TILES * SBUF; ++i) mbar_init(&s_ready[i], 1), mbar_init(&p_ready[i], 128);
         for (int i = 0; i < TILES * 2; ++i) mbar_init(&pv_done[i], 1);
@@ -539,17 +540,21 @@ attn_chunk_kernel(AttnArgs a) {
         constexpr int WARPS = 4, ROWS = N / WARPS;
         if (Sh::SPLIT) set_registers<Sh::PRODUCER_REGS, false>();
         AttnCursor cur = s_cursor;
-        const int w = warp - kProducerWarp;
+        const int w = (warp - kProducerWarp) & 3, half = (warp - kProducerWarp) >> 2;   // rows; of their columns, with two warpgroups
         using CacheT = typename std::conditional<FP8, uint8_t, uint16_t>::type;
         constexpr int CPR = D * (FP8 ? 1 : 2) / 16;       // 16-byte pieces of a cache row
         constexpr int RPI = 32 / (CPR < 8 ? CPR : 8);     // rows a warp touches at once
         constexpr int LPR = 32 / RPI;                     // lanes per row
+        constexpr int NCH = CPR / LPR / Sh::PRODUCERS;    // pieces of a row that a lane takes
+        constexpr int PIECES = ROWS / RPI * NCH;          // of a tile
         constexpr int DEPTH = 3;              // tiles on their way
+        if (FP8) s_scales += half * Sh::SCALE_STEPS * 2 * N;
         uint32_t asked[2] = {0, 0};           // K and V tiles so far
         uint32_t pending = 0, in_flight = 0;  // the slots not handed over yet, four bits each, the oldest on top
         // place of this thread's nth piece of codes: the upper half of what the warp's own rows are widened into
         auto code_at = [&](uint8_t* tile, int n) {
-            return tile + (D == 64 ? ROWS * 64 : (D / 128 + n / 4) * N * 128) + w * ROWS * 128 + (n % 4 * 32 + lane) * 16;
+            const int panel = Sh::PRODUCERS == 2 ? 2 * half + 1 : D / 128 + n / 4;   // (64 columns)
+            return tile + (D == 64 ? ROWS * 64 : panel * N * 128) + w * ROWS * 128 + (n % 4 * 32 + lane) * 16;
         };
         // Hands over the oldest tile on its way, or all of them, once they have arrived. bf16 rows are where they belong. E4M3
         // codes are widened: each lane takes up the codes that it copied, and when its warp has, the f16 rows are written over
@@ -565,9 +570,9 @@ attn_chunk_kernel(AttnArgs a) {
                 const uint32_t slot = pending >> (4 * (in_flight - 1)) & 15;
                 if (FP8) {
                     uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
-                    uint4 code[ROWS / RPI * (CPR / LPR)];
+                    uint4 code[PIECES];
 #pragma unroll
-                    for (int n = 0; n < ROWS / RPI * (CPR / LPR); ++n) code[n] = *reinterpret_cast<const uint4*>(code_at(tile, n));
+                    for (int n = 0; n < PIECES; ++n) code[n] = *reinterpret_cast<const uint4*>(code_at(tile, n));
                     const uint32_t which = slot / SLOTS, nth = widened[which]++ % Sh::SCALE_STEPS;
                     const float* sc = s_scales + nth * 2 * N + w * ROWS + lane % ROWS;   // (as this lane or lane % ROWS copied them)
                     __syncwarp();
@@ -581,7 +586,7 @@ attn_chunk_kernel(AttnArgs a) {
                     if (which == 0) {
                         const int ek = exponent(k);
                         unit = k * __int_as_float((127 - ek) << 23);
-                        if (lane == 0) {
+                        if (lane == 0 && half == 0) {
                             s_exponents[nth * 8 + w] = ek, s_exponents[nth * 8 + 4 + w] = ev;
                             mbar_arrive(&exponents_ready[nth]);
                         }
@@ -590,14 +595,14 @@ attn_chunk_kernel(AttnArgs a) {
                     const uint32_t by = pack_f16x2(unit, unit);
                     __syncwarp();   // (every lane has its codes)
 #pragma unroll
-                    for (int n = 0; n < ROWS / RPI * (CPR / LPR); ++n) {
-                        const int r = w * ROWS + n / (CPR / LPR) * RPI + lane / LPR, ch = 2 * (lane % LPR + n % (CPR / LPR) * LPR);
+                    for (int n = 0; n < PIECES; ++n) {
+                        const int r = w * ROWS + n / NCH * RPI + lane / LPR, ch = 2 * (lane % LPR + (n % NCH + half * NCH) * LPR);
                         uint4 lo, hi;
                         e4m3x4_to_f16(code[n].x, lo.x, lo.y);
                         e4m3x4_to_f16(code[n].y, lo.z, lo.w);
                         e4m3x4_to_f16(code[n].z, hi.x, hi.y);
                         e4m3x4_to_f16(code[n].w, hi.z, hi.w);
-                        const uint32_t f = __shfl_sync(kFullMask, by, n / (CPR / LPR) * RPI + lane / LPR);
+                        const uint32_t f = __shfl_sync(kFullMask, by, n / NCH * RPI + lane / LPR);
                         lo = make_uint4(mul_f16x2(lo.x, f), mul_f16x2(lo.y, f), mul_f16x2(lo.z, f), mul_f16x2(lo.w, f));
                         hi = make_uint4(mul_f16x2(hi.x, f), mul_f16x2(hi.y, f), mul_f16x2(hi.z, f), mul_f16x2(hi.w, f));
                         *reinterpret_cast<uint4*>(tile + tile_offset(r, ch, N)) = lo;
@@ -631,9 +636,9 @@ attn_chunk_kernel(AttnArgs a) {
                 const int row = __shfl_sync(kFullMask, row32, r);
                 const uint8_t* p = reinterpret_cast<const uint8_t*>(src + ((size_t)(row < 0 ? 0 : row) * a.kv_heads + cur.head) * D);
 #pragma unroll
-                for (int j = 0; j < CPR / LPR; ++j) {
-                    const int ch = lane % LPR + j * LPR;
-                    const uint32_t dst = smem_addr(FP8 ? code_at(tile, i * (CPR / LPR) + j) : tile + tile_offset(w * ROWS + r, ch, N));
+                for (int j = 0; j < NCH; ++j) {
+                    const int ch = lane % LPR + (j + half * NCH) * LPR;
+                    const uint32_t dst = smem_addr(FP8 ? code_at(tile, i * NCH + j) : tile + tile_offset(w * ROWS + r, ch, N));
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p + 16 * ch), "r"(row < 0 ? 0 : 16) : "memory");
                 }
             }
