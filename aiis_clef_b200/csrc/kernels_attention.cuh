@@ -265,6 +265,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // and 16 bytes at column 16 r of keys 2c, 2c + 1, 2c + 8, 2c + 9 for O^T, where a byte permute pairs two keys. Warps
 // take 16 keys each, keep their own softmax statistics, and are joined in shared memory at the end of a row tile.
 // The next keys are requested as soon as the registers of the current ones are free.
+// Bound by the cache bytes: one token over 130,712 keys of 2 x 256 in bf16 (268 MB) 51.6 us with the join = 5.2 TB/s, 64 tokens
+// over up to 8,192 keys of 2 x 128 in FP8 (157 MB) 41.5 us = 3.8 TB/s, where the conversions take their part. (Through shared
+// memory with asynchronous copies, three steps deep, the latter took 65 us against 49 then.)
 // An FP8 cache is multiplied in f16, which holds every E4M3 code and which one conversion instruction gives for two
 // codes (bf16 takes five). What else enters the products is brought into f16's range by powers of two: a q row is
 // divided by one so that its largest element is in [1, 2), and weight times value scale by the running maximum of the
