@@ -504,6 +504,8 @@ class Device:
         for t, name in ((page_table, "page_table"), (q_start, "q_start"), (kv_len, "kv_len")):
             self._operand(t, name, torch.int32, 0)
         self._operand(q, "q", q.dtype, 0)
+        if min(q_heads, kv_heads, head_dim, page_size) <= 0:
+            raise ClefError(f"q_heads {q_heads}, kv_heads {kv_heads}, head_dim {head_dim} and page_size {page_size} must be positive")
         n_seqs, total_q = kv_len.numel(), q.numel() // (q_heads * head_dim)
         if page_table.dim() != 2 or page_table.shape[0] != n_seqs or q_start.numel() != n_seqs + 1:
             raise ClefError(f"page_table {tuple(page_table.shape)} and q_start {tuple(q_start.shape)} must be [n_seqs, width] "
@@ -535,6 +537,8 @@ class Device:
         """Checks the four buffers of an FP8 cache against each other; returns its rows."""
         if cache_k.dtype not in (torch.uint8, torch.float8_e4m3fn):
             raise ClefError(f"cache_k must hold E4M3 codes (uint8 or float8_e4m3fn), got {cache_k.dtype}")
+        if kv_heads <= 0 or head_dim <= 0:
+            raise ClefError(f"kv_heads {kv_heads} and head_dim {head_dim} must be positive")
         rows = cache_k.numel() // (kv_heads * head_dim)
         self._operand(cache_k, "cache_k", cache_k.dtype, 0)
         self._operand(cache_v, "cache_v", cache_k.dtype, cache_k.numel())

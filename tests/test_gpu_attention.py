@@ -383,3 +383,41 @@ def test_the_binding_refuses_what_does_not_fit(cuda_dev):
     refused("CUDA", page_table=p.table)
     refused("out must", out=good["q"].float())
     refused("workspace", workspace=torch.empty(256, dtype=torch.uint8, device="cuda"))
+    for name in ("q_heads", "kv_heads", "head_dim", "page_size"):
+        refused("positive", **{name: 0})
+
+
+def test_calls_without_a_token_or_a_sequence(cuda_dev):
+    p = Problem([(1, 100)], (4, 2), 128, 16)
+    k, v = p.k.cuda(), p.v.cuda()
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q = torch.empty(0, 4, 128, dtype=torch.bfloat16, device="cuda")
+    rest = (4, 2, 128, 16, 0.1)
+    assert cuda_dev.paged_attention_dev(q, k, v, p.table.cuda()[:0], zero, none, *rest).shape == q.shape
+    assert cuda_dev.paged_attention_dev(q, k, v, p.table.cuda(), torch.zeros(2, dtype=torch.int32, device="cuda"), p.kv_len.cuda(), *rest).shape == q.shape
+    out = torch.full((3, 4, 128), 5.0, dtype=torch.bfloat16, device="cuda")      # rows, but no sequence to own them
+    cuda_dev.paged_attention_dev(out.clone(), k, v, p.table.cuda()[:0], zero, none, *rest, out=out)
+    torch.cuda.synchronize()
+    assert (out == 5).all()
+
+
+def test_replayed_with_other_lengths(cuda_dev):
+    """A captured call, replayed after its lengths, pages and tokens were changed in place, against a plain call."""
+    big = Problem([(5, 900), (60, 700), (1, 1200)], (8, 2), 128, 16, seed=4)
+    small = Problem([(30, 901), (2, 697), (34, 1190)], (8, 2), 128, 16, seed=5)
+    assert big.table.shape == small.table.shape and big.q.shape == small.q.shape and big.k.shape == small.k.shape
+    at = [t.cuda() for t in (big.q, big.k, big.v, big.table, big.q_start, big.kv_len)]
+    out = torch.full_like(at[0], 77.0)
+    call = lambda: cuda_dev.paged_attention_dev(*at, 8, 2, 128, 16, big.scale, out=out)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for p in (small, big):
+        for dst, src in zip(at, (p.q, p.k, p.v, p.table, p.q_start, p.kv_len)):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        p.check(out)
