@@ -546,12 +546,14 @@ class Device:
         self._operand(v_scales, "v_scales", torch.float32, rows * kv_heads)
         return rows
 
-    def _kv_write_inputs(self, k, v, cos, sin, tokens: int, kv_heads: int, head_dim: int, seq_start, pos_base, pos_map, cache_map,
-                         cache_len):
-        """Checks what the three writers of an FP8 cache read beside it."""
+    def _kv_write_inputs(self, k, v, cos, sin, tokens: int, kv_heads: int, head_dim: int, rotary_dim: int, seq_start, pos_base,
+                         pos_map, cache_map, cache_len):
+        """Checks what the three writers of an FP8 cache read beside it. Positions on the device are the caller's to keep inside
+        the tables; those that a call without them stands for, 0 .. tokens - 1, are checked here."""
         self._operand(k, "k", k.dtype, tokens * kv_heads * head_dim)
         self._operand(v, "v", k.dtype, tokens * kv_heads * head_dim)
-        self._operand(cos, "cos", torch.float32, 0)
+        plain = seq_start is None and pos_base is None and pos_map is None
+        self._operand(cos, "cos", torch.float32, (tokens if plain else min(tokens, 1)) * rotary_dim)
         self._operand(sin, "sin", torch.float32, cos.numel())
         for t, name, least in ((seq_start, "seq_start", 1), (pos_base, "pos_base", 1), (pos_map, "pos_map", tokens),
                                (cache_map, "cache_map", tokens), (cache_len, "cache_len", 1)):
@@ -562,7 +564,8 @@ class Device:
                               head_dim: int, rotary_dim: int, seq_start=None, pos_base=None, pos_map=None, cache_map=None,
                               cache_len=None):
         """rope_apply_dev on k, then k and v into the FP8 caches and their scales (in place), one launch."""
-        self._kv_write_inputs(k, v, cos, sin, tokens, kv_heads, head_dim, seq_start, pos_base, pos_map, cache_map, cache_len)
+        self._kv_write_inputs(k, v, cos, sin, tokens, kv_heads, head_dim, rotary_dim, seq_start, pos_base, pos_map,
+                              cache_map, cache_len)
         rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
         self._call("clef_rope_kv_write_fp8", cache_k.data_ptr(), cache_v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                    k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), tokens, kv_heads, head_dim, rotary_dim,
@@ -572,7 +575,8 @@ class Device:
                                kv_heads: int, head_dim: int, rotary_dim: int, seq_start=None, pos_base=None, pos_map=None,
                                cache_map=None, cache_len=None):
         """rope_apply_dev on q (returned) and rope_kv_write_fp8_dev on k, v (caches written in place), one launch."""
-        self._kv_write_inputs(k, v, cos, sin, tokens, kv_heads, head_dim, seq_start, pos_base, pos_map, cache_map, cache_len)
+        self._kv_write_inputs(k, v, cos, sin, tokens, kv_heads, head_dim, rotary_dim, seq_start, pos_base, pos_map,
+                              cache_map, cache_len)
         self._operand(q, "q", k.dtype, tokens * q_heads * head_dim)
         rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
         q_out = self._like(q, (tokens, q_heads, head_dim), q.dtype)
@@ -586,7 +590,8 @@ class Device:
                                       kv_heads: int, head_dim: int, rotary_dim: int, eps: float, seq_start=None,
                                       pos_base=None, pos_map=None, cache_map=None, cache_len=None):
         """qk_norm_rope_dev on k_raw, then k and v into the FP8 caches and their scales (in place), one launch."""
-        self._kv_write_inputs(k_raw, v, cos, sin, tokens, kv_heads, head_dim, seq_start, pos_base, pos_map, cache_map, cache_len)
+        self._kv_write_inputs(k_raw, v, cos, sin, tokens, kv_heads, head_dim, rotary_dim, seq_start, pos_base, pos_map,
+                              cache_map, cache_len)
         self._operand(weight, "weight", torch.float32, head_dim)
         rows = self._fp8_cache(cache_k, cache_v, k_scales, v_scales, kv_heads, head_dim)
         self._call("clef_qk_norm_rope_kv_write_fp8", cache_k.data_ptr(), cache_v.data_ptr(), k_scales.data_ptr(),

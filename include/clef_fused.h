@@ -281,6 +281,9 @@ int clef_paged_attention(clef_stream_t stream, void* out, const void* q, const v
  * clef_rope_kv_write_fp8, clef_rope_qkv_write_fp8 and clef_qk_norm_rope_kv_write_fp8 take the arguments of the bf16
  * forms above (positions, cache_map, cache_len) with the scales beside the caches, and cache_rows: a token whose row is
  * outside 0 .. cache_rows - 1 (a padding token, mapped to -1) is not written. The rows of the others must be distinct.
+ * Positions must lie inside the tables, which have one row at least, except those of padding tokens: any position serves
+ * where only k and v are written; in the form with q, whose rows are rotated for padding tokens too, a negative one is
+ * taken as 0.
  * One launch each. head_dim % 8 == 0 and at most 256, rotary_dim % 16 == 0. */
 int clef_rope_kv_write_fp8(clef_stream_t stream, uint8_t* cache_k, uint8_t* cache_v, float* k_scales, float* v_scales,
                            const void* k, const void* v, const float* cos_table, const float* sin_table, int tokens,
