@@ -401,6 +401,10 @@ attn_chunk_kernel(AttnArgs a) {
                         // weight times 2^e stays within f16 (O and the sum are divided by the same)
                         v_exponent = max(v_exponent, v[g]);
                     }
+                    // Weights of a group so far below the reference are 0 in f16 whatever its exponent; they are taken 2^40 below
+                    // it, where f32 still holds them for the sum. (Groups without a value have an exponent of -100.)
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g) e_v[g] = max(e_v[g], v_exponent - 40);
                 }
                 mbar_wait_warp(&s_ready[t * SBUF + buf], s_parity, gave_up);
                 tc_fence_after();
