@@ -271,7 +271,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // An FP8 cache is multiplied in f16, which holds every E4M3 code and which one conversion instruction gives for two
 // codes (bf16 takes five). What else enters the products is brought into f16's range by powers of two: a q row is
 // divided by one so that its largest element is in [1, 2), and weight times value scale by the running maximum of the
-// value scales; both are multiplied back in f32. f16 then rounds finer than bf16 (2^-11), down to 2^-14 of the maximum.
+// value scales that the ROW sees; both are multiplied back in f32. f16 then rounds finer than bf16 (2^-11), down to 2^-14 of
+// the maximum.
 // ---------------------------------------------------------------------------------------------
 template <typename T, bool FP8, int D, int NT>
 __global__ void __launch_bounds__(kAttnThreads, (D == 256 || NT > 1 || !FP8) ? 1 : 2)
@@ -354,7 +355,7 @@ attn_rows_kernel(AttnArgs a) {
         uint32_t qf[NT][D / 16][2];
         int lim[NT][2];     // keys seen by rows 2c and 2c + 1 of each 8
         float back[NT][2];  // FP8: score scale of those rows
-        float v_most = 0.0f;   // FP8: a power of two no value scale so far is above; o is that much too small
+        float v_most[NT][2];   // FP8: a power of two no value scale so far that those rows see is above; o is that much too small
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int x = row0 + nt * 8 + r;
@@ -409,6 +410,7 @@ attn_rows_kernel(AttnArgs a) {
             }
             m[nt][0] = m[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.0f;
+            v_most[nt][0] = v_most[nt][1] = 0.0f;
         }
         for (int tile = begin; tile < end; ++tile) {
             const int t0 = tile * kAttnKeys + warp * 16;
@@ -439,26 +441,49 @@ attn_rows_kernel(AttnArgs a) {
             }
             float ks0 = 0.0f, ks1 = 0.0f, vs0 = 0.0f, vs1 = 0.0f;
             if (FP8) {
-                ks0 = ks[0], ks1 = ks[1];
-                const float most = fmaxf(vs[0], vs[1]);
-                if (__any_sync(kFullMask, most > v_most)) {
-                    float now = most;
+                ks0 = ks[0], ks1 = ks[1], vs0 = vs[0], vs1 = vs[1];
+                float most[NT][2];
+                bool raised = false, apart = false;   // apart: rows that see a part of these keys
 #pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) now = fmaxf(now, __shfl_xor_sync(kFullMask, now, off));
-                    now = __uint_as_float((__float_as_uint(fmaxf(now, 1e-37f)) + 0x007fffffu) & 0x7f800000u);   // up to a power of two
-                    const float fix = v_most / now;   // 0 at first
-                    v_most = now;
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        most[nt][e] = fmaxf(t0 + r < lim[nt][e] ? vs0 : 0.0f, t0 + r + 8 < lim[nt][e] ? vs1 : 0.0f);
+                        raised |= most[nt][e] > v_most[nt][e];
+                        apart |= t0 + 16 > lim[nt][e] && lim[nt][e] > 0;
+                    }
+                }
+                if (__any_sync(kFullMask, raised)) {
+                    const bool one = !__any_sync(kFullMask, apart);   // one maximum for all rows, or one for each
+                    float all = fmaxf(fmaxf(vs0, vs1), 0.0f);
+                    if (one) all = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(all)));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
+                        float fix[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float now = all;
+                            if (!one) {
+                                now = most[nt][e];
+#pragma unroll
+                                for (int off = 4; off < 32; off <<= 1) now = fmaxf(now, __shfl_xor_sync(kFullMask, now, off));
+                            }
+                            // up to a power of two, kept where its reciprocal is a normal number too
+                            now = __uint_as_float((__float_as_uint(fmaxf(now, 1e-37f)) + 0x007fffffu) & 0x7f800000u);
+                            now = fmaxf(fminf(now, 0x1p126f), v_most[nt][e]);
+                            fix[e] = v_most[nt][e] * __uint_as_float(0x7f000000u - __float_as_uint(now));   // 0 at first
+                            v_most[nt][e] = now;
+                        }
 #pragma unroll
                         for (int b = 0; b < VL; ++b) {
 #pragma unroll
-                            for (int i = 0; i < VCH / 2; ++i) o[nt][b][i][0] *= fix, o[nt][b][i][1] *= fix, o[nt][b][i][2] *= fix, o[nt][b][i][3] *= fix;
+                            for (int i = 0; i < VCH / 2; ++i) {
+                                o[nt][b][i][0] *= fix[0], o[nt][b][i][1] *= fix[1];
+                                o[nt][b][i][2] *= fix[0], o[nt][b][i][3] *= fix[1];
+                            }
                         }
                     }
                 }
-                const float inv = v_most > 0.0f ? 1.0f / v_most : 0.0f;
-                vs0 = vs[0] * inv, vs1 = vs[1] * inv;
             }
             const bool more = tile + 1 < end;
             if (more) load_k(row16);
@@ -509,8 +534,9 @@ attn_rows_kernel(AttnArgs a) {
                 if (FP8) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        p[e] = t0 + r < lim[nt][e] ? p[e] * vs0 : 0.0f;
-                        p[2 + e] = t0 + r + 8 < lim[nt][e] ? p[2 + e] * vs1 : 0.0f;
+                        const float inv = __uint_as_float(0x7f000000u - __float_as_uint(v_most[nt][e]));   // 1 / v_most, exactly
+                        p[e] = t0 + r < lim[nt][e] ? p[e] * (vs0 * inv) : 0.0f;
+                        p[2 + e] = t0 + r + 8 < lim[nt][e] ? p[2 + e] * (vs1 * inv) : 0.0f;
                     }
                 }
                 pf[nt][0] = transpose8x8(FP8 ? pack_f16x2(p[0], p[1]) : pack_bf16x2(p[0], p[1]));
@@ -561,7 +587,7 @@ attn_rows_kernel(AttnArgs a) {
                 for (int b = 0; b < VL; ++b) {
 #pragma unroll
                     for (int i = 0; i < VCH / 2; ++i) {
-                        const float by = FP8 ? v_most : 1.0f;
+                        const float by = FP8 ? v_most[nt][e] : 1.0f;
                         *reinterpret_cast<float2*>(dst + 8 * VCH * b + 2 * i) = make_float2(o[nt][b][i][e] * by, o[nt][b][i][2 + e] * by);
                     }
                 }

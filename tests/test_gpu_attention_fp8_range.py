@@ -1,4 +1,5 @@
-"""clef_paged_attention over FP8 caches whose scales lie far apart: keys without a value still weigh beside large ones.
+"""clef_paged_attention over FP8 caches whose scales lie far apart: what a row of the output is must not depend on keys that the
+causal mask hides from it, and keys without a value still weigh.
 
 Tolerances, relative to the largest |v| among the keys that the ROW sees (an output is a convex combination of those): the weight
 times the value scale is rounded to f16 (2^-11) beside a value rounded to f16 at most twice (2^-11 each), the output to bf16
@@ -37,6 +38,39 @@ def check(p, out):
     assert (err <= BOUND * most).all(), f"off by {worst:.3g} of the largest value that the row sees, allowed {BOUND:.3g}"
 
 
+# the last tokens' 16 keys begin inside and at a tile's end
+BATCHES = {"two_tokens": [(2, 60)], "four_tokens": [(4, 64), (4, 140)], "five_tokens": [(5, 33)]}
+
+
+@pytest.mark.parametrize("power", [6, 12, 16, 20, 24, 40])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("batch", list(BATCHES))
+def test_a_late_value_does_not_cost_earlier_rows_precision(cuda_dev, batch, head_dim, power):
+    """The last key of each sequence has values 2^power larger: only the last row sees it."""
+    p = Problem(BATCHES[batch], (8, 2), head_dim, 16, True, seed=power)
+    for rows in p.rows:
+        p.vs[rows[-1]] *= 2.0 ** power
+        p.v64[rows[-1]] *= 2.0 ** power
+    check(p, p.run(cuda_dev))
+
+
+@pytest.mark.parametrize("power", [6, 16, 24, 40])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("batch", list(BATCHES))
+def test_a_late_key_does_not_cost_earlier_rows_precision(cuda_dev, batch, head_dim, power):
+    """The last key itself is 2^power larger; the row that sees it has scores to match and is left out."""
+    p = Problem(BATCHES[batch], (8, 2), head_dim, 16, True, seed=power)
+    last = []
+    for s, rows in enumerate(p.rows):
+        p.ks[rows[-1]] *= 2.0 ** power
+        p.k64[rows[-1]] *= 2.0 ** power
+        last.append(sum(n for n, _ in p.lens[:s + 1]) - 1)
+    out = p.run(cuda_dev)
+    want, _ = p.want()
+    out[last] = want[last].to(out.dtype).cuda()
+    check(p, out)
+
+
 @pytest.mark.parametrize("power", [0, 20, 40, 100])
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
 @pytest.mark.parametrize("lens", [[(1, 160)], [(40, 160)]], ids=["token", "chunk"])
@@ -47,4 +81,18 @@ def test_keys_without_a_value_beside_large_ones_still_weigh(cuda_dev, lens, head
         rows, factor = p.rows[0][start:start + 16], 0.0 if start % 32 else 2.0 ** power
         p.vs[rows] *= factor
         p.v64[rows] *= factor
+    check(p, p.run(cuda_dev))
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(1, 150)], [(3, 150)]], ids=["token", "tokens"])
+def test_every_key_on_a_scale_of_its_own(cuda_dev, lens, head_dim):
+    """Scales of K and V that rise along the sequence from 2^-20 to 2^20, up and down by 2^6 from key to key."""
+    p = Problem(lens, (8, 2), head_dim, 16, True, seed=head_dim)
+    t = torch.arange(150)
+    rise = torch.exp2((t * 40 // 150 - 20 + 6 * (t % 2)).float())
+    for scales, values in ((p.ks, p.k64), (p.vs, p.v64)):
+        scales[p.rows[0]] *= rise[:, None]
+        values[p.rows[0]] *= rise[:, None, None].double()
+    p.q = (p.q.float() * 2.0 ** -26).to(p.q.dtype)        # scores stay moderate
     check(p, p.run(cuda_dev))
