@@ -12,7 +12,10 @@
 // An FP8 cache is multiplied in f16: the 16 rows that a producer warp widens are brought under one power of two,
 // code * (scale / 2^e) in f16 (2^-11 per value, next to the codes' own 2^-4), which the softmax multiplies back: 2^e of K
 // with the score scale of those 16 keys, 2^e of V with the reference of their weights. (With scaled rows
-// as bf16 the outputs' error was 0.0048 of their size, 0.0020 so.)
+// as bf16 the outputs' error was 0.0048 of their size, 0.0020 so.) In the last steps of a row tile, where the mask hides some
+// keys from some row, what is hidden must not decide how finely the rest is held: rows whose scales lie further apart than
+// 2^13 (K) or 2^4 (V) are multiplied as bare codes there, and the softmax takes their scales one by one, those of K with the
+// scores, those of V, against the largest that its row sees, with the weights.
 //
 // Measured (16 + 2 heads of 128, pages of 64): 8,192 causal tokens 291 to 303 us = 945 to 907 TFLOP/s; 2,011 tokens after
 // 30,757 in FP8 605 us = 865 TFLOP/s; head_dim 256, FP8, 2,048 tokens after 6,144: 375 us. What bounds it: the softmax's
@@ -138,6 +141,22 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const float* v) {
                  "r"(addr)
                  : "memory");
 }
+__device__ __forceinline__ void tc_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tc_ld8(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
+                 : "memory");
+}
 __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]),
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
@@ -204,6 +223,12 @@ __device__ __forceinline__ void set_registers() {
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
+// The power of two that a scale lies below (NaN and infinity: none, -100), kept where it and its reciprocal are normal numbers.
+__device__ __forceinline__ int scale_exponent(float scale) {
+    return scale < INFINITY ? min(max((int)(__float_as_uint(scale) >> 23) - 126, -100), 126) : -100;
+}
+constexpr int kBareCodes = 0x1000;   // in place of the exponent of 16 keys that are multiplied as bare codes
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -243,6 +268,12 @@ __device__ __forceinline__ void chunk_steps(const AttnArgs& a, const AttnCursor&
     keys = attn_visible(a, c.span, min((c.tile + 1) * Sh::R, c.span.n * a.group));
     from = begin * PER;
     to = max(from + 1, min(end * PER, (keys + Sh::N - 1) / Sh::N));
+}
+
+// The first step of a row tile in which some row does not see every key.
+template <int N>
+__device__ __forceinline__ int chunk_hides_from(const AttnArgs& a, const AttnSeq& span, int row0) {
+    return attn_visible(a, span, row0 + 1) / N;
 }
 
 // The 128 threads of row block t.
@@ -372,16 +403,13 @@ attn_chunk_kernel(AttnArgs a) {
             const int lim = row0 + x < rows ? attn_visible(a, span, row0 + x + 1) : 0x7fffffff;
             const bool warp_live = row0 + (x & ~31) < rows;
             float m = -INFINITY, l = 0.0f;
-#pragma unroll 1
-            for (int step = from; step < to; ++step, ++steps_done) {
+            // One step, all keys of which every live row of the row tile sees, or not (compiled twice: a test per pair of keys
+            // would cost more than the pair).
+            auto one_step = [&](int step, auto with_hidden) {
+                constexpr bool HIDES = decltype(with_hidden)::value;
                 const int buf = SBUF == 1 ? 0 : (steps_done & 1);
                 const uint32_t s_addr = tmem + lanes + Sh::S_COL + (t * SBUF + buf) * N;
                 const uint32_t s_parity = (SBUF == 1 ? steps_done : steps_done >> 1) & 1;
-                if (!warp_live) {
-                    mbar_wait_warp(&s_ready[t * SBUF + buf], s_parity, gave_up);
-                    mbar_arrive(&p_ready[t * SBUF + buf]);
-                    continue;
-                }
                 const uint32_t nth_kv = kv_first + (step - from);
                 if (FP8) mbar_wait_warp(&exponents_ready[nth_kv % Sh::SCALE_STEPS], (nth_kv / Sh::SCALE_STEPS) & 1, gave_up);
                 // score scale and weight exponent of each 16 keys
@@ -389,32 +417,61 @@ attn_chunk_kernel(AttnArgs a) {
                 float by[GROUPS];
                 int e_v[GROUPS];
                 by[0] = scale, e_v[0] = 0;
+                const int base = step * N;
+                const int* exponents = s_exponents + nth_kv % Sh::SCALE_STEPS * 8;       // of K, then of V
+                const float* scales = s_scales + nth_kv % Sh::SCALE_STEPS * 2 * N;       // likewise
+                bool bare = false;
                 if (FP8) {
-                    const int4 ek = *reinterpret_cast<const int4*>(s_exponents + nth_kv % Sh::SCALE_STEPS * 8);
-                    const int4 ev = *reinterpret_cast<const int4*>(s_exponents + nth_kv % Sh::SCALE_STEPS * 8 + 4);
+                    const int4 ek = *reinterpret_cast<const int4*>(exponents);
+                    const int4 ev = *reinterpret_cast<const int4*>(exponents + 4);
                     const int k[4] = {ek.x, ek.y, ek.z, ek.w}, v[4] = {ev.x, ev.y, ev.z, ev.w};
 #pragma unroll
                     for (int g = 0; g < GROUPS; ++g) {
-                        by[g] = scale * __int_as_float((127 + k[g]) << 23);
+                        by[g] = scale * __uint_as_float((uint32_t)(127 + k[g]) << 23);   // (2^0 for bare codes)
                         e_v[g] = v[g];
                         // the reference that weights are taken against is raised by the largest exponent of V so far, so that
-                        // weight times 2^e stays within f16 (O and the sum are divided by the same)
-                        v_exponent = max(v_exponent, v[g]);
+                        // weight times 2^e stays within f16 (O and the sum are divided by the same); groups that the row does
+                        // not see have no part in it
+                        if (!HIDES || (base + 16 * g < lim && v[g] != kBareCodes)) v_exponent = max(v_exponent, v[g]);
+                    }
+                    if (HIDES) {
+                        bare = k[0] == kBareCodes || k[1] == kBareCodes || k[2] == kBareCodes || k[3] == kBareCodes ||
+                               v[0] == kBareCodes || v[1] == kBareCodes || v[2] == kBareCodes || v[3] == kBareCodes;
+                        if (bare) {
+#pragma unroll 1
+                            for (int i = 0; i < N; ++i) {
+                                const bool own = exponents[4 + i / 16] == kBareCodes && base + i < lim;
+                                v_exponent = own ? max(v_exponent, scale_exponent(scales[N + i])) : v_exponent;
+                            }
+                            __syncwarp();
+                        }
                     }
                     // Weights of a group so far below the reference are 0 in f16 whatever its exponent; they are taken 2^40 below
-                    // it, where f32 still holds them for the sum. (Groups without a value have an exponent of -100.)
+                    // it, where f32 still holds them for the sum. (Groups without a value have an exponent of -100.) Those of bare
+                    // codes are taken against the reference itself.
 #pragma unroll
-                    for (int g = 0; g < GROUPS; ++g) e_v[g] = max(e_v[g], v_exponent - 40);
+                    for (int g = 0; g < GROUPS; ++g) e_v[g] = HIDES && e_v[g] == kBareCodes ? v_exponent : max(e_v[g], v_exponent - 40);
                 }
                 mbar_wait_warp(&s_ready[t * SBUF + buf], s_parity, gave_up);
                 tc_fence_after();
+                if (FP8 && HIDES && bare) {   // the scores of bare codes of K take their scales
+#pragma unroll 1
+                    for (int g = 0; g < N / 16; ++g) {
+                        if (exponents[g] != kBareCodes) continue;
+                        uint32_t x[16];
+                        tc_ld16(s_addr + 16 * g, x);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * scales[16 * g + i]);
+                        tc_st16(s_addr + 16 * g, x);
+                    }
+                    tc_wait_st();
+                }
                 f32x2 s[N / 2];
 #pragma unroll
                 for (int c = 0; c < N; c += 32) tc_ld32(s_addr + c, reinterpret_cast<float*>(s + c / 2));
                 tc_wait_ld();
-                const int base = step * N;
-                const bool edge = __any_sync(kFullMask, base + N > lim);   // some keys of the step are hidden from some row
-                if (edge) {
+                if (HIDES) {
 #pragma unroll
                     for (int i = 0; i < N / 2; ++i) {
                         s[i].x = base + 2 * i < lim ? s[i].x : -INFINITY;
@@ -457,38 +514,66 @@ attn_chunk_kernel(AttnArgs a) {
                 }
                 const float ref = m == -INFINITY ? 0.0f : -m;
                 f32x2 sums[GROUPS][2];
-                auto weights = [&](auto with_edge) {   // (compiled twice: a test per pair would cost more than the pair)
-                    constexpr bool EDGE = decltype(with_edge)::value;
 #pragma unroll
-                    for (int c = 0; c < N / 2; c += 16) {
-                        uint32_t p[16];
+                for (int c = 0; c < N / 2; c += 16) {
+                    uint32_t p[16];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int g = FP8 ? (c + i) / 8 : 0;
-                            f32x2 e = f2_fma(s[c + i], f2_splat(by[g]), f2_splat(FP8 ? ref + (float)e_v[g] : ref));
-                            if (EDGE) {   // hidden keys: a weight of exactly 0 (and scale 0 would make NaN of their -inf)
-                                e.x = base + 2 * (c + i) < lim ? fast_exp2(e.x) : 0.0f;
-                                e.y = base + 2 * (c + i) + 1 < lim ? fast_exp2(e.y) : 0.0f;
-                            } else {
-                                e = f2_pack(fast_exp2(e.x), fast_exp2(e.y));
-                            }
-                            const bool opens = FP8 ? (c + i) % 8 < 2 : c + i < 2;
-                            sums[g][i % 2] = opens ? e : f2_add(sums[g][i % 2], e);
-                            p[i] = FP8 ? pack_f16x2(e.x, e.y) : pack_bf16x2(e.x, e.y);
+                    for (int i = 0; i < 16; ++i) {
+                        const int g = FP8 ? (c + i) / 8 : 0;
+                        f32x2 e = f2_fma(s[c + i], f2_splat(by[g]), f2_splat(FP8 ? ref + (float)e_v[g] : ref));
+                        if (HIDES) {   // hidden keys: a weight of exactly 0 (and scale 0 would make NaN of their -inf)
+                            e.x = base + 2 * (c + i) < lim ? fast_exp2(e.x) : 0.0f;
+                            e.y = base + 2 * (c + i) + 1 < lim ? fast_exp2(e.y) : 0.0f;
+                        } else {
+                            e = f2_pack(fast_exp2(e.x), fast_exp2(e.y));
                         }
-                        tc_st16(s_addr + c, p);   // over columns of S that are in registers
+                        const bool opens = FP8 ? (c + i) % 8 < 2 : c + i < 2;
+                        sums[g][i % 2] = opens ? e : f2_add(sums[g][i % 2], e);
+                        p[i] = FP8 ? pack_f16x2(e.x, e.y) : pack_bf16x2(e.x, e.y);
                     }
-                };
-                if (edge) weights(std::true_type{});
-                else weights(std::false_type{});
+                    tc_st16(s_addr + c, p);   // over columns of S that are in registers
+                }
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
                     const f32x2 sum = f2_add(sums[g][0], sums[g][1]);
                     l = FP8 ? fmaf(sum.x + sum.y, __int_as_float((127 - e_v[g]) << 23), l) : l + (sum.x + sum.y);
                 }
                 tc_wait_st();
+                if (FP8 && HIDES && bare) {   // the weights of bare codes of V take theirs, against the largest that the row sees
+                    const float down = __int_as_float((127 - v_exponent) << 23);
+#pragma unroll 1
+                    for (int g = 0; g < N / 16; ++g) {
+                        if (exponents[4 + g] != kBareCodes) continue;
+                        uint32_t p[8];
+                        tc_ld8(s_addr + 8 * g, p);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {   // (hidden keys have weights of 0 and may have larger scales)
+                            const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&p[i]));
+                            const float* v = scales + N + 16 * g + 2 * i;
+                            p[i] = pack_f16x2(w.x * fminf(v[0] * down, 1.0f), w.y * fminf(v[1] * down, 1.0f));
+                        }
+                        tc_st8(s_addr + 8 * g, p);
+                    }
+                    tc_wait_st();
+                }
                 tc_fence_before();
                 mbar_arrive(&p_ready[t * SBUF + buf]);
+                ++steps_done;
+            };
+            if (warp_live) {
+                const int hides_from = min(to, max(from, chunk_hides_from<N>(a, span, cur.tile * R)));
+#pragma unroll 1
+                for (int step = from; step < hides_from; ++step) one_step(step, std::false_type{});
+#pragma unroll 1
+                for (int step = hides_from; step < to; ++step) one_step(step, std::true_type{});
+            } else {
+#pragma unroll 1
+                for (int step = from; step < to; ++step, ++steps_done) {
+                    const int at = t * SBUF + (SBUF == 1 ? 0 : (steps_done & 1));
+                    mbar_wait_warp(&s_ready[at], (SBUF == 1 ? steps_done : steps_done >> 1) & 1, gave_up);
+                    mbar_arrive(&p_ready[at]);
+                }
             }
             wait_outputs(steps_done - 1);
             const bool whole = begin == 0 && end == cur.keys;
@@ -567,7 +652,9 @@ attn_chunk_kernel(AttnArgs a) {
         constexpr int DEPTH = 3;              // tiles on their way
         if (FP8) s_scales += half * Sh::SCALE_STEPS * 2 * N;
         uint32_t asked[2] = {0, 0};           // K and V tiles so far
-        uint32_t pending = 0, in_flight = 0;  // the slots not handed over yet, four bits each, the oldest on top
+        // the slots not handed over yet, four bits each, the oldest on top; the fourth: the step hides keys from some row
+        uint32_t pending = 0, in_flight = 0;
+        static_assert(2 * SLOTS <= 8, "a slot number takes three bits");
         // place of this thread's nth piece of codes: the upper half of what the warp's own rows are widened into
         auto code_at = [&](uint8_t* tile, int n) {
             const int panel = Sh::PRODUCERS == 2 ? 2 * half + 1 : D / 128 + n / 4;   // (64 columns)
@@ -575,39 +662,45 @@ attn_chunk_kernel(AttnArgs a) {
         };
         // Hands over the oldest tile on its way, or all of them, once they have arrived. bf16 rows are where they belong. E4M3
         // codes are widened: each lane takes up the codes that it copied, and when its warp has, the f16 rows are written over
-        // them. A head row that held no number (its scale is NaN) makes its score NaN, whichever of the two it is, and
-        // counts as zeros in V: a row that does not see the key is spared.
-        uint32_t widened[2] = {0, 0};
+        // them, or the bare codes. A head row that held no number (its scale is NaN) makes its score NaN, whichever of the two
+        // it is, and counts as zeros in V: a row that does not see the key is spared.
+        uint32_t widened_k = 0, widened_v = 0;
         auto hand_over = [&](bool all) {
             if (in_flight == 0) return;
             if (all) asm volatile("cp.async.wait_group 0;" ::: "memory");
             else asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
             if (!FP8) async_proxy_fence();
             for (; in_flight > (all ? 0u : DEPTH - 1u); --in_flight) {
-                const uint32_t slot = pending >> (4 * (in_flight - 1)) & 15;
+                const uint32_t entry = pending >> (4 * (in_flight - 1)), slot = entry & 7;
                 if (FP8) {
                     uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
                     uint4 code[PIECES];
 #pragma unroll
                     for (int n = 0; n < PIECES; ++n) code[n] = *reinterpret_cast<const uint4*>(code_at(tile, n));
-                    const uint32_t which = slot / SLOTS, nth = widened[which]++ % Sh::SCALE_STEPS;
-                    const float* sc = s_scales + nth * 2 * N + w * ROWS + lane % ROWS;   // (as this lane or lane % ROWS copied them)
+                    const uint32_t which = slot / SLOTS, nth = (which == 0 ? widened_k++ : widened_v++) % Sh::SCALE_STEPS;
+                    float* sc = s_scales + nth * 2 * N + w * ROWS + lane % ROWS;   // (as this lane or lane % ROWS copied them)
                     __syncwarp();
                     const float k = sc[0], v = sc[N];
                     // the powers of two that no scale of the warp's rows reaches
-                    auto exponent = [](float scale) {
-                        return __reduce_max_sync(kFullMask, scale < INFINITY ? max((int)(__float_as_uint(scale) >> 23) - 126, -100) : -100);
-                    };
-                    const int ev = exponent(v);
-                    float unit = v * __int_as_float((127 - ev) << 23);
-                    if (which == 0) {
-                        const int ek = exponent(k);
-                        unit = k * __int_as_float((127 - ek) << 23);
-                        if (lane == 0 && half == 0) {
-                            s_exponents[nth * 8 + w] = ek, s_exponents[nth * 8 + 4 + w] = ev;
-                            mbar_arrive(&exponents_ready[nth]);
-                        }
+                    int ev = __reduce_max_sync(kFullMask, scale_exponent(v)), own_e = ev;
+                    float own = v;
+                    if (which == 0) own_e = __reduce_max_sync(kFullMask, scale_exponent(k)), own = k;
+                    if (__builtin_expect(entry & 8, 0)) {   // the last few steps of a row tile: are they bare codes?
+                        const auto apart = [](float scale, int e, float least) {
+                            const float unit = scale * __int_as_float((127 - e) << 23);
+                            return __any_sync(kFullMask, unit > 0.0f && unit < least);
+                        };
+                        const bool v_bare = apart(v, ev, 0x1p-4f), bare = which == 0 ? apart(k, own_e, 0x1p-13f) : v_bare;
+                        if (v_bare) ev = kBareCodes;
+                        if (bare) own_e = kBareCodes, own = own > 0.0f ? 1.0f : 0.0f;
+                        if (which == 0 && !(v < INFINITY) && lane < ROWS) sc[0] = __int_as_float(0x7fc00000), sc[N] = 0.0f;   // (as the softmax reads them)
+                        __syncwarp();
                     }
+                    if (which == 0 && lane == 0 && half == 0) {
+                        s_exponents[nth * 8 + w] = own_e, s_exponents[nth * 8 + 4 + w] = ev;
+                        mbar_arrive(&exponents_ready[nth]);
+                    }
+                    float unit = own * __uint_as_float((uint32_t)(127 - own_e) << 23);   // (times 1 for bare codes)
                     if (!(v < INFINITY)) unit = which == 0 ? __int_as_float(0x7fc00000) : 0.0f;
                     const uint32_t by = pack_f16x2(unit, unit);
                     __syncwarp();   // (every lane has its codes)
@@ -630,8 +723,8 @@ attn_chunk_kernel(AttnArgs a) {
                 mbar_arrive(&full[slot]);
             }
         };
-        // tile `which` (0: K, 1: V) of the step whose cache rows are row32
-        auto fetch = [&](int which, int row32) {
+        // tile `which` (0: K, 1: V) of the step whose cache rows are row32, some of which the mask hides from some row, or not
+        auto fetch = [&](int which, int row32, bool hides) {
             const uint32_t nth = asked[which]++, slot = which * SLOTS + nth % SLOTS, parity = ((nth / SLOTS) & 1) ^ 1;
             uint8_t* tile = s_kv + slot * Sh::KV_BYTES;
             // While the slot is still being read, what has been asked for is handed over as it arrives.
@@ -660,7 +753,7 @@ attn_chunk_kernel(AttnArgs a) {
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
-            pending = pending << 4 | slot;
+            pending = pending << 4 | (hides ? 8u : 0u) | slot;
             if (++in_flight == DEPTH) hand_over(false);
         };
         for (; cur.left > 0; attn_advance<R, OV>(a, cur)) {
@@ -668,6 +761,7 @@ attn_chunk_kernel(AttnArgs a) {
             attn_segment<OV>(a, cur, begin, end);
             if (begin == end) continue;
             chunk_steps<D, FP8>(a, cur, begin, end, keys, from, to);
+            const int hides_from = chunk_hides_from<N>(a, cur.span, cur.tile * R);
             auto lookup = [&](int step) {
                 const int key = step * N + w * ROWS + (lane % ROWS);
                 return step < to && key < keys ? attn_cache_row(a, cur.seq, key) : -1;
@@ -678,12 +772,12 @@ attn_chunk_kernel(AttnArgs a) {
             for (int j = 0; j <= SBUF; ++j) rows_of[j] = lookup(from + j);
 #pragma unroll
             for (int j = 0; j < SBUF; ++j) {
-                if (from + j < to) fetch(0, rows_of[j]);
+                if (from + j < to) fetch(0, rows_of[j], from + j >= hides_from);
             }
             for (int step = from; step < to; ++step) {
                 const int ahead = lookup(step + SBUF + 1);
-                fetch(1, rows_of[0]);
-                if (step + SBUF < to) fetch(0, rows_of[SBUF]);
+                fetch(1, rows_of[0], step >= hides_from);
+                if (step + SBUF < to) fetch(0, rows_of[SBUF], step + SBUF >= hides_from);
 #pragma unroll
                 for (int j = 0; j < SBUF; ++j) rows_of[j] = rows_of[j + 1];
                 rows_of[SBUF] = ahead;

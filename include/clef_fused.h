@@ -260,9 +260,12 @@ int clef_embed_rms_norm_quantise_nvfp4(clef_stream_t stream, const void* table, 
  * Lengths are read on the device and clamped to the shapes (kv_len to table_width * page_size, q_start to total_q). q and
  * the softmax weights enter the products as bf16 (f16 over an FP8 cache), everything is summed in f32. Keys past kv_len are
  * never read. A key that the causal mask hides from a row has weight exactly 0, but in a bf16 cache its value still enters
- * the row's product: values of the new tokens must be finite there. Scales of an FP8 cache are not negative; a head row
- * whose scale is NaN makes NaN of the rows that see it, and of no other, and values more than 2^24 below the largest of
- * their sequence count as zeros. head_dim 64, 128 or 256; at most 64 query heads per kv head.
+ * the row's product: values of the new tokens must be finite there. Scales of an FP8 cache are finite and not negative,
+ * or NaN; a head row whose scale is NaN makes NaN of the rows that see it, and of no other. Scales may lie far apart, and
+ * keys that the mask hides have no part in what follows: weight times value scale enters the product in f16 under the
+ * largest value scale that the row sees, so it loses bits from 2^-9 of that on and counts as zero from 2^-20 on; and in
+ * chunks a key whose scale is below 2^-14 of the largest among keys 16 j .. 16 j + 15 of its sequence that are seen with
+ * it loses bits, and counts as zero from 2^-25 on. head_dim 64, 128 or 256; at most 64 query heads per kv head.
  * workspace: clef_paged_attention_workspace bytes, 16-byte aligned, contents arbitrary; two calls that may run at the
  * same time need two of them. Results do not depend on timing. */
 int clef_paged_attention_workspace(int n_seqs, int total_q, int q_heads, int kv_heads, int head_dim, size_t* bytes);

@@ -38,8 +38,10 @@ def check(p, out):
     assert (err <= BOUND * most).all(), f"off by {worst:.3g} of the largest value that the row sees, allowed {BOUND:.3g}"
 
 
-# the last tokens' 16 keys begin inside and at a tile's end
-BATCHES = {"two_tokens": [(2, 60)], "four_tokens": [(4, 64), (4, 140)], "five_tokens": [(5, 33)]}
+# two, four and five tokens go to the kernel for few rows, the others to the one for chunks; the last tokens' 16 keys begin
+# inside, at, and before a tile's end
+BATCHES = {"two_tokens": [(2, 60)], "four_tokens": [(4, 64), (4, 140)], "five_tokens": [(5, 33)], "chunk": [(40, 100)], "prompt": [(150, 150)],
+           "edges": [(33, 129), (20, 64), (17, 17)]}
 
 
 @pytest.mark.parametrize("power", [6, 12, 16, 20, 24, 40])
@@ -85,7 +87,7 @@ def test_keys_without_a_value_beside_large_ones_still_weigh(cuda_dev, lens, head
 
 
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
-@pytest.mark.parametrize("lens", [[(1, 150)], [(3, 150)]], ids=["token", "tokens"])
+@pytest.mark.parametrize("lens", [[(1, 150)], [(3, 150)], [(40, 150)], [(150, 150)]], ids=["token", "tokens", "chunk", "prompt"])
 def test_every_key_on_a_scale_of_its_own(cuda_dev, lens, head_dim):
     """Scales of K and V that rise along the sequence from 2^-20 to 2^20, up and down by 2^6 from key to key."""
     p = Problem(lens, (8, 2), head_dim, 16, True, seed=head_dim)
