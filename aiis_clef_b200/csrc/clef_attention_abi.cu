@@ -192,6 +192,10 @@ int clef_paged_attention(clef_stream_t stream, void* out, const void* q, const v
     if (!aligned(out, 16) || !aligned(q, 16) || !aligned(cache_k, 16) || !aligned(cache_v, 16) || !aligned(workspace, 16)) {
         return fail(CLEF_ERR_INVALID, "%s: out, q, caches and workspace must be 16-byte aligned", what);
     }
+    if (!aligned(page_table, 4) || !aligned(q_start, 4) || !aligned(kv_len, 4) ||
+        (cache_dtype == CLEF_E4M3 && (!aligned(k_scales, 4) || !aligned(v_scales, 4)))) {
+        return fail(CLEF_ERR_INVALID, "%s: scales, page table and lengths must be 4-byte aligned", what);
+    }
     const AttnPlan plan = attn_plan(n_seqs, total_q, q_heads, kv_heads, head_dim, cache_dtype == CLEF_E4M3);
     if (workspace_bytes < plan.bytes) {
         return fail(CLEF_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, plan.bytes);

@@ -77,6 +77,10 @@ int kv_write_impl(const char* what, clef_stream_t stream, KvWriteArgs a, bool wi
         !aligned(a.k_scales, 4) || !aligned(a.v_scales, 4) || !aligned(a.weight, 4)) {
         return fail(CLEF_ERR_INVALID, "%s: activations and tables must be 16-byte aligned, codes 8-byte", what);
     }
+    if (!aligned(a.seq_start, 4) || !aligned(a.pos_base, 4) || !aligned(a.pos_map, 4) || !aligned(a.cache_map, 4) ||
+        !aligned(a.cache_len, 4)) {
+        return fail(CLEF_ERR_INVALID, "%s: positions and maps must be 4-byte aligned", what);
+    }
     const long long per_token = (long long)a.q_heads + 2LL * a.kv_heads;
     // the grid-stride counter advances past the last head row by up to one grid of them
     if (per_token * a.tokens >= 0x40000000LL) return fail(CLEF_ERR_TOO_LARGE, "%s: %d tokens x %lld head rows", what, a.tokens, per_token);
@@ -138,8 +142,8 @@ int clef_kv_read_fp8(clef_stream_t stream, void* k_out, void* v_out, const uint8
     if (rows == 0) return CLEF_OK;
     if (!k_out || !v_out || !cache_k || !cache_v || !k_scales || !v_scales) return fail(CLEF_ERR_INVALID, "%s: null pointer", what);
     if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(cache_k, 8) || !aligned(cache_v, 8) || !aligned(k_scales, 4) ||
-        !aligned(v_scales, 4)) {
-        return fail(CLEF_ERR_INVALID, "%s: outputs must be 16-byte aligned, codes 8-byte", what);
+        !aligned(v_scales, 4) || !aligned(row_map, 4)) {
+        return fail(CLEF_ERR_INVALID, "%s: outputs must be 16-byte aligned, codes 8-byte, scales and the map 4-byte", what);
     }
     const unsigned long long head_rows = (unsigned long long)rows * kv_heads;
     if (head_rows >= 0x7fffffffull || head_rows * (head_dim / 8) >= 0x7fffffffull) {
