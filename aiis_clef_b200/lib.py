@@ -506,6 +506,8 @@ class Device:
         self._operand(q, "q", q.dtype, 0)
         if min(q_heads, kv_heads, head_dim, page_size) <= 0:
             raise ClefError(f"q_heads {q_heads}, kv_heads {kv_heads}, head_dim {head_dim} and page_size {page_size} must be positive")
+        if q.numel() % (q_heads * head_dim):
+            raise ClefError(f"q must hold whole rows of {q_heads} x {head_dim}, got {tuple(q.shape)}")
         n_seqs, total_q = kv_len.numel(), q.numel() // (q_heads * head_dim)
         if page_table.dim() != 2 or page_table.shape[0] != n_seqs or q_start.numel() != n_seqs + 1:
             raise ClefError(f"page_table {tuple(page_table.shape)} and q_start {tuple(q_start.shape)} must be [n_seqs, width] "
