@@ -1,5 +1,6 @@
 """The FP8 cache's writers at their edges: padding tokens whose positions lie outside the tables, tables too short for the
-positions a call stands for. Bytes are compared as in test_gpu_kv_cache_fp8.py."""
+positions a call stands for, passes so large that a warp takes two groups of head rows. Bytes are compared as in
+test_gpu_kv_cache_fp8.py."""
 import pytest
 import torch
 
@@ -89,3 +90,46 @@ def test_tables_too_short_for_the_default_positions_are_refused(cuda_dev):
     torch.cuda.synchronize()
     code, scale = recipe(x.float())
     assert torch.equal(cache[1][:tokens], code) and torch.equal(cache[3][:tokens], scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("tokens,qh,kvh,dim,rotary", [(9001, 3, 1, 64, 32), (9001, 5, 2, 48, 16), (3001, 6, 2, 128, 64), (3001, 5, 2, 96, 96),
+                                                      (1501, 5, 1, 256, 64), (1203, 4, 3, 192, 0), (3203, 1, 1, 256, 256)])
+def test_full_passes(cuda_dev, tokens, qh, kvh, dim, rotary, dtype):
+    """Passes of so many head rows that a warp takes two groups of them (4,736 warps and more on 148 SMs): head counts that leave the
+    last group of a token short, and groups that hold rows of q and of k, or of k and of v."""
+    g = gen(tokens + dim)
+    q, k, v = (torch.randn(tokens, h, dim, generator=g, device="cuda").to(dtype) for h in (qh, kvh, kvh))
+    per_warp = 32 // (4 if dim <= 64 else 8 if dim <= 128 else 16)
+    assert tokens * (qh + 2 * kvh) // per_warp >= torch.cuda.get_device_properties(0).multi_processor_count * 32
+    cos, sin = tables(tokens, max(rotary, 2))
+    pos = torch.randperm(tokens, generator=g, device="cuda").to(torch.int32)
+    where = torch.randperm(tokens + 7, generator=g, device="cuda")[:tokens].to(torch.int32)
+    skipped = torch.arange(0, tokens, 97, device="cuda")
+    where[skipped] = -1
+    keep = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    keep[skipped] = False
+    cache, q_out = Cache(tokens + 7, kvh, dim), Guarded(q.numel() * q.element_size())
+    call("clef_rope_qkv_write_fp8", stream(), q_out.ptr, ptr(q), qh, *cache.pointers(), ptr(k), ptr(v), kvh, ptr(cos), ptr(sin), tokens, dim,
+         rotary, None, None, ptr(pos), ptr(where), None, tokens + 7, 0 if dtype == torch.bfloat16 else 1)
+    torch.cuda.synchronize()
+    q_out.check_guards("q_out")
+    want_q = cuda_dev.rope_apply_dev(q, cos, sin, tokens, qh, dim, rotary, pos_map=pos) if rotary else q
+    turned = cuda_dev.rope_apply_dev(k.float(), cos, sin, tokens, kvh, dim, rotary, pos_map=pos) if rotary else k.float()
+    assert torch.equal(q_out.payload().view(dtype).view(q.shape), want_q)
+    cache.check(where[keep].long(), turned[keep], v[keep].float())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("tokens,kvh,dim,rotary", [(20001, 1, 64, 64), (9001, 3, 128, 32), (9001, 1, 256, 64)])
+def test_full_passes_without_q(cuda_dev, tokens, kvh, dim, rotary, dtype):
+    g = gen(tokens + dim)
+    k, v = (torch.randn(tokens, kvh, dim, generator=g, device="cuda").to(dtype) for _ in range(2))
+    per_warp = 32 // (4 if dim <= 64 else 8 if dim <= 128 else 16)
+    assert tokens * 2 * kvh // per_warp >= torch.cuda.get_device_properties(0).multi_processor_count * 32
+    cos, sin = tables(tokens, rotary)
+    cache = Cache(tokens, kvh, dim)
+    call("clef_rope_kv_write_fp8", stream(), *cache.pointers(), ptr(k), ptr(v), ptr(cos), ptr(sin), tokens, kvh, dim, rotary, None, None, None,
+         None, None, tokens, 0 if dtype == torch.bfloat16 else 1)
+    torch.cuda.synchronize()
+    cache.check(torch.arange(tokens, device="cuda"), cuda_dev.rope_apply_dev(k.float(), cos, sin, tokens, kvh, dim, rotary), v.float())
