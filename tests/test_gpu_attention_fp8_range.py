@@ -29,13 +29,13 @@ def most_seen(p):
     return most
 
 
-def check(p, out):
+def check(p, out, bound=BOUND):
     want, _ = p.want()
     most = most_seen(p)
     err = (out.cpu().double()[:p.tokens] - want).abs()
     assert torch.isfinite(out).all()
     worst = (err / most.clamp(min=1e-300)).max().item()
-    assert (err <= BOUND * most).all(), f"off by {worst:.3g} of the largest value that the row sees, allowed {BOUND:.3g}"
+    assert (err <= bound * most).all(), f"off by {worst:.3g} of the largest value that the row sees, allowed {bound:.3g}"
 
 
 # two, four and five tokens go to the kernel for few rows, the others to the one for chunks; the last tokens' 16 keys begin
@@ -98,3 +98,19 @@ def test_every_key_on_a_scale_of_its_own(cuda_dev, lens, head_dim):
         values[p.rows[0]] *= rise[:, None, None].double()
     p.q = (p.q.float() * 2.0 ** -26).to(p.q.dtype)        # scores stay moderate
     check(p, p.run(cuda_dev))
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("heads", [(16, 2), (4, 4)])
+def test_long_chunks_on_scales_far_apart(cuda_dev, heads, head_dim):
+    """Chunks cut over many CTAs, every scale a random power of two up to 2^30: 2,500 keys instead of the 160 that the bound at the
+    top counts with, 2^-19 each, add 2^-7.7 at the very most."""
+    p = Problem([(600, 2500), (1, 900), (300, 300)], heads, head_dim, 16, True, seed=heads[0])
+    g = torch.Generator().manual_seed(head_dim)
+    for scales, values in ((p.ks, p.k64), (p.vs, p.v64)):
+        factor = torch.exp2(torch.randint(0, 31, scales.shape, generator=g).float())
+        for rows in p.rows:
+            scales[rows] *= factor[rows]
+            values[rows] *= factor[rows][..., None].double()
+    p.q = (p.q.float() * 2.0 ** -30).to(p.q.dtype)
+    check(p, p.run(cuda_dev), BOUND + 2.0 ** -7.7)
