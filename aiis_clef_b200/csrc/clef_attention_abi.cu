@@ -27,8 +27,9 @@ struct AttnPlan {
 };
 
 // attn_rows_kernel up to an average of `most` rows per (sequence, kv head), attn_chunk_kernel above. At 32 rows of 8,192
-// keys, 32 sequences: bf16 57 us in rows of 16, 53 us in chunks; FP8 51 against 70 us. Two groups of 8 rows of 256 bf16
-// dims do not fit the registers (16 rows: 143 us, in chunks 84 us).
+// keys, 32 sequences: bf16 57 us in rows of 16, 53 us in chunks; FP8 53 against 70 us. Two groups of 8 rows of 256 bf16
+// dims do not fit the registers (16 rows: 143 us, in chunks 84 us). Measured with equal rows in all sequences, the limit for
+// FP8 at 128 dims alone: a batch of many single tokens and one chunk goes to one of the two whatever its parts would take.
 AttnPlan attn_plan(int n_seqs, int total_q, int q_heads, int kv_heads, int head_dim, bool fp8) {
     AttnPlan p;
     const long long rows = (long long)total_q * (q_heads / kv_heads);

@@ -17,12 +17,16 @@
 // 2^13 (K) or 2^4 (V) are multiplied as bare codes there, and the softmax takes their scales one by one, those of K with the
 // scores, those of V, against the largest that its row sees, with the weights.
 //
-// Measured (16 + 2 heads of 128, pages of 64): 8,192 causal tokens 291 to 303 us = 945 to 907 TFLOP/s; 2,011 tokens after
-// 30,757 in FP8 605 us = 865 TFLOP/s; head_dim 256, FP8, 2,048 tokens after 6,144: 375 us. What bounds it: the softmax's
-// chain of latencies. A step of 64 keys takes 2,150 clocks; its products fill the tensor pipe for about 1,280 of them (at 64 keys
+// Measured with the join (16 + 2 heads of 128, pages of 64), in 20 calls behind each other and in a long stream of calls, where
+// the card holds a lower clock: 8,192 causal tokens 275 to 282 and 308 us = 1,000 and 893 TFLOP/s; 2,011 tokens after 30,757 in
+// FP8 600 and 653 us = 872 and 802 TFLOP/s; head_dim 256, FP8, 2,048 tokens after 6,144: 375 us = 642 TFLOP/s in the former. What
+// bounds it: the softmax's chain of latencies. When 8,192 tokens took 299 us a step of 64 keys took 2,150 clocks; its products
+// filled the tensor pipe for about 1,280 of them (at 64 keys
 // the scores' operands come out of shared memory at less than the pipe's rate) and its exponentials their units for
-// 1,060, but a thread's way from scores to weights (barrier, load, maximum, fma, exp2, sum, pack, store) is some 1,800 clocks
-// alone, and only two warps on each quarter of the SM share it out. Not kept, prefill in us against 299: 128 keys a step with
+// 1,060, but a thread's way from scores to weights (barrier, load, maximum, fma, exp2, sum, pack, store) was some 1,800 clocks
+// alone, and only two warps on each quarter of the SM share it out. The step compiled apart for steps that hide keys: 282 us
+// from 295, for FP8 no change where contexts are long and 2 to 4 us more for prompts of 2,048 (35.7 from 31.7 us with 8 + 8 heads),
+// where the larger kernel is fetched and bare codes are looked for. Not kept, prefill in us against 299: 128 keys a step with
 // one S buffer 325 (the long FP8 case gained 6 %, FP8 prompts of 2,048 lost 13 %), the row blocks' exponentials in turns 297,
 // weights against the last reference with the maximum beside them 305, one arrival per warp on the barriers 313,
 // a quarter of the exponentials as polynomials 297.

@@ -10,8 +10,8 @@
 // to a power of two); nothing is exchanged but the row maximum. A warp takes U groups of 32 / G head rows of ONE token,
 // requested together: a lane's columns, and with them its cosines and sines, are the same in all of them, and the chain
 // position -> table runs beside the rows' own loads. With the per-head norm (k rows only) a lane takes 8 consecutive
-// values instead, the order of the sum. Measured: 8,192 tokens of 16 + 2 heads of 128 (84 MB) 17.0 us = 4.9 TB/s (a lane
-// of 8 values with its partner fetched by shuffles: 22.4 us).
+// values instead, the order of the sum. Measured: 8,192 tokens of 16 + 2 heads of 128 (84 MB) 18.7 us a call in a stream of
+// calls = 4.5 TB/s, 17.2 us under a profiler, alone (a lane of 8 values with its partner fetched by shuffles: 22.4 us).
 #pragma once
 
 #include "kernels_generic.cuh"
@@ -301,7 +301,7 @@ kv_norm_write_fp8_kernel(KvWriteArgs a) {
 // back as zeros. A lane takes CODES of a row's k and the same of its v (16 where head_dim allows: 16-byte loads, 32 bytes
 // out), so that the way from the row number to the codes is walked once for both, and each thread has one piece: with
 // full occupancy that streamed better than several pieces a thread. Bound by HBM bytes: 130,712 rows of 2 x 128 to bf16
-// (204 MB) 30.4 us = 6.7 TB/s.
+// (204 MB) 33.5 us a call in a stream of calls = 6.1 TB/s (30.1 us under a profiler, alone).
 template <typename T, int CODES>
 __global__ void __launch_bounds__(kCtaThreads)
 kv_read_fp8_kernel(typename T::storage* __restrict__ k_out, typename T::storage* __restrict__ v_out,

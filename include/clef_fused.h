@@ -276,8 +276,9 @@ int clef_paged_attention(clef_stream_t stream, void* out, const void* q, const v
                          size_t workspace_bytes, int cache_dtype, int dtype);
 
 /* The FP8 cache: rows of kv_heads * head_dim E4M3 codes, and one f32 scale per row and head ([cache_rows, kv_heads]). A
- * head row is stored as scale = max |x| / 448 and codes of x / scale, rounded to nearest even, where x is the f32 value
- * that the bf16 cache would round; code * scale is what it stands for. A head row whose maximum is below 2^-100 is
+ * head row is stored as scale = max |x| / 448 and codes of x * (1 / scale), rounded to nearest even, where x is the f32
+ * value that the bf16 cache would round and the reciprocal and the product are rounded to f32 (codes next to a tie may be a
+ * step from those of x / scale); code * scale is what it stands for. A head row whose maximum is below 2^-100 is
  * stored as zeros (scale 0); one that holds an infinity or a NaN as scale NaN. Codes never hold a NaN. No counterpart in
  * the reference, whose cache is bf16.
  *
