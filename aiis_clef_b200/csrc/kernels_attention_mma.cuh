@@ -565,6 +565,9 @@ attn_chunk_kernel(AttnArgs a) {
                 mbar_arrive(&p_ready[t * SBUF + buf]);
                 ++steps_done;
             };
+            // A row block that had no row in the last row tiles is ahead of the keys: the phase of the exponents that it would wait for
+            // could be taken for an older one of the same parity. Once the scores of its first step are there, so are the exponents.
+            if (FP8) mbar_wait_warp(&s_ready[t * SBUF + (SBUF == 1 ? 0 : (steps_done & 1))], (SBUF == 1 ? steps_done : steps_done >> 1) & 1, gave_up);
             if (warp_live) {
                 const int hides_from = min(to, max(from, chunk_hides_from<N>(a, span, cur.tile * R)));
 #pragma unroll 1

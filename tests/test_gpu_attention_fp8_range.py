@@ -114,3 +114,18 @@ def test_long_chunks_on_scales_far_apart(cuda_dev, heads, head_dim):
             values[rows] *= factor[rows][..., None].double()
     p.q = (p.q.float() * 2.0 ** -30).to(p.q.dtype)
     check(p, p.run(cuda_dev), BOUND + 2.0 ** -7.7)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("short", [600, 1100, 1700, 3000])
+def test_row_tiles_with_and_without_a_second_block_in_turn(cuda_dev, short, head_dim):
+    """So many row tiles that a CTA takes several behind each other: of 100 rows (one block of 128, up to 47 steps of 64 keys) and of
+    256 (two blocks). The second block has nothing to do in the former and is ahead of the keys when it comes to the latter."""
+    p = Problem([(100, short), (256, 700)] * 24, (8, 8), head_dim, 64, True, seed=short)
+    g = torch.Generator().manual_seed(short)
+    for scales, values in ((p.ks, p.k64), (p.vs, p.v64)):     # every sixteen keys under an exponent of their own
+        for rows in p.rows:
+            factor = torch.exp2(torch.randint(-6, 1, (len(rows) // 16 + 1,), generator=g).float()).repeat_interleave(16)[:len(rows)]
+            scales[rows] *= factor[:, None]
+            values[rows] *= factor[:, None, None].double()
+    check(p, p.run(cuda_dev), BOUND + 2.0 ** -7.4)
